@@ -215,6 +215,55 @@ int b200_kv_append(const void* k_new, const void* v_new, void* k_pool, void* v_p
                    int batch, int num_kv_heads, int head_dim, int page_size, int num_blocks,
                    int max_pages_per_seq, int dtype, void* stream);
 
+/* ------------------------------------------------------ 8-bit page cache -- */
+
+/*
+ * Keys and values in 8 bits (no counterpart in the reference, whose cache is 16 bits wide: kv_cache/block_manager.py:33-49):
+ *
+ *   k_pool/v_pool   [num_blocks, num_kv_heads, 16, head_dim] e4m3, head_dim 64 or 128, 16-byte aligned
+ *   k_scale/v_scale [num_blocks, num_kv_heads] bytes: the numbers of a page and kv head stand for themselves times 2^(byte - 127)
+ *                   (e8m0).  Exponents go from -32 to 31; a byte beyond is taken for the nearest.
+ *
+ * b200_kv_slot_map: slots of new tokens from request lengths, pages for them from a list of free ones.
+ *   ctx_lens, new_lens [num_seqs]   tokens that a sequence has, and gets
+ *   block_table [num_seqs, max_pages_per_seq]  page ids; the first ceil(ctx / 16) of a row are read where new tokens go there, the
+ *                        fresh ones behind them are written, all others left as they were
+ *   supply [supply_len]  free page ids, handed out in order from entry *supply_used on, to the sequences in their order
+ *   lens [num_seqs]      ctx + new;  row_start [num_seqs + 1] first row of every sequence, and the sum
+ *   row_seq, positions, slots [num_rows]  of every new token, sequence by sequence: its sequence, its position, and page * 16 +
+ *                        position % 16.  Rows behind the last token: -1, 0, -1.
+ *   supply_used_out [1]  entries of the supply that are used now
+ * Findings (status word, optional): a sequence with a negative length or more tokens than its table row gets nothing; more tokens
+ * than num_rows; fewer free pages than needed or a page id outside [0, num_blocks): slots of -1.  At most 4096 sequences and fewer
+ * than 2^31 tokens in the table.  lens and supply_used_out must not be inputs.
+ *
+ * b200_kv8_append: rows of keys and values (bf16 or fp32; [num_rows, num_kv_heads, head_dim] with a row stride in elements) into
+ * their slots; a negative slot is no slot.  Rows that go to one page stand side by side, in rising order and without gaps, and the page is no other
+ * sequence's: two groups of rows of one page in a call race for its scale.  Naming a slot twice in a row keeps the last.
+ * The scale of a page becomes the smallest 2^e with largest finite magnitude <= 448 * 2^e; that of a page whose first slot is not
+ * among the rows never falls, and where it grows, the rows ahead of the new ones are rounded again.  Slots behind the new ones
+ * are left as they were.  Numbers are rounded to nearest even; infinities and NaN become NaN.
+ *
+ * b200_kv8_attn_decode: softmax(q K^T * scale) V, one query row per sequence over its pages.  q, out [batch, num_q_heads, head_dim] bf16, any
+ * number of query heads per kv head.  scale > 0.  workspace: b200_kv8_attn_workspace_bytes bytes, 16-byte aligned, starting with the status word;
+ * calls that share it must not overlap.  split_tokens: tokens per CTA, a multiple of 16; 0: the library's choice, the same for
+ * both calls.  A row without tokens is zero.  Pages behind a row's last token are not read, and what the last page
+ * holds behind it does not matter, NaN included.
+ */
+int b200_kv_slot_map(const int32_t* ctx_lens, const int32_t* new_lens, int32_t* block_table, const int32_t* supply,
+                     const int32_t* supply_used, int supply_len, int32_t* lens, int32_t* row_start, int32_t* row_seq,
+                     int32_t* positions, int32_t* slots, int32_t* supply_used_out, void* status_word, int num_seqs, int num_rows,
+                     int num_blocks, int max_pages_per_seq, void* stream);
+int b200_kv8_append(const void* k_new, const void* v_new, int64_t k_row_stride, int64_t v_row_stride, void* k_pool, void* v_pool,
+                    void* k_scale, void* v_scale, const int32_t* slots, void* status_word, int num_rows, int num_kv_heads, int head_dim,
+                    int num_blocks, int dtype, void* stream);
+size_t b200_kv8_attn_workspace_bytes(int batch, int num_q_heads, int num_kv_heads, int head_dim, int max_pages_per_seq,
+                                     int split_tokens);
+int b200_kv8_attn_decode(const void* q, const void* k_pool, const void* v_pool, const void* k_scale, const void* v_scale,
+                         const int32_t* block_table, const int32_t* ctx_lens, void* out, void* workspace, size_t workspace_bytes,
+                         int batch, int num_q_heads, int num_kv_heads, int head_dim, int num_blocks, int max_pages_per_seq, float scale,
+                         int split_tokens, void* stream);
+
 /* ----------------------------------------------------- dense projections -- */
 
 /*

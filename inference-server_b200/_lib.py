@@ -9,7 +9,7 @@ from __future__ import annotations
 
 import ctypes
 import os
-from ctypes import c_char_p, c_float, c_int, c_size_t, c_void_p
+from ctypes import c_char_p, c_float, c_int, c_int64, c_size_t, c_void_p
 
 _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(_HERE, "libb200decode.so")
@@ -35,6 +35,10 @@ SIGNATURES = {
     "b200_paged_attn_prefill": (c_int, [c_void_p] * 6 + [c_int] * 8 + [c_float, c_void_p]),
     "b200_paged_attn_decode_static": (c_int, [c_void_p] * 7 + [c_int] * 7 + [c_float, c_int, c_void_p]),
     "b200_kv_append": (c_int, [c_void_p] * 7 + [c_int] * 7 + [c_void_p]),
+    "b200_kv_slot_map": (c_int, [c_void_p] * 5 + [c_int] + [c_void_p] * 7 + [c_int] * 4 + [c_void_p]),
+    "b200_kv8_append": (c_int, [c_void_p] * 2 + [c_int64] * 2 + [c_void_p] * 6 + [c_int] * 5 + [c_void_p]),
+    "b200_kv8_attn_workspace_bytes": (c_size_t, [c_int] * 6),
+    "b200_kv8_attn_decode": (c_int, [c_void_p] * 9 + [c_size_t] + [c_int] * 6 + [c_float, c_int, c_void_p]),
     "b200_dense_gemm_workspace_bytes": (c_size_t, [c_int, c_int]),
     "b200_dense_gemm_row_tile": (c_int, [c_int] * 3),
     "b200_dense_gemm_bf16": (c_int, [c_void_p] * 4 + [c_size_t, c_void_p] + [c_int] * 4 + [c_void_p]),

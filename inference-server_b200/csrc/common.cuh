@@ -33,6 +33,7 @@ enum : int {
   kErrDevWaitTimeout = 18,  // a bounded mbarrier wait ran out
   kErrDevBadExpert = 19,    // expert id outside [0, E)
   kErrDevPeerTimeout = 20,  // a bounded wait for another rank's flag ran out
+  kErrDevNoPages = 21,      // fewer free pages than the new tokens need
 };
 
 // Peer receive buffers of the expert-parallel dispatch, one entry per rank (this rank included); all null

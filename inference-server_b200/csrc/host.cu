@@ -285,6 +285,7 @@ extern "C" const char* b200_strerror(int code) {
     case kErrDevWaitTimeout: return "device: a bounded barrier wait ran out";
     case kErrDevBadExpert: return "device: expert id outside [0, num_experts)";
     case kErrDevPeerTimeout: return "device: a bounded wait for another rank's flag ran out";
+    case kErrDevNoPages: return "device: fewer free pages than the new tokens need";
     default: return "unknown error";
   }
 }

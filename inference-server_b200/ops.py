@@ -7,6 +7,8 @@ the library, or off a CUDA device, the calls raise.
 """
 from __future__ import annotations
 
+from typing import NamedTuple
+
 import torch
 
 from . import _lib
@@ -182,6 +184,152 @@ def kv_append(k_new, v_new, k_pool, v_pool, block_table, positions, status: torc
         _ptr(status), B, Hkv, D, page, nb, block_table.shape[1], DTYPE_CODE[k_pool.dtype], _stream(),
     )
     check(rc, "b200_kv_append")
+
+
+# ---------------------------------------------------------- 8-bit page cache
+
+KV8_DTYPE, KV8_SCALE_DTYPE = torch.float8_e4m3fn, torch.float8_e8m0fnu
+
+
+class KvSlotMap(NamedTuple):
+    """What `kv_slot_map` makes of request lengths: lengths with the new tokens [B], first row per sequence [B + 1], per new token
+    its sequence, position and slot [num_rows], and the used entries of the supply [1]; all int32."""
+    lens: torch.Tensor
+    row_start: torch.Tensor
+    row_seq: torch.Tensor
+    positions: torch.Tensor
+    slots: torch.Tensor
+    supply_used: torch.Tensor
+
+
+def _on_current_device(t: torch.Tensor, *others: torch.Tensor) -> None:
+    """The kernels run on the current device's current stream: operands of another device are an error and not a fault."""
+    device = t.device
+    if device.index != torch.cuda.current_device():
+        raise ValueError(f"operands are on {device}, the current device is cuda:{torch.cuda.current_device()}")
+    for o in others:
+        if o.device != device:
+            raise ValueError(f"operands are on {device} and {o.device}")
+
+
+def _status_word(status: torch.Tensor | None) -> None:
+    if status is not None:
+        _need(status, "status")
+        if status.numel() * status.element_size() < 4:
+            raise ValueError("status holds less than a 4-byte word")
+
+
+def kv8_pools(num_blocks: int, num_kv_heads: int, head_dim: int, device="cuda"):
+    """Pools of an 8-bit page cache, all zeros: (k_pool, v_pool, k_scale, v_scale)."""
+    pools = [torch.zeros(num_blocks, num_kv_heads, 16, head_dim, dtype=torch.uint8, device=device).view(KV8_DTYPE) for _ in range(2)]
+    scales = [torch.full((num_blocks, num_kv_heads), 95, dtype=torch.uint8, device=device).view(KV8_SCALE_DTYPE) for _ in range(2)]
+    return *pools, *scales
+
+
+def _kv8_cache(k_pool, v_pool, k_scale, v_scale) -> tuple[int, int, int]:
+    _need(k_pool, "k_pool", KV8_DTYPE)
+    _need(v_pool, "v_pool", KV8_DTYPE)
+    _need(k_scale, "k_scale", KV8_SCALE_DTYPE)
+    _need(v_scale, "v_scale", KV8_SCALE_DTYPE)
+    if k_pool.dim() != 4 or k_pool.shape[2] != 16:
+        raise ValueError(f"k_pool must be [num_blocks, kv_heads, 16, head_dim], got {list(k_pool.shape)}")
+    nb, Hkv, _, D = k_pool.shape
+    if v_pool.shape != k_pool.shape or k_scale.shape != (nb, Hkv) or v_scale.shape != (nb, Hkv):
+        raise ValueError("pools and scales do not match each other")
+    return nb, Hkv, D
+
+
+def kv_slot_map(ctx_lens, new_lens, block_table, supply, supply_used, num_rows: int, num_blocks: int,
+                status: torch.Tensor | None = None) -> KvSlotMap:
+    """Where the new tokens of a pass go, worked out on the GPU: sequence b has ctx_lens[b] tokens and gets new_lens[b] more.  Pages they
+    need are taken from `supply` [any], free page ids, from entry supply_used [1] on, and entered into block_table [B, max_pages] in
+    place.  `num_rows`: rows of the pass, at least the sum of new_lens; rows behind the last token get slot -1.  Slots are
+    page * 16 + position % 16, for `kv8_append` or any other cache of 16-token pages; page ids outside [0, num_blocks) are findings."""
+    for t, name in ((ctx_lens, "ctx_lens"), (new_lens, "new_lens"), (block_table, "block_table"), (supply, "supply"),
+                    (supply_used, "supply_used")):
+        _need(t, name, torch.int32)
+    _status_word(status)
+    _on_current_device(ctx_lens, new_lens, block_table, supply, supply_used)
+    B, R = ctx_lens.shape[0], int(num_rows)
+    if ctx_lens.dim() != 1 or new_lens.shape != ctx_lens.shape or block_table.dim() != 2 or block_table.shape[0] != B or supply_used.numel() != 1:
+        raise ValueError("lengths, block table or supply_used do not match")
+    if R < 0:
+        raise ValueError(f"{R} rows")
+    m = KvSlotMap(*torch.empty(2 * B + 2 + 3 * R, dtype=torch.int32, device=ctx_lens.device).split((B, B + 1, R, R, R, 1)))
+    rc = _lib.load().b200_kv_slot_map(
+        _ptr(ctx_lens), _ptr(new_lens), _ptr(block_table), _ptr(supply), _ptr(supply_used), supply.numel(), _ptr(m.lens),
+        _ptr(m.row_start), _ptr(m.row_seq), _ptr(m.positions), _ptr(m.slots), _ptr(m.supply_used), _ptr(status), B, R,
+        int(num_blocks), block_table.shape[1], _stream())
+    check(rc, "b200_kv_slot_map")
+    return m
+
+
+def kv8_append(k_new, v_new, k_pool, v_pool, k_scale, v_scale, slots, status: torch.Tensor | None = None) -> None:
+    """Write K/V rows [R, Hkv, D] (bf16 or fp32; rows may be strided, as slices of a fused projection are) into an 8-bit page cache.
+    slots [R] int32 = page * 16 + offset, as `kv_slot_map` gives them; negative: the row goes nowhere.  Rows of one page stand side
+    by side, in order.  The scale of a page is the smallest power of two for which its largest number fits; see the header
+    for how it grows."""
+    nb, Hkv, D = _kv8_cache(k_pool, v_pool, k_scale, v_scale)
+    _need(slots, "slots", torch.int32)
+    _status_word(status)
+    if k_new.dtype not in DTYPE_CODE or v_new.dtype != k_new.dtype:
+        raise ValueError(f"k_new and v_new must be bfloat16 or float32, got {k_new.dtype} and {v_new.dtype}")
+    R = slots.numel()
+    for t, name in ((k_new, "k_new"), (v_new, "v_new")):
+        if not t.is_cuda:
+            raise ValueError(f"{name} must be a CUDA tensor (this path has no CPU implementation)")
+        if t.shape != (R, Hkv, D):
+            raise ValueError(f"{name} must be [{R}, {Hkv}, {D}], got {list(t.shape)}")
+        if R > 0 and (t.stride(2) != 1 or (Hkv > 1 and t.stride(1) != D) or (R > 1 and t.stride(0) < Hkv * D)):
+            raise ValueError(f"{name} may be strided in its rows only")
+    _on_current_device(k_pool, v_pool, k_scale, v_scale, k_new, v_new, slots)
+    if R == 0:
+        return
+    rc = _lib.load().b200_kv8_append(
+        _ptr(k_new), _ptr(v_new), k_new.stride(0), v_new.stride(0), _ptr(k_pool), _ptr(v_pool), _ptr(k_scale), _ptr(v_scale),
+        _ptr(slots), _ptr(status), R, Hkv, D, nb, DTYPE_CODE[k_new.dtype], _stream())
+    check(rc, "b200_kv8_append")
+
+
+def kv8_attn_workspace(batch: int, num_q_heads: int, num_kv_heads: int, head_dim: int, max_pages: int, device,
+                       split_tokens: int = 0) -> torch.Tensor:
+    """Workspace of `kv8_attn_decode`, starting with the status word; kept for all steps of a batch shape."""
+    n = _lib.load().b200_kv8_attn_workspace_bytes(batch, num_q_heads, num_kv_heads, head_dim, max_pages, split_tokens)
+    return torch.zeros(n, dtype=torch.uint8, device=device)
+
+
+def kv8_attn_decode(q, k_pool, v_pool, k_scale, v_scale, block_table, ctx_lens, scale: float, split_tokens: int = 0,
+                    workspace: torch.Tensor | None = None, out: torch.Tensor | None = None) -> torch.Tensor:
+    """`paged_attn_decode` over an 8-bit page cache: softmax(q K^T * scale) V for one bf16 query row [B, Hq, D] per sequence; head_dim 64
+    or 128, any head grouping.  `split_tokens` 0: the library's choice."""
+    nb, Hkv, D = _kv8_cache(k_pool, v_pool, k_scale, v_scale)
+    _need(q, "q", torch.bfloat16)
+    _need(block_table, "block_table", torch.int32)
+    _need(ctx_lens, "ctx_lens", torch.int32)
+    if q.dim() != 3 or q.shape[2] != D:
+        raise ValueError(f"q must be [batch, heads, {D}], got {list(q.shape)}")
+    B, Hq, _ = q.shape
+    if block_table.dim() != 2 or block_table.shape[0] != B or ctx_lens.shape != (B,):
+        raise ValueError("block_table / ctx_lens batch mismatch")
+    if out is None:
+        out = torch.empty_like(q)
+    else:
+        _need(out, "out", torch.bfloat16)
+        if out.shape != q.shape:
+            raise ValueError("out does not match q")
+    _on_current_device(q, k_pool, v_pool, k_scale, v_scale, block_table, ctx_lens, out)
+    if B == 0:
+        return out
+    if workspace is None:
+        workspace = kv8_attn_workspace(B, Hq, Hkv, D, block_table.shape[1], q.device, int(split_tokens))
+    else:
+        _need(workspace, "workspace", torch.uint8)
+        _on_current_device(workspace)
+    rc = _lib.load().b200_kv8_attn_decode(
+        _ptr(q), _ptr(k_pool), _ptr(v_pool), _ptr(k_scale), _ptr(v_scale), _ptr(block_table), _ptr(ctx_lens), _ptr(out),
+        _ptr(workspace), workspace.numel(), B, Hq, Hkv, D, nb, block_table.shape[1], float(scale), int(split_tokens), _stream())
+    check(rc, "b200_kv8_attn_decode")
+    return out
 
 
 # ---------------------------------------------------------- dense projections
