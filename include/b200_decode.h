@@ -249,6 +249,10 @@ int b200_kv_append(const void* k_new, const void* v_new, void* k_pool, void* v_p
  * calls that share it must not overlap.  split_tokens: tokens per CTA, a multiple of 16; 0: the library's choice, the same for
  * both calls.  A row without tokens is zero.  Pages behind a row's last token are not read, and what the last page
  * holds behind it does not matter, NaN included.
+ *
+ * b200_kv8_attn_prefill: causal attention of num_tokens consecutive tokens of one sequence, at positions first_position .., whose keys
+ * and values are in their slots.  q, out [num_tokens, num_q_heads, head_dim] bf16, at most 128 query heads per kv head.  workspace:
+ * b200_kv8_attn_prefill_workspace_bytes bytes (the same rules).  A NaN value of a token reaches the rows of up to 127 tokens before it.
  */
 int b200_kv_slot_map(const int32_t* ctx_lens, const int32_t* new_lens, int32_t* block_table, const int32_t* supply,
                      const int32_t* supply_used, int supply_len, int32_t* lens, int32_t* row_start, int32_t* row_seq,
@@ -263,6 +267,11 @@ int b200_kv8_attn_decode(const void* q, const void* k_pool, const void* v_pool, 
                          const int32_t* block_table, const int32_t* ctx_lens, void* out, void* workspace, size_t workspace_bytes,
                          int batch, int num_q_heads, int num_kv_heads, int head_dim, int num_blocks, int max_pages_per_seq, float scale,
                          int split_tokens, void* stream);
+size_t b200_kv8_attn_prefill_workspace_bytes(int num_tokens, int first_position, int num_q_heads, int num_kv_heads, int head_dim);
+int b200_kv8_attn_prefill(const void* q, const void* k_pool, const void* v_pool, const void* k_scale, const void* v_scale,
+                          const int32_t* block_table_row, void* out, void* workspace, size_t workspace_bytes, int num_tokens,
+                          int first_position, int num_q_heads, int num_kv_heads, int head_dim, int num_blocks, int max_pages_per_seq,
+                          float scale, void* stream);
 
 /* ----------------------------------------------------- dense projections -- */
 

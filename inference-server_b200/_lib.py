@@ -39,6 +39,8 @@ SIGNATURES = {
     "b200_kv8_append": (c_int, [c_void_p] * 2 + [c_int64] * 2 + [c_void_p] * 6 + [c_int] * 5 + [c_void_p]),
     "b200_kv8_attn_workspace_bytes": (c_size_t, [c_int] * 6),
     "b200_kv8_attn_decode": (c_int, [c_void_p] * 9 + [c_size_t] + [c_int] * 6 + [c_float, c_int, c_void_p]),
+    "b200_kv8_attn_prefill_workspace_bytes": (c_size_t, [c_int] * 5),
+    "b200_kv8_attn_prefill": (c_int, [c_void_p] * 8 + [c_size_t] + [c_int] * 7 + [c_float, c_void_p]),
     "b200_dense_gemm_workspace_bytes": (c_size_t, [c_int, c_int]),
     "b200_dense_gemm_row_tile": (c_int, [c_int] * 3),
     "b200_dense_gemm_bf16": (c_int, [c_void_p] * 4 + [c_size_t, c_void_p] + [c_int] * 4 + [c_void_p]),

@@ -154,8 +154,9 @@ struct MapKey {
   int elem_bytes;
   uint32_t box[4];
   uint64_t stride[3];  // bytes, of dim[1..]
+  uint32_t swizzle = 128;  // bytes: 128 or 64, and the width of a box
   bool operator==(const MapKey& o) const {
-    if (base != o.base || device != o.device || elem_bytes != o.elem_bytes) return false;
+    if (base != o.base || device != o.device || elem_bytes != o.elem_bytes || swizzle != o.swizzle) return false;
     for (int i = 0; i < 4; ++i)
       if (dim[i] != o.dim[i] || box[i] != o.box[i] || (i < 3 && stride[i] != o.stride[i])) return false;
     return true;
@@ -211,7 +212,7 @@ static int get_tensor_map(int rank, MapKey key, CUtensorMap* out) {
     g_encode = reinterpret_cast<EncodeTiledFn>(fn);
   }
   const unsigned long long cols = key.dim[0], rows = key.dim[1];
-  if (key.box[0] * static_cast<uint32_t>(key.elem_bytes) != 128u || key.box[1] == 0 || key.box[1] > 256 || key.box[2] == 0 ||
+  if (key.box[0] * static_cast<uint32_t>(key.elem_bytes) != key.swizzle || key.box[1] == 0 || key.box[1] > 256 || key.box[2] == 0 ||
       key.box[2] > 256 || key.box[3] == 0 || key.box[3] > 256 || (reinterpret_cast<uintptr_t>(key.base) & 15) != 0 || key.stride[0] % 16 != 0) {
     set_detail("tensor map: base %p rows %llu cols %llu elem %d box %ux%ux%u is not encodable", key.base, rows, cols,
                key.elem_bytes, key.box[2], key.box[1], key.box[0]);
@@ -226,7 +227,7 @@ static int get_tensor_map(int rank, MapKey key, CUtensorMap* out) {
   CUresult r = g_encode(&entry.map,
                         key.elem_bytes == 2 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_UINT8,
                         rank, const_cast<void*>(key.base), gdim, gstride, box, estr,
-                        CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                        CU_TENSOR_MAP_INTERLEAVE_NONE, key.swizzle == 128 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B,
                         CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   if (r != CUDA_SUCCESS) {
     set_detail("cuTensorMapEncodeTiled failed with CUresult %d (base %p rows %llu cols %llu)", (int)r, key.base, rows, cols);
@@ -241,6 +242,10 @@ static int get_tensor_map(int rank, MapKey key, CUtensorMap* out) {
 int get_tensor_map_2d(const void* base, uint64_t rows, uint64_t cols, int elem_bytes,
                       uint32_t box_rows, uint32_t box_cols, CUtensorMap* out) {
   return get_tensor_map(2, MapKey{0, base, {cols, rows, 1, 1}, elem_bytes, {box_cols, box_rows, 1, 1}, {cols * elem_bytes, 0, 0}}, out);
+}
+
+int get_tensor_map_2d_64(const void* base, uint64_t rows, uint32_t box_rows, CUtensorMap* out) {
+  return get_tensor_map(2, MapKey{0, base, {64, rows, 1, 1}, 1, {64, box_rows, 1, 1}, {64, 0, 0}, 64}, out);
 }
 
 int get_tensor_map_3d(const void* base, uint64_t planes, uint64_t rows, uint64_t cols, int elem_bytes, uint32_t box_planes,

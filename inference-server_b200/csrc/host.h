@@ -37,7 +37,10 @@ int many_form_pays(const void* few, const void* many, int threads, size_t few_sm
 int get_tensor_map_2d(const void* base, uint64_t rows, uint64_t cols, int elem_bytes,
                       uint32_t box_rows, uint32_t box_cols, CUtensorMap* out);
 
-// The same for a dense [planes, rows, cols] tensor; the box's rows of every plane lie one after the other.
+// Rows of 64 bytes, box = box_rows of them, 64-byte swizzle.
+int get_tensor_map_2d_64(const void* base, uint64_t rows, uint32_t box_rows, CUtensorMap* out);
+
+// get_tensor_map_2d for a dense [planes, rows, cols] tensor; the box's rows of every plane lie one after the other.
 int get_tensor_map_3d(const void* base, uint64_t planes, uint64_t rows, uint64_t cols, int elem_bytes, uint32_t box_planes,
                       uint32_t box_rows, uint32_t box_cols, CUtensorMap* out);
 
@@ -106,6 +109,12 @@ inline AttnWorkspace carve(void* ws, int batch, int hq, int D, int max_splits) {
   w.bytes = off;
   return w;
 }
+
+// Argument checks that the attention entry points of the 8-bit page cache share; joining their partials (kv8_decode.cu).
+int check_kv8(const char* name, int rows, int hq, int hkv, int head_dim, int num_blocks, int max_pages, const void* q, const void* k_pool,
+              const void* v_pool, const void* out, float scale);
+int launch_kv8_join(int head_dim, const AttnWorkspace& w, const int* ctx_lens, void* out, int rows, int hq, int max_splits, int split_tokens,
+                    int max_ctx, cudaStream_t st);
 
 }  // namespace b200
 

@@ -387,8 +387,9 @@ kv8_attn_decode_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_c
 #endif
 }
 
-// Joins the partials of one (sequence, query head): a CTA of four warps, warp w taking splits w, w + 4, ..., each lane D / 32
-// columns.  The sums over splits are taken in a fixed order.
+// Joins the partials of one (row, query head): a CTA of four warps, warp w taking splits w, w + 4, ..., each lane D / 32
+// columns.  The sums over splits are taken in a fixed order.  Without lengths every row has max_splits of them, some perhaps empty (their
+// reference is -inf and their sums are not written).
 template <int D>
 __global__ void __launch_bounds__(128)
 kv8_attn_join_kernel(const float* __restrict__ part_o, const float2* __restrict__ part_ml, const int* __restrict__ ctx_lens,
@@ -400,9 +401,12 @@ kv8_attn_join_kernel(const float* __restrict__ part_o, const float2* __restrict_
   __shared__ float ml_sm[4][2];
   const size_t row = blockIdx.x;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int L = min(max(ctx_lens[row / num_q_heads], 0), max_ctx);
-  const int n = (L + split_tokens - 1) / split_tokens;
-  if (n <= 1) return;
+  int n = max_splits;
+  if (ctx_lens != nullptr) {
+    const int L = min(max(ctx_lens[row / num_q_heads], 0), max_ctx);
+    n = (L + split_tokens - 1) / split_tokens;
+    if (n <= 1) return;  // written by its one CTA
+  }
   const size_t base = row * max_splits;
   float top = -INFINITY, den = 0.f, acc[V];
 #pragma unroll
@@ -419,11 +423,13 @@ kv8_attn_join_kernel(const float* __restrict__ part_o, const float2* __restrict_
         const float* from = part_o + (base + s) * D + lane * V;
 #pragma unroll
         for (int j = 0; j < V; ++j) v[u][j] = from[j];
-      } else {
-#pragma unroll
-        for (int j = 0; j < V; ++j) v[u][j] = 0.f;
       }
     }
+#pragma unroll
+    for (int u = 0; u < 4; ++u)
+#pragma unroll
+      for (int j = 0; j < V; ++j)
+        if (ml[u].x == -INFINITY) v[u][j] = 0.f;
     const float t = fmaxf(fmaxf(top, fmaxf(ml[0].x, ml[1].x)), fmaxf(ml[2].x, ml[3].x));
     const float ref = t == -INFINITY ? 0.f : t;
     const float a = exp2f(top - ref);
@@ -458,6 +464,13 @@ kv8_attn_join_kernel(const float* __restrict__ part_o, const float2* __restrict_
     sum += x * ml_sm[w][1];
   }
   out[row * D + d] = __float2bfloat16(num / sum);
+}
+
+int launch_kv8_join(int head_dim, const AttnWorkspace& w, const int* ctx_lens, void* out, int rows, int hq, int max_splits, int split_tokens,
+                    int max_ctx, cudaStream_t st) {
+  B200_CUDA(launch_overlapped(head_dim == 128 ? kv8_attn_join_kernel<128> : kv8_attn_join_kernel<64>, dim3(rows * hq), dim3(128), 0, st, w.o,
+                              w.ml, ctx_lens, static_cast<__nv_bfloat16*>(out), hq, max_splits, split_tokens, max_ctx));
+  return 0;
 }
 
 // Tokens per split where the caller names none.  Few rows: so that all CTAs are there at once and the GPU is full, but no fewer than 64
@@ -515,8 +528,7 @@ static int launch_kv8_decode(const Kv8Args& a) {
                               a.w.err, a.hq, a.hkv, a.num_blocks, a.max_pages, a.plan.split, a.plan.max_splits,
                               a.scale * 1.4426950408889634f));
   if (a.plan.max_splits > 1)
-    B200_CUDA(launch_overlapped(kv8_attn_join_kernel<D>, dim3(a.batch * a.hq), dim3(128), 0, a.st, a.w.o, a.w.ml, a.ctx,
-                                static_cast<__nv_bfloat16*>(a.out), a.hq, a.plan.max_splits, a.plan.split, a.max_pages * kKvPage));
+    return launch_kv8_join(D, a.w, a.ctx, a.out, a.batch, a.hq, a.plan.max_splits, a.plan.split, a.max_pages * kKvPage, a.st);
   return 0;
 }
 
@@ -534,7 +546,7 @@ static int launch_kv8_heads(const Kv8Args& a) {
 
 using namespace b200;
 
-static int check_kv8(const char* name, int batch, int hq, int hkv, int head_dim, int num_blocks, int max_pages, const void* q,
+int b200::check_kv8(const char* name, int batch, int hq, int hkv, int head_dim, int num_blocks, int max_pages, const void* q,
                      const void* k_pool, const void* v_pool, const void* out, float scale) {
   B200_REQUIRE(batch > 0 && hq > 0 && hkv > 0 && num_blocks > 0 && max_pages > 0, "%s: non-positive dimension", name);
   B200_REQUIRE(hq % hkv == 0, "%s: q heads %d not a multiple of kv heads %d", name, hq, hkv);

@@ -1,0 +1,601 @@
+// Causal attention of a chunk of prompt tokens over the 8-bit page cache (kv8.cuh) on the tcgen05 tensor cores (sm_100a), head_dim 64 or 128,
+// up to 128 query heads per kv head: the counterpart of paged_prefill_pairs.cu, which reads 16-bit pools and has the same shape of
+// work (rows of the score matrix, tiles of 128 keys, two tiles of rows in flight per CTA), and replaces the same steps of the
+// reference (src/inference_server/kv_cache/hf_format.py:21-45 + src/inference_server/backends/torch_backend.py:107-147).
+//
+// Mathematics as in kv8_decode.cu: a value's scale is taken into its weight's exponent, keys' scales multiply the scores.
+//
+//   S = Q K^T   from the 8-bit keys as they are, kind::f8f6f4 with both operands K-major in shared memory.  A query is the sum of two
+//               e4m3 numbers, hi = the nearest and lo = what is left: bf16 has 8 bits, hi takes 4, and lo needs 4 more, so the sum is exact
+//               but for the ends of the range (rows are brought to a top of 256 to 448; a query 2^-7 of the row's largest
+//               or smaller loses bits below 2^-19 of it).  Two products of twice the rate cost what one in 16 bits does, and keys need neither conversion
+//               nor room in 16 bits.
+//   P V         kind::f16: weights are f16 in TMEM (11 bits), values are converted to f16 (exactly) by a warp of their own and
+//               stored as MN-major swizzled tiles.  A conversion serves both tiles of rows.
+//
+//   grid     (CTAs of tiles, late ones first) x splits of the keys x kv heads.  The keys are split where the tiles alone leave SMs idle; fp32
+//            partials are then joined by kv8_attn_join_kernel.
+//   warp 0   producer: per key tile, 8 pages of keys by TMA and 8 of values as plain bulk copies, two stages each.
+//   warp 1   S issuer (one thread), warp 2 P V issuer (one thread).
+//   warp 3   values: 16 bytes of a row to 16 f16 numbers; zero for what lies behind the last token, where a page may hold NaN.
+//   warps 4-7, 8-11   first the queries of both tiles (bf16 to hi and lo, a row's top by shuffles), then the softmax of tile 0 and of tile 1,
+//            a thread per score row; the scales of a key tile's 8 pages come to each warp by its own lanes, two key tiles
+//            ahead (ids) and one (scales), and from a corner of shared memory to all lanes.
+//
+// Every mbarrier wait is bounded; a wait that runs out records kErrDevWaitTimeout and the thread stops waiting but keeps the loop
+// structure, so the kernel ends.
+// TMEM: O0, O1, S 128 columns each, P0, P1 64 (two f16 per column).
+
+#include <algorithm>
+
+#include "host.h"
+#include "kv8.cuh"
+#include "prefill_tc.cuh"
+
+namespace b200 {
+
+constexpr int kKv8PrefillThreads = 384;
+constexpr float kKv8PLift = 6.f;  // weights are taken times 2^6, at most 2^14 with the slack of kTcRescaleLog2
+
+template <int D>
+struct Kv8PrefillCfg {
+  static constexpr int kTile8 = kTcKeys * D;                 // bytes of 128 rows in 8 bits
+  static constexpr int kTile16 = 2 * kTile8;
+  static constexpr int kQ = 0;                                // [2 tiles][hi, lo]
+  static constexpr int kK = kQ + 4 * kTile8;                  // [2 stages]
+  static constexpr int kRaw = kK + 2 * kTile8;                // [2 stages] values as they are
+  static constexpr int kV = kRaw + 2 * kTile8;                // [2 stages] values in f16
+  static constexpr int kScales = kV + 2 * kTile16;            // [8 warps][2][8 pages] float4
+  static constexpr int kRowScale = kScales + 8 * 2 * 8 * 16;  // [2 tiles][128] float
+  static constexpr int kSums = kRowScale + 2 * 128 * 4;       // [128] float
+  static constexpr int kBars = kSums + 128 * 4;
+  static constexpr int kSmemBytes = kBars + 256 + 1024 /* alignment slack */;
+};
+
+// Descriptor of a K-major operand tile in 8 bits: rows of 128 bytes with 128-byte swizzle, or of 64 bytes with 64-byte swizzle.
+template <int D>
+__device__ __forceinline__ uint64_t desc_k8(uint32_t smem_addr) {
+  if constexpr (D == 128) return umma_desc_k128(smem_addr);
+  uint64_t d = 0;
+  d |= static_cast<uint64_t>((smem_addr & 0x3FFFFu) >> 4);
+  d |= static_cast<uint64_t>(1) << 16;           // leading byte offset (unused)
+  d |= static_cast<uint64_t>(512 >> 4) << 32;    // groups of 8 rows
+  d |= static_cast<uint64_t>(1) << 46;           // descriptor version (sm_100)
+  d |= static_cast<uint64_t>(4) << 61;           // 64-byte swizzle
+  return d;
+}
+// f16 x f16 -> f32, A K-major, B MN-major.
+__host__ __device__ constexpr uint32_t idesc_f16_mn(uint32_t m, uint32_t n) {
+  return (1u << 4) | (1u << 16) | ((n >> 3) << 17) | ((m >> 4) << 24);
+}
+// D[tmem] (+)= A[tmem] * B[smem], f16: a lane of A is a row, a 32-bit column two neighbouring K elements.
+__device__ __forceinline__ void mma_f16_ts(uint32_t d_tmem, uint32_t a_tmem, uint64_t b_desc, uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}"
+      ::"r"(d_tmem), "r"(a_tmem), "l"(b_desc), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+__device__ __forceinline__ float max_of_3(float a, float b, float c) {
+  float d;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+  return d;
+}
+
+template <int D>
+__global__ void __launch_bounds__(kKv8PrefillThreads, 1)
+kv8_attn_prefill_kernel(const __grid_constant__ CUtensorMap k_map, const uint8_t* __restrict__ v_pool, const uint8_t* __restrict__ k_scale,
+                        const uint8_t* __restrict__ v_scale, const int* __restrict__ table_row, const __nv_bfloat16* __restrict__ q,
+                        __nv_bfloat16* __restrict__ out, float* __restrict__ part_o, float2* __restrict__ part_ml, int* __restrict__ err,
+                        int num_tokens, int first_pos, int num_q_heads, int num_kv_heads, int num_blocks, float scale_log2, int pairs,
+                        int splits, int split_tiles) {
+#ifdef B200_DEVICE_OK
+  using Cfg = Kv8PrefillCfg<D>;
+  constexpr int kPageBytes8 = kKvPage * D, kPageBytes16 = 2 * kPageBytes8;
+  constexpr uint32_t kAtomGroup = D / 64 * 1024;  // 8 rows of f16
+  const int gr = num_q_heads / num_kv_heads;
+  const int QT = kTcRows / gr;  // prompt positions per tile
+  extern __shared__ uint8_t smem_raw[];
+  const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u;
+  uint8_t* base_ptr = smem_raw + (base - smem_u32(smem_raw));
+  const uint32_t bars = base + Cfg::kBars;
+  const uint32_t bar_kfull = bars, bar_kempty = bars + 16;        // [2 stages] each
+  const uint32_t bar_rawfull = bars + 32, bar_rawempty = bars + 48;
+  const uint32_t bar_vfull = bars + 64, bar_vempty = bars + 80;
+  const uint32_t bar_q = bars + 96;                               // Q written
+  const uint32_t bar_sempty = bars + 104;                         // S read
+  const uint32_t bar_sfull = bars + 112;                          // [2 tiles] S written, for this tile
+  const uint32_t bar_odone = bars + 128;                          // [2 tiles] O += P V finished
+  const uint32_t bar_pfull = bars + 144;                          // [2 tiles][2 halves of 64 keys] P written, O rescaled
+  uint32_t* tmem_base_sm = reinterpret_cast<uint32_t*>(base_ptr + Cfg::kBars + 192);
+  float* row_scale = reinterpret_cast<float*>(base_ptr + Cfg::kRowScale);
+  float* sums = reinterpret_cast<float*>(base_ptr + Cfg::kSums);
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  if (threadIdx.x == 32) tma_prefetch_desc(&k_map);
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < 2; ++s) {
+      mbar_init(bar_kfull + 8 * s, 1);
+      mbar_init(bar_kempty + 8 * s, 1);
+      mbar_init(bar_rawfull + 8 * s, 1);
+      mbar_init(bar_rawempty + 8 * s, 1);
+      mbar_init(bar_vfull + 8 * s, 1);
+      mbar_init(bar_vempty + 8 * s, 1);
+      mbar_init(bar_sfull + 8 * s, 1);
+      mbar_init(bar_odone + 8 * s, 1);
+      mbar_init(bar_pfull + 16 * s, 4);
+      mbar_init(bar_pfull + 16 * s + 8, 4);
+    }
+    mbar_init(bar_q, 8);
+    mbar_init(bar_sempty, 4);
+    fence_mbar_init();
+    fence_proxy_async();
+  }
+  if (warp == 1) tmem_alloc(smem_u32(tmem_base_sm), 512);
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem_base = *tmem_base_sm;
+  const uint32_t tmem_o = tmem_base, tmem_s = tmem_base + 2 * kTcKeys, tmem_p = tmem_s + kTcKeys;  // O0, O1, S, P0, P1
+  // late positions first, all splits and kv heads of them side by side; the first `pairs` CTAs of a head take two tiles of rows each
+  const int h = static_cast<int>(blockIdx.x) % num_kv_heads, rest = static_cast<int>(blockIdx.x) / num_kv_heads;
+  const int split = rest % splits, cta = rest / splits;
+  const int own = cta < pairs ? 2 : 1;
+  const int t0 = ((num_tokens + QT - 1) / QT - own - cta - min(cta, pairs)) * QT;
+  const int t_end = min(t0 + own * QT, num_tokens);
+  const int last_pos = first_pos + t_end - 1;
+  // key tiles of this CTA: kt0 ..; each tile of rows takes the first n_of[] of them
+  const int kt0 = split * split_tiles;
+  const int n_tiles = max(0, min(last_pos / kTcKeys + 1, kt0 + split_tiles) - kt0);
+  int n_of[2];
+#pragma unroll
+  for (int t = 0; t < 2; ++t) {
+    const int first = t0 + t * QT;
+    n_of[t] = first < t_end ? max(0, min(n_tiles, (first_pos + min(first + QT, t_end) - 1) / kTcKeys + 1 - kt0)) : 0;
+  }
+  const int last_page = last_pos / kKvPage;
+
+  grid_dep_wait();  // set-up done; Q and this chunk's pages come from the kernels before
+  grid_dep_launch();
+
+  if (warp < 4) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
+    if (warp == 0) {
+      // ------------------------------------------------- pages ------
+      // Lane i of the first 8 owns page i of a tile's keys, of the second 8 that of its values.
+      const int pg = lane & 7;
+      bool alive = true;
+#pragma unroll 1
+      for (int j = 0; j < n_tiles; ++j) {
+        const int st = j & 1;
+        // the last page stands in for those behind it, so that every stage is the same number of bytes
+        int page = __ldg(table_row + min((kt0 + j) * kTcPages + pg, last_page));
+        if (page < 0 || page >= num_blocks) {
+          set_error(err, kErrDevBadBlockId);
+          page = 0;
+        }
+        const size_t cell = static_cast<size_t>(page) * num_kv_heads + h;
+        if (alive) alive = mbar_wait(bar_kempty + 8 * st, ((j >> 1) & 1) ^ 1, err);
+        if (!__all_sync(0xffffffffu, alive)) break;
+        if (lane == 0) mbar_arrive_expect_tx(bar_kfull + 8 * st, Cfg::kTile8);
+        __syncwarp();
+        if (lane < kTcPages)
+          tma_load_2d(base + Cfg::kK + st * Cfg::kTile8 + pg * kPageBytes8, &k_map, bar_kfull + 8 * st, 0, static_cast<int>(cell) * kKvPage);
+        if (alive) alive = mbar_wait(bar_rawempty + 8 * st, ((j >> 1) & 1) ^ 1, err);
+        if (!__all_sync(0xffffffffu, alive)) break;
+        if (lane == 0) mbar_arrive_expect_tx(bar_rawfull + 8 * st, Cfg::kTile8);
+        __syncwarp();
+        if (lane >= 8 && lane < 16)
+          bulk_load(base + Cfg::kRaw + st * Cfg::kTile8 + pg * kPageBytes8, v_pool + cell * kPageBytes8, kPageBytes8, bar_rawfull + 8 * st);
+      }
+    } else if (warp == 3) {
+      // ------------------------------------------------- V in f16 ------
+      // A lane takes 16 bytes of a row at a time.  Their 32 bytes in f16 are two pieces of a swizzled row; the lanes of the second
+      // column half store theirs in the other order, so that a quarter warp's pieces lie in different banks.
+      constexpr int kPieces = D / 16, kRowsAt = 32 / kPieces;  // pieces of a row; rows that the warp takes at a time
+      const int c = lane % kPieces, lr = lane / kPieces;
+      const uint32_t half_off = (c >> 2) * 1024;
+      const int first_piece = (2 * c) & 7, swap = D == 128 ? c >> 2 : 0;
+      bool alive = true;
+#pragma unroll 1
+      for (int j = 0; j < n_tiles && alive; ++j) {
+        const int st = j & 1;
+        alive = mbar_wait(bar_rawfull + 8 * st, (j >> 1) & 1, err) && mbar_wait(bar_vempty + 8 * st, ((j >> 1) & 1) ^ 1, err);
+        if (!__all_sync(0xffffffffu, alive)) break;
+        const uint32_t from = base + Cfg::kRaw + st * Cfg::kTile8, to = base + Cfg::kV + st * Cfg::kTile16;
+        const int rows = last_pos - (kt0 + j) * kTcKeys + 1;  // of them hold tokens
+#pragma unroll 1
+        for (int r0 = 0; r0 < kTcKeys; r0 += 4 * kRowsAt) {
+          uint32_t w[4][4];
+#pragma unroll
+          for (int u = 0; u < 4; ++u) {
+            const int r = r0 + u * kRowsAt + lr;
+            asm volatile("ld.shared.v4.b32 {%0,%1,%2,%3}, [%4];"
+                         : "=r"(w[u][0]), "=r"(w[u][1]), "=r"(w[u][2]), "=r"(w[u][3]) : "r"(from + r * D + c * 16) : "memory");
+            if (r >= rows) w[u][0] = w[u][1] = w[u][2] = w[u][3] = 0u;
+          }
+#pragma unroll
+          for (int u = 0; u < 4; ++u) {
+            const int r = r0 + u * kRowsAt + lr;
+            uint32_t a[2][4];
+#pragma unroll
+            for (int k = 0; k < 4; ++k) e4m3x4_to_f16(w[u][k], a[k >> 1][(k & 1) * 2], a[k >> 1][(k & 1) * 2 + 1]);
+            const uint32_t row = to + (r >> 3) * kAtomGroup + half_off;
+#pragma unroll
+            for (int k = 0; k < 2; ++k) {
+              const int which = k ^ swap;
+              asm volatile("st.shared.v4.b32 [%0], {%1,%2,%3,%4};" ::"r"(row + swz128(r & 7, first_piece + which)), "r"(which ? a[1][0] : a[0][0]),
+                           "r"(which ? a[1][1] : a[0][1]), "r"(which ? a[1][2] : a[0][2]), "r"(which ? a[1][3] : a[0][3])
+                           : "memory");
+            }
+          }
+        }
+        fence_proxy_async();  // the tensor core reads the tile, and the next copy writes the stage, through the async proxy
+        __syncwarp();
+        if (lane == 0) {
+          mbar_arrive(bar_vfull + 8 * st);
+          mbar_arrive(bar_rawempty + 8 * st);
+        }
+      }
+    } else if (warp == 1) {
+      // ------------------------------------------------- S = Q K^T ------
+      if (elect_one()) {
+        constexpr uint32_t idesc_s = umma_idesc_f8(kTcRows, kTcKeys);
+        bool alive = mbar_wait(bar_q, 0, err);
+        uint32_t n = 0;
+#pragma unroll 1
+        for (int j = 0; j < n_tiles && alive; ++j) {
+          const int st = j & 1;
+          alive = mbar_wait(bar_kfull + 8 * st, (j >> 1) & 1, err);
+          const uint64_t b0 = desc_k8<D>(base + Cfg::kK + st * Cfg::kTile8);
+#pragma unroll
+          for (int t = 0; t < 2; ++t) {
+            if (j >= n_of[t]) continue;  // none of this tile's rows sees these keys
+            if (alive) alive = mbar_wait(bar_sempty, (n & 1) ^ 1, err);
+            if (!alive) break;
+            ++n;
+            tc_fence_after();
+#pragma unroll
+            for (int part = 0; part < 2; ++part) {
+              const uint64_t a0 = desc_k8<D>(base + Cfg::kQ + (2 * t + part) * Cfg::kTile8);
+#pragma unroll
+              for (int k = 0; k < D / 32; ++k) tc_mma_f8(tmem_s, a0 + 2 * k, b0 + 2 * k, idesc_s, part + k > 0 ? 1u : 0u);
+            }
+            tc_commit(bar_sfull + 8 * t);
+          }
+          tc_commit(bar_kempty + 8 * st);
+        }
+      }
+    } else if (elect_one()) {
+      // ------------------------------------------------- O += P V ------
+      constexpr uint32_t idesc_o = idesc_f16_mn(kTcRows, D);
+      bool alive = true;
+#pragma unroll 1
+      for (int j = 0; j < n_tiles && alive; ++j) {
+        const int st = j & 1;
+        alive = mbar_wait(bar_vfull + 8 * st, (j >> 1) & 1, err);
+#pragma unroll
+        for (int t = 0; t < 2; ++t) {
+          if (j >= n_of[t]) continue;
+#pragma unroll
+          for (int half = 0; half < 2; ++half) {
+            if (alive) alive = mbar_wait(bar_pfull + 16 * t + 8 * half, j & 1, err);
+            if (!alive) break;
+            tc_fence_after();
+#pragma unroll
+            for (int kk = half * 4; kk < half * 4 + 4; ++kk) {  // 16 keys each
+              const uint64_t b = umma_desc_mn128(base + Cfg::kV + st * Cfg::kTile16 + kk * kPageBytes16, 1024, kAtomGroup);
+              mma_f16_ts(tmem_o + t * kTcKeys, tmem_p + t * 64 + kk * 8, b, idesc_o, (j > 0 || kk > 0) ? 1u : 0u);
+            }
+          }
+          tc_commit(bar_odone + 8 * t);
+        }
+        tc_commit(bar_vempty + 8 * st);
+      }
+    }
+  } else {
+    // -------------------------------------------------------- softmax ------
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 224;");
+    const int t = (warp >> 2) - 1;           // tile of rows
+    const int quarter = warp & 3;            // TMEM lanes this warp may touch
+    const int r = quarter * 32 + lane;       // score row
+    const uint32_t lane_off = static_cast<uint32_t>(quarter * 32) << 16;
+    const uint32_t s_acc = tmem_s + lane_off, o_acc = tmem_o + t * kTcKeys + lane_off, p_tm = tmem_p + t * 64 + lane_off;
+    const uint32_t sfull = bar_sfull + 8 * t, odone = bar_odone + 8 * t, pfull = bar_pfull + 16 * t;
+    const int tt0 = t0 + t * QT, rt = r / gr, n_own = t ? n_of[1] : n_of[0];
+    const int pos = first_pos + min(tt0 + rt, min(tt0 + QT, num_tokens) - 1);  // the last key this row may see
+
+    // Scales of the pages of a key tile: lane i of 8 asks for those of page i.
+    const int pg = lane & 7;
+    auto page_id = [&](int j) {
+      const int id = j < n_own ? __ldg(table_row + min((kt0 + j) * kTcPages + pg, last_page)) : 0;
+      return id < 0 || id >= num_blocks ? 0 : id;  // the producer reports it
+    };
+    int id = page_id(0);
+    int kb = k_scale[static_cast<size_t>(id) * num_kv_heads + h], vb = v_scale[static_cast<size_t>(id) * num_kv_heads + h];
+    id = page_id(1);
+
+    // Q tiles: neighbouring threads neighbouring pieces of 8 numbers of a row
+    for (int u = 0; u < own; ++u) {
+      uint4 v[D / 16];
+#pragma unroll
+      for (int k = 0; k < D / 16; ++k) {
+        const int i = threadIdx.x - 128 + k * 256, qr = i / (D / 8), qt_l = qr / gr, tok = t0 + u * QT + qt_l;
+        v[k] = make_uint4(0u, 0u, 0u, 0u);
+        if (qt_l < QT && tok < num_tokens)
+          v[k] = *reinterpret_cast<const uint4*>(q + (static_cast<size_t>(tok) * num_q_heads + h * gr + (qr - qt_l * gr)) * D + i % (D / 8) * 8);
+      }
+#pragma unroll
+      for (int k = 0; k < D / 16; ++k) {
+        const int i = threadIdx.x - 128 + k * 256, qr = i / (D / 8), ch = i % (D / 8);
+        const uint32_t x[4] = {v[k].x, v[k].y, v[k].z, v[k].w};
+        uint32_t top = 0;
+#pragma unroll
+        for (int w = 0; w < 4; ++w) top = max(top, max((x[w] & 0x7fff0000u), (x[w] & 0x7fffu) << 16));
+#pragma unroll
+        for (int o = 1; o < D / 8; o <<= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
+        // the exponent that brings the row's top to (224, 448]; tiny rows may stay below, a row with an infinity is all NaN
+        const int e = max(static_cast<int>(top >> 23) - 127 - 8 + ((top & 0x7fffffu) > 0x600000u ? 1 : 0), -100);
+        const float by = top < 0x7f800000u ? power_of_two(-e) : NAN;
+        uint32_t hi[2], lo[2];
+#pragma unroll
+        for (int w = 0; w < 2; ++w) {
+          uint32_t pair[2], rest_of[2];
+#pragma unroll
+          for (int p = 0; p < 2; ++p) {
+            const float a = __uint_as_float(x[2 * w + p] << 16) * by, b = __uint_as_float(x[2 * w + p] & 0xffff0000u) * by;
+            pair[p] = to_e4m3x2(a, b);
+            uint32_t near, unused;
+            e4m3x4_to_f16(pair[p], near, unused);
+            const float2 n2 = __half22float2(*reinterpret_cast<const __half2*>(&near));
+            rest_of[p] = to_e4m3x2(a - n2.x, b - n2.y);
+          }
+          hi[w] = pair[0] | pair[1] << 16;
+          lo[w] = rest_of[0] | rest_of[1] << 16;
+        }
+        uint32_t at;
+        if constexpr (D == 128) at = (qr >> 3) * 1024 + swz128(qr & 7, ch >> 1) + (ch & 1) * 8;
+        else at = qr * 64 + (((ch >> 1) ^ ((qr >> 1) & 3)) << 4) + (ch & 1) * 8;
+        *reinterpret_cast<uint2*>(base_ptr + Cfg::kQ + 2 * u * Cfg::kTile8 + at) = make_uint2(hi[0], hi[1]);
+        *reinterpret_cast<uint2*>(base_ptr + Cfg::kQ + (2 * u + 1) * Cfg::kTile8 + at) = make_uint2(lo[0], lo[1]);
+        if (ch == 0) row_scale[u * kTcRows + qr] = fmaxf(scale_log2 * power_of_two(min(e, 120)), 0x1p-90f);
+      }
+    }
+    fence_proxy_async();  // the tensor core reads Q through the async proxy
+    asm volatile("bar.sync 1, 256;" ::: "memory");
+    if (lane == 0) mbar_arrive(bar_q);
+    const float f_q = own > t ? row_scale[t * kTcRows + r] : 1.f;
+    float4* scales = reinterpret_cast<float4*>(base_ptr + Cfg::kScales) + (warp - 4) * 16;
+
+    float m_run = -INFINITY, l_run = 0.f;
+    bool alive = true, s_ready = false;
+    int kbase = kt0 * kTcKeys;
+#pragma unroll 1
+    for (int i = 0; i < n_own; ++i, kbase += kTcKeys) {
+      {
+        const int ev = scale_exponent(vb);
+        if (lane < 8) scales[(i & 1) * 8 + pg] = make_float4(power_of_two(scale_exponent(kb)), static_cast<float>(ev), power_of_two(-ev), 0.f);
+        __syncwarp();
+        if (i + 1 < n_own) {
+          kb = k_scale[static_cast<size_t>(id) * num_kv_heads + h];
+          vb = v_scale[static_cast<size_t>(id) * num_kv_heads + h];
+          id = page_id(i + 2);
+        }
+      }
+      const float4* sc = scales + (i & 1) * 8;
+      if (!__all_sync(0xffffffffu, s_ready) && alive) alive = mbar_wait(sfull, i & 1, err);
+      tc_fence_after();
+      float s[128];
+      {
+        uint32_t (&raw)[4][32] = *reinterpret_cast<uint32_t(*)[4][32]>(s);
+#pragma unroll
+        for (int c = 0; c < 4; ++c) tmem_ld32(s_acc + c * 32, raw[c]);
+        tmem_ld_wait();
+      }
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(bar_sempty);  // S is the other tile's now
+      if (kbase + kTcKeys - 1 > pos) {  // the causal edge runs through this row
+#pragma unroll
+        for (int c = 0; c < 128; ++c)
+          if (kbase + c > pos) s[c] = -INFINITY;
+      }
+      // a scale is positive: the largest product of a page is that of its largest score
+      float m_new = m_run;
+#pragma unroll
+      for (int p = 0; p < 8; ++p) {
+        const float* x = s + 16 * p;
+        const float a = max_of_3(max_of_3(x[0], x[1], x[2]), x[3], x[4]), b = max_of_3(max_of_3(x[5], x[6], x[7]), x[8], x[9]);
+        const float c = max_of_3(max_of_3(x[10], x[11], x[12]), x[13], x[14]);
+        m_new = fmaxf(m_new, fmaf(max_of_3(max_of_3(a, b, c), x[15], x[15]), f_q * sc[p].x, sc[p].y));
+      }
+      const bool need = m_new - m_run > kTcRescaleLog2;  // true on the first tile (m_run = -inf)
+      if (__any_sync(0xffffffffu, need)) {
+        if (i > 0) {
+          // O may be touched once the product of the tile before has finished
+          if (alive) alive = mbar_wait(odone, (i - 1) & 1, err);
+          tc_fence_after();
+          // a row that has seen no key yet holds exact zeros
+          const float alpha = m_new == -INFINITY ? 1.f : fast_exp2(m_run - m_new);
+          l_run *= alpha;
+#pragma unroll
+          for (int c0 = 0; c0 < D; c0 += 32) {
+            uint32_t o[32];
+            tmem_ld32(o_acc + c0, o);
+            tmem_ld_wait();
+#pragma unroll
+            for (int c = 0; c < 32; ++c) o[c] = __float_as_uint(__uint_as_float(o[c]) * alpha);
+            tmem_st32(o_acc + c0, o);
+          }
+        }
+        m_run = m_new;
+      }
+      const float mb = m_run == -INFINITY ? 0.f : m_run - kKv8PLift;
+      bool p_free = i == 0;
+#pragma unroll
+      for (int half = 0; half < 2; ++half) {
+        uint32_t pk[32];
+#pragma unroll
+        for (int p = 0; p < 4; ++p) {
+          const float4 w = sc[half * 4 + p];
+          const float f = f_q * w.x, off = w.y - mb;
+          float sum[2];
+#pragma unroll
+          for (int ch = 0; ch < 2; ++ch) {
+            // asked here, needed behind this half: P was last read by the product of the tile before; the next S
+            if (p == 2 && ch == 1 && half == 0 && i > 0) p_free = mbar_test(odone, (i - 1) & 1);
+            if (p == 2 && ch == 1 && half == 1) s_ready = mbar_test(sfull, (i + 1) & 1);
+            float e[8];
+#pragma unroll
+            for (int k = 0; k < 8; ++k) e[k] = fast_exp2(fmaf(s[half * 64 + p * 16 + ch * 8 + k], f, off));
+            sum[ch] = ((e[0] + e[1]) + (e[2] + e[3])) + ((e[4] + e[5]) + (e[6] + e[7]));
+#pragma unroll
+            for (int k = 0; k < 4; ++k) pk[p * 8 + ch * 4 + k] = pack_f16x2(e[2 * k], e[2 * k + 1]);
+          }
+          l_run = fmaf(sum[0] + sum[1], w.z, l_run);
+        }
+        if (half == 0 && !__all_sync(0xffffffffu, p_free) && alive) alive = mbar_wait(odone, (i - 1) & 1, err);
+        tc_fence_after();
+        tmem_st32(p_tm + half * 32, pk);
+        tmem_st_wait();
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(pfull + 8 * half);
+      }
+    }
+    // ---- epilogue, once the product of the last key tile has finished.  The warps of a CTA with one tile share its columns.
+    const int e = own == 2 ? t : 0, cols = own == 2 ? D : D / 2, col0 = own == 2 ? 0 : t * (D / 2), n_e = e ? n_of[1] : n_of[0];
+    const int tok = t0 + e * QT + rt;
+    const bool real = rt < QT && tok < t_end;
+    const size_t oidx = static_cast<size_t>(tok) * num_q_heads + h * gr + (r - rt * gr);
+    float l = l_run;
+    if (splits > 1 && real && e == t) part_ml[oidx * splits + split] = make_float2(m_run, l);
+    if (own == 1) {
+      if (t == 0) sums[r] = l;
+      asm volatile("bar.sync 1, 256;" ::: "memory");
+      l = sums[r];
+    }
+    if (n_e > 0) {
+      if (alive) alive = mbar_wait(bar_odone + 8 * e, (n_e - 1) & 1, err);
+      tc_fence_after();
+      const float inv = 1.f / l;
+#pragma unroll 1
+      for (int c0 = 0; c0 < cols; c0 += 32) {
+        uint32_t o[32];
+        tmem_ld32(tmem_o + e * kTcKeys + lane_off + col0 + c0, o);
+        tmem_ld_wait();
+        if (real && alive) {
+          if (splits > 1) {
+            float4* to = reinterpret_cast<float4*>(part_o + (oidx * splits + split) * D + col0 + c0);
+#pragma unroll
+            for (int c = 0; c < 8; ++c)
+              to[c] = make_float4(__uint_as_float(o[4 * c]), __uint_as_float(o[4 * c + 1]), __uint_as_float(o[4 * c + 2]), __uint_as_float(o[4 * c + 3]));
+          } else {
+            uint4* to = reinterpret_cast<uint4*>(out + oidx * D + col0 + c0);
+#pragma unroll
+            for (int c = 0; c < 4; ++c) {
+              uint32_t w[4];
+#pragma unroll
+              for (int k = 0; k < 4; ++k) w[k] = pack_bf16x2(__uint_as_float(o[8 * c + 2 * k]) * inv, __uint_as_float(o[8 * c + 2 * k + 1]) * inv);
+              to[c] = make_uint4(w[0], w[1], w[2], w[3]);
+            }
+          }
+        }
+      }
+    }
+  }
+
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 1) {
+    tc_fence_after();
+    tmem_dealloc(tmem_base, 512);
+  }
+#endif
+}
+
+// How a call is laid out: tiles of 128 score rows per kv head, how many CTAs of a head take two of them (the rule of the 16-bit kernel,
+// paged_prefill_pairs.cu), and into how many parts of `split_tiles` key tiles the keys are cut.
+struct Kv8PrefillPlan {
+  int ctas, pairs, splits, split_tiles;
+};
+static int kv8_prefill_plan(int num_tokens, int first_pos, int hq, int hkv, Kv8PrefillPlan* p) {
+  int sms = 0;
+  const int rc = device_sm_count(&sms);
+  if (rc) return rc;
+  p->pairs = b200_paged_attn_prefill_pairs(num_tokens, first_pos, hq, hkv, 0, sms, nullptr);
+  if (p->pairs < 0) return p->pairs;
+  const int qt = kTcRows / (hq / hkv), key_tiles = (first_pos + num_tokens - 1) / kTcKeys + 1;
+  p->ctas = (num_tokens + qt - 1) / qt - p->pairs;
+  const long long all = static_cast<long long>(p->ctas) * hkv;
+  // as many parts as SMs are there for, of two key tiles at least: a part's set-up and its partials cost about as much
+  const int want = static_cast<int>(std::max(1ll, std::min<long long>(sms / all, (key_tiles + 1) / 2)));
+  p->split_tiles = (key_tiles + want - 1) / want;
+  p->splits = (key_tiles + p->split_tiles - 1) / p->split_tiles;
+  return 0;
+}
+
+template <int D>
+static int launch_kv8_prefill(const void* q, const void* k_pool, const void* v_pool, const void* k_scale, const void* v_scale,
+                              const int* table_row, void* out, const AttnWorkspace& w, int num_tokens, int first_pos, int hq, int hkv,
+                              int num_blocks, float scale, const Kv8PrefillPlan& p, cudaStream_t st) {
+  CUtensorMap kmap;
+  const uint64_t rows = static_cast<uint64_t>(num_blocks) * hkv * kKvPage;
+  int rc = D == 128 ? get_tensor_map_2d(k_pool, rows, 128, 1, kKvPage, 128, &kmap) : get_tensor_map_2d_64(k_pool, rows, kKvPage, &kmap);
+  if (rc) return rc;
+  rc = ensure_dynamic_smem(reinterpret_cast<const void*>(&kv8_attn_prefill_kernel<D>), Kv8PrefillCfg<D>::kSmemBytes);
+  if (rc) return rc;
+  B200_CUDA(launch_overlapped(kv8_attn_prefill_kernel<D>, dim3(p.ctas * p.splits * hkv), dim3(kKv8PrefillThreads), Kv8PrefillCfg<D>::kSmemBytes,
+                              st, kmap, static_cast<const uint8_t*>(v_pool), static_cast<const uint8_t*>(k_scale),
+                              static_cast<const uint8_t*>(v_scale), table_row, static_cast<const __nv_bfloat16*>(q),
+                              static_cast<__nv_bfloat16*>(out), w.o, w.ml, w.err, num_tokens, first_pos, hq, hkv, num_blocks,
+                              scale * 1.4426950408889634f, p.pairs, p.splits, p.split_tiles));
+  if (p.splits > 1) return launch_kv8_join(D, w, nullptr, out, num_tokens, hq, p.splits, 0, 0, st);
+  return 0;
+}
+
+}  // namespace b200
+
+using namespace b200;
+
+extern "C" size_t b200_kv8_attn_prefill_workspace_bytes(int num_tokens, int first_position, int num_q_heads, int num_kv_heads, int head_dim) {
+  if (num_tokens <= 0 || first_position < 0 || num_q_heads <= 0 || num_kv_heads <= 0 || head_dim <= 0 || num_q_heads % num_kv_heads != 0 ||
+      num_q_heads / num_kv_heads > kTcRows || static_cast<long long>(num_tokens) + first_position >= (1ll << 31) - kTcKeys)
+    return 256;
+  Kv8PrefillPlan p;
+  if (kv8_prefill_plan(num_tokens, first_position, num_q_heads, num_kv_heads, &p) || p.splits == 1) return 256;
+  return carve(nullptr, num_tokens, num_q_heads, head_dim, p.splits).bytes;
+}
+
+extern "C" int b200_kv8_attn_prefill(const void* q, const void* k_pool, const void* v_pool, const void* k_scale, const void* v_scale,
+                                     const int32_t* block_table_row, void* out, void* workspace, size_t workspace_bytes, int num_tokens,
+                                     int first_position, int num_q_heads, int num_kv_heads, int head_dim, int num_blocks,
+                                     int max_pages_per_seq, float scale, void* stream) {
+  B200_REQUIRE(q && k_pool && v_pool && k_scale && v_scale && block_table_row && out && workspace, "kv8_attn_prefill: null pointer");
+  int rc = check_kv8("kv8_attn_prefill", num_tokens, num_q_heads, num_kv_heads, head_dim, num_blocks, max_pages_per_seq, q, k_pool, v_pool, out,
+                     scale);
+  if (rc) return rc;
+  B200_REQUIRE(num_q_heads / num_kv_heads <= kTcRows, "kv8_attn_prefill: more than %d q heads per kv head", kTcRows);
+  B200_REQUIRE(first_position >= 0 && static_cast<long long>(first_position) + num_tokens <= static_cast<long long>(max_pages_per_seq) * kKvPage,
+               "kv8_attn_prefill: positions %d .. of %d tokens do not fit %d pages", first_position, num_tokens, max_pages_per_seq);
+  B200_REQUIRE(static_cast<long long>(first_position) + num_tokens < (1ll << 31) - kTcKeys &&
+                   static_cast<long long>(num_tokens) * num_q_heads < (1ll << 31),
+               "kv8_attn_prefill: positions or rows past 2^31");
+  rc = check_device(nullptr);
+  if (rc) return rc;
+  Kv8PrefillPlan p;
+  rc = kv8_prefill_plan(num_tokens, first_position, num_q_heads, num_kv_heads, &p);
+  if (rc) return rc;
+  B200_REQUIRE(static_cast<long long>(p.ctas) * p.splits * num_kv_heads < (1ll << 31), "kv8_attn_prefill: grid too large");
+  AttnWorkspace w = carve(workspace, num_tokens, num_q_heads, head_dim, p.splits);
+  const size_t need = p.splits > 1 ? w.bytes : 256;
+  if (workspace_bytes < need || (reinterpret_cast<uintptr_t>(workspace) & 15) != 0) {
+    set_detail("kv8_attn_prefill: workspace of %zu bytes at %p, %zu on a 16-byte boundary are needed", workspace_bytes, workspace, need);
+    return -kErrWorkspace;
+  }
+#define B200_KV8_ARGS q, k_pool, v_pool, k_scale, v_scale, block_table_row, out, w, num_tokens, first_position, num_q_heads, num_kv_heads, \
+                      num_blocks, scale, p, as_stream(stream)
+  return head_dim == 128 ? launch_kv8_prefill<128>(B200_KV8_ARGS) : launch_kv8_prefill<64>(B200_KV8_ARGS);
+#undef B200_KV8_ARGS
+}

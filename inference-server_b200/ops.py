@@ -332,6 +332,46 @@ def kv8_attn_decode(q, k_pool, v_pool, k_scale, v_scale, block_table, ctx_lens, 
     return out
 
 
+def kv8_attn_prefill_workspace(num_tokens: int, first_pos: int, num_q_heads: int, num_kv_heads: int, head_dim: int, device) -> torch.Tensor:
+    """Workspace of `kv8_attn_prefill`, starting with the status word."""
+    n = _lib.load().b200_kv8_attn_prefill_workspace_bytes(num_tokens, first_pos, num_q_heads, num_kv_heads, head_dim)
+    return torch.zeros(n, dtype=torch.uint8, device=device)
+
+
+def kv8_attn_prefill(q, k_pool, v_pool, k_scale, v_scale, table_row, first_pos: int, scale: float, workspace: torch.Tensor | None = None,
+                     out: torch.Tensor | None = None) -> torch.Tensor:
+    """`paged_attn_prefill` over an 8-bit page cache: causal attention of consecutive prompt tokens of one sequence, q [R, Hq, D] bf16 at
+    positions first_pos .. first_pos + R - 1, keys and values already in their slots; table_row [max_pages] int32.  head_dim 64 or 128, up to 128 query
+    heads per kv head.  Few rows over many keys are shared out along the keys and joined in the workspace."""
+    nb, Hkv, D = _kv8_cache(k_pool, v_pool, k_scale, v_scale)
+    _need(q, "q", torch.bfloat16)
+    _need(table_row, "table_row", torch.int32)
+    if q.dim() != 3 or q.shape[2] != D:
+        raise ValueError(f"q must be [tokens, heads, {D}], got {list(q.shape)}")
+    if table_row.dim() != 1:
+        raise ValueError("table_row must be one row of a block table")
+    R, Hq, _ = q.shape
+    if out is None:
+        out = torch.empty_like(q)
+    else:
+        _need(out, "out", torch.bfloat16)
+        if out.shape != q.shape:
+            raise ValueError("out does not match q")
+    _on_current_device(q, k_pool, v_pool, k_scale, v_scale, table_row, out)
+    if R == 0:
+        return out
+    if workspace is None:
+        workspace = kv8_attn_prefill_workspace(R, int(first_pos), Hq, Hkv, D, q.device)
+    else:
+        _need(workspace, "workspace", torch.uint8)
+        _on_current_device(workspace)
+    rc = _lib.load().b200_kv8_attn_prefill(
+        _ptr(q), _ptr(k_pool), _ptr(v_pool), _ptr(k_scale), _ptr(v_scale), _ptr(table_row), _ptr(out), _ptr(workspace), workspace.numel(),
+        R, int(first_pos), Hq, Hkv, D, nb, table_row.numel(), float(scale), _stream())
+    check(rc, "b200_kv8_attn_prefill")
+    return out
+
+
 # ---------------------------------------------------------- dense projections
 
 

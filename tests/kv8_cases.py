@@ -75,9 +75,9 @@ def random_cache(rng, blocks: int, H: int, D: int, spread: int = 3):
     return codes, rng.integers(-6 - spread, -6 + spread + 1, (blocks, H))
 
 
-def attention(q: np.ndarray, k: np.ndarray, v: np.ndarray, unit: np.ndarray, scale: float):
+def attention(q: np.ndarray, k: np.ndarray, v: np.ndarray, unit: np.ndarray, scale: float, q_step: float = 0.0):
     """(softmax(q k^T scale) v, a bound on the error of the kernels) for one query row q [Hq, D] over k, v [L, H, D], whose values have
-    scales unit [L, H]."""
+    scales unit [L, H].  `q_step`: how far a kernel's query may be off, as a part of the row's largest."""
     Hq, D = q.shape
     L, H, _ = k.shape
     out, tol = np.zeros((Hq, D)), np.zeros((Hq, D))
@@ -97,6 +97,7 @@ def attention(q: np.ndarray, k: np.ndarray, v: np.ndarray, unit: np.ndarray, sca
         # scale in it, is 2^6 at least: 2^-31 of that, times a code of at most 448.  The sum of the weights is off by ds, and the
         # result is rounded to 8 bits, 2^-8 with what an approximate quotient adds.
         ds = D * 2.0 ** -24 * (np.abs(kh) @ np.abs(q[h])).max() * scale + (np.abs(s).max() * 1.45 + 32) * 2.0 ** -22 + 2.0 ** -22
+        ds += q_step * np.abs(q[h]).max() * np.abs(kh).sum(1).max() * scale
         tol[h] = 2.0 ** -8 * np.abs(out[h]) + (2 * ds + 2.0 ** -11) * (p @ np.abs(vh)) + L * 448 * 2.0 ** -31 * (p * unit[:, g]).max()
     return out, tol
 

@@ -232,11 +232,11 @@ def rows_at(codes, exps, row, L):
     return x.transpose(0, 2, 1, 3).reshape(-1, codes.shape[1], codes.shape[3])[:L]
 
 
-def check_attn(got, q, kc, ke, vc, ve, table, lens, scale):
+def check_attn(got, q, kc, ke, vc, ve, table, lens, scale, q_step=0.0):
     got = got.double().cpu().numpy()
     for b, L in enumerate(lens):
         unit = np.repeat(2.0 ** np.clip(ve[table[b][:-(-L // 16)]], -32, 31), 16, axis=0)[:L]
-        want, tol = plain.attention(q[b].double().numpy(), rows_at(kc, ke, table[b], L), rows_at(vc, ve, table[b], L), unit, scale)
+        want, tol = plain.attention(q[b].double().numpy(), rows_at(kc, ke, table[b], L), rows_at(vc, ve, table[b], L), unit, scale, q_step)
         over = np.abs(got[b] - want) - tol
         assert np.isfinite(got[b]).all() and over.max() <= 0, (b, L, float(over.max()), float(np.abs(want).max()))
 
@@ -332,6 +332,89 @@ def test_decode_pages_past_32_bits_of_bytes(ops):
     assert torch.equal(got, ops.kv8_attn_decode(q, *small, ints([[0, 1, 2]]), ints([41]), 0.1))
     check_attn(got, q.cpu(), *(f(c) for c in (small[0], small[2], small[1], small[3]) for f in [lambda c: c.view(torch.uint8).cpu().numpy()
                if c.dtype == plain.E4M3 else c.view(torch.uint8).cpu().numpy().astype(int) - 127]), np.array([[0, 1, 2]]), [41], 0.1)
+
+
+# -------------------------------------------------------------------- prompt
+
+
+def run_prefill(ops, n, first, Hq, H, D, seed, spread=3, q_size=1.0, scale=0.1, rows=None, width=0):
+    """A prompt of n tokens behind `first`, checked at `rows` (all by default)."""
+    rng = np.random.default_rng(seed)
+    q, kc, ke, vc, ve, table = attn_case(rng, [first + n], Hq, H, D, spread, 1.0)
+    q = torch.from_numpy((rng.standard_normal((n, Hq, D)) * q_size).astype(np.float32)).bfloat16()
+    table = np.concatenate([table[0], np.full(width, -1, dtype=np.int32)])
+    dev = q.to(DEV)
+    ws = ops.kv8_attn_prefill_workspace(n, first, Hq, H, D, DEV)
+    ws[4:] = 255  # partials hold NaN before the call
+    out = ops.kv8_attn_prefill(dev, plain.pool_of(kc), plain.pool_of(vc), plain.scale_of(ke), plain.scale_of(ve), torch.from_numpy(table).to(DEV), first,
+                               scale, workspace=ws, out=torch.full_like(dev, float("nan")))
+    ops.read_status(ws, "kv8_attn_prefill")
+    assert not out.isnan().any()
+    rows = range(n) if rows is None else sorted({r for r in rows if 0 <= r < n})
+    # a query is the sum of two e4m3 numbers of a row whose top is above 224: off by half a step of 2^-9 at most
+    check_attn(out[list(rows)], q[list(rows)], kc, ke, vc, ve, [table] * len(rows), [first + r + 1 for r in rows], scale, 2.0 ** -10 / 224)
+
+
+@pytest.mark.parametrize("Hq,H,D", [(32, 4, 128), (64, 4, 128), (8, 2, 64), (16, 2, 64), (3, 3, 128), (14, 2, 64), (5, 1, 128), (100, 1, 64), (128, 1, 128)])
+@pytest.mark.parametrize("n,first", [(1, 0), (1, 300), (17, 0), (50, 78), (33, 1000), (130, 127)])
+def test_prefill_heads(ops, Hq, H, D, n, first):
+    run_prefill(ops, n, first, Hq, H, D, seed=n + first, rows=[0, 1, 2, 15, 16, 31, 32, 49, n // 2, n - 2, n - 1])
+
+
+@pytest.mark.parametrize("Hq,H,D", [(8, 2, 128), (4, 2, 64)])
+@pytest.mark.parametrize("n,first", [(300, 0), (257, 5), (128, 128)])
+def test_prefill_every_row(ops, Hq, H, D, n, first):
+    run_prefill(ops, n, first, Hq, H, D, seed=n, width=5)
+
+
+@pytest.mark.parametrize("Hq,H,D,n,first", [(32, 4, 128, 1500, 100), (32, 4, 128, 2048, 0), (8, 8, 128, 700, 900), (16, 2, 64, 2000, 3000), (64, 4, 128, 40, 9001),
+                                            (8, 2, 64, 3, 12000)])
+def test_prefill_long(ops, Hq, H, D, n, first):
+    run_prefill(ops, n, first, Hq, H, D, seed=n, rows=[0, 1, 127, 128, n // 3, n // 2, n - 17, n - 1])
+
+
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("spread,q_size,scale", [(0, 1.0, 0.1), (20, 1.0, 0.1), (3, 30.0, 1.0), (3, 1e-30, 1.0), (3, 1e20, 1e-20), (25, 1e-6, 1.0)])
+def test_prefill_magnitudes(ops, D, spread, q_size, scale):
+    for n, first in ((40, 500), (300, 0)):
+        run_prefill(ops, n, first, 8, 2, D, seed=31, spread=spread, q_size=q_size, scale=scale, rows=range(0, n, 7))
+
+
+def test_prefill_findings_and_refusals(ops):
+    rng = np.random.default_rng(32)
+    q, kc, ke, vc, ve, table = attn_case(rng, [100], 8, 2, 64)
+    args = [plain.pool_of(kc), plain.pool_of(vc), plain.scale_of(ke), plain.scale_of(ve)]
+    q = torch.zeros(50, 8, 64, device=DEV, dtype=torch.bfloat16)
+    err = pkg("_lib").B200Error
+    for bad in (-1, kc.shape[0]):
+        t = torch.from_numpy(table[0].copy()).to(DEV)
+        t[2] = bad
+        ws = ops.kv8_attn_prefill_workspace(50, 50, 8, 2, 64, DEV)
+        ops.kv8_attn_prefill(q, *args, t, 50, 0.1, workspace=ws)
+        with pytest.raises(err, match="pool"):
+            ops.read_status(ws, "prefill")
+    row = torch.from_numpy(table[0]).to(DEV)
+    with pytest.raises(err, match="do not fit"):
+        ops.kv8_attn_prefill(q, *args, row, 16 * row.numel() - 49, 0.1)
+    with pytest.raises(err, match="workspace"):
+        ops.kv8_attn_prefill(q, *args, row, 50, 0.1, workspace=torch.zeros(128, dtype=torch.uint8, device=DEV))
+    for bad in (dict(q=q.float()), dict(q=q[0]), dict(table_row=row[None]), dict(table_row=row.long()), dict(out=q[:3]), dict(workspace=row)):
+        with pytest.raises(ValueError):
+            ops.kv8_attn_prefill(**(dict(q=q, k_pool=args[0], v_pool=args[1], k_scale=args[2], v_scale=args[3], table_row=row, first_pos=0, scale=0.1) | bad))
+    assert ops.kv8_attn_prefill(q[:0], *args, row, 50, 0.1).shape == (0, 8, 64)
+
+
+def test_prefill_agrees_with_decode(ops):
+    """The last row of a prompt is a decode row."""
+    rng = np.random.default_rng(33)
+    _, kc, ke, vc, ve, table = attn_case(rng, [777], 32, 4, 128)
+    args = [plain.pool_of(kc), plain.pool_of(vc), plain.scale_of(ke), plain.scale_of(ve)]
+    q = torch.randn(20, 32, 128, device=DEV).bfloat16()
+    t = torch.from_numpy(table).to(DEV)
+    a = ops.kv8_attn_prefill(q, *args, t[0], 757, 0.09)[19].float()
+    b = ops.kv8_attn_decode(q[19:].contiguous(), *args, t, ints([777]), 0.09)[0].float()
+    # both within half a bf16 step and 2^-11 of weights of the exact value
+    assert ((a - b).abs() <= 2.0 ** -7 * b.abs() + 2.0 ** -9 * b.abs().max()).all()
 
 
 # --------------------------------------------------------------- used together

@@ -93,6 +93,28 @@ def test_decode_refuses():
     refused(call(split=-16), "split_tokens -16")
 
 
+def test_prefill_refuses():
+    lib = pkg("_lib").load()
+
+    def call(q=P, kp=P, vp=P, ks=P, vs=P, table=P, out=P, ws=P, n=1 << 20, R=5, first=0, hq=8, hkv=2, dim=64, blocks=9, width=4, scale=0.1):
+        return lib.b200_kv8_attn_prefill(q, kp, vp, ks, vs, table, out, ws, n, R, first, hq, hkv, dim, blocks, width, scale, None)
+
+    for name in ("q", "kp", "vp", "ks", "vs", "table", "out", "ws"):
+        refused(call(**{name: None}), "null")
+    for name in ("R", "hq", "hkv", "blocks", "width"):
+        refused(call(**{name: 0}), "non-positive")
+    refused(call(hq=7), "multiple of kv heads")
+    refused(call(hq=258), "128 q heads")
+    refused(call(dim=96), "head_dim 96")
+    refused(call(first=-1), "positions -1")
+    refused(call(first=60), "do not fit 4 pages")
+    refused(call(first=2 ** 31 - 2), "do not fit")
+    refused(call(first=2 ** 31 - 100, R=50, width=2 ** 27 - 1), "2^31")
+    refused(call(scale=-0.1), "scale")
+    for name in ("q", "kp", "vp", "out"):
+        refused(call(**{name: P + 8}), "16-byte")
+
+
 def test_wrappers_refuse_what_is_not_on_a_gpu():
     ops = pkg("ops")
     i = torch.zeros(3, dtype=torch.int32)
@@ -104,3 +126,5 @@ def test_wrappers_refuse_what_is_not_on_a_gpu():
         ops.kv8_append(torch.zeros(3, 2, 64), torch.zeros(3, 2, 64), *pools, i)
     with pytest.raises(ValueError, match="CUDA"):
         ops.kv8_attn_decode(torch.zeros(3, 4, 64, dtype=torch.bfloat16), *pools, i.view(3, 1), i, 0.1)
+    with pytest.raises(ValueError, match="CUDA"):
+        ops.kv8_attn_prefill(torch.zeros(3, 4, 64, dtype=torch.bfloat16), *pools, i, 0, 0.1)
