@@ -117,8 +117,10 @@ __device__ __forceinline__ bool mbar_test(uint32_t bar, uint32_t parity) {
       : "memory");
   return ok != 0;
 }
-// Bounded wait: gives up after roughly a second and flags the error word.
+// Bounded wait: gives up after roughly a second and flags the error word.  Not to be unrolled: a dozen unrolled waits were half of a prompt
+// attention kernel's 100 to 130 KB of code, more than the instruction caches hold next to its straight-line loops.
 __device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity, int* err) {
+#pragma unroll 1
   for (uint32_t i = 0; i < (1u << 21); ++i) {
     if (mbar_try_wait(bar, parity)) return true;
     if (i > 2048) __nanosleep(128);
@@ -128,6 +130,7 @@ __device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity, int* er
 }
 // The same for a whole converged warp: true if no lane's wait ran out.
 __device__ __forceinline__ bool mbar_wait_warp(uint32_t bar, uint32_t parity, int* err) {
+#pragma unroll 1
   for (uint32_t i = 0; i < (1u << 21); ++i) {
     if (__all_sync(0xffffffffu, mbar_try_wait(bar, parity))) return true;
     if (i > 2048) __nanosleep(128);

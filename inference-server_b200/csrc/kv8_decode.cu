@@ -48,13 +48,6 @@ __device__ __forceinline__ uint32_t transpose_8x8(uint32_t x) {
   asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
   return y;
 }
-template <int BYTES>
-__device__ __forceinline__ void lds_words(uint32_t addr, uint32_t* w) {
-  if constexpr (BYTES == 16)
-    asm volatile("ld.shared.v4.b32 {%0,%1,%2,%3}, [%4];" : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3]) : "r"(addr));
-  else
-    asm volatile("ld.shared.v2.b32 {%0,%1}, [%2];" : "=r"(w[0]), "=r"(w[1]) : "r"(addr));
-}
 
 // D: head_dim.  HKV: kv heads = consumer warps.  NT: tiles of 8 query heads per kv head.  PPS: pages per stage.
 template <int D, int HKV, int NT, int PPS, int STAGES>

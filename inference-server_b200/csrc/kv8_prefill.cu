@@ -10,14 +10,15 @@
 //               but for the ends of the range (rows are brought to a top of 256 to 448; a query 2^-7 of the row's largest
 //               or smaller loses bits below 2^-19 of it).  Two products of twice the rate cost what one in 16 bits does, and keys need neither conversion
 //               nor room in 16 bits.
-//   P V         kind::f16: weights are f16 in TMEM (11 bits), values are converted to f16 (exactly) by a warp of their own and
+//   P V         kind::f16: weights are f16 in TMEM (11 bits), values are converted to f16 (exactly) by two warps and
 //               stored as MN-major swizzled tiles.  A conversion serves both tiles of rows.
 //
 //   grid     (CTAs of tiles, late ones first) x splits of the keys x kv heads.  The keys are split where the tiles alone leave SMs idle; fp32
 //            partials are then joined by kv8_attn_join_kernel.
 //   warp 0   producer: per key tile, 8 pages of keys by TMA and 8 of values as plain bulk copies, two stages each.
+//   warps 0, 3   half of a tile's values each: 16 bytes of a row to 16 f16 numbers; zero for what lies behind the last token, where a page
+//            may hold NaN.
 //   warp 1   S issuer (one thread), warp 2 P V issuer (one thread).
-//   warp 3   values: 16 bytes of a row to 16 f16 numbers; zero for what lies behind the last token, where a page may hold NaN.
 //   warps 4-7, 8-11   first the queries of both tiles (bf16 to hi and lo, a row's top by shuffles), then the softmax of tile 0 and of tile 1,
 //            a thread per score row; the scales of a key tile's 8 pages come to each warp by its own lanes, two key tiles
 //            ahead (ids) and one (scales), and from a corner of shared memory to all lanes.
@@ -83,6 +84,48 @@ __device__ __forceinline__ float max_of_3(float a, float b, float c) {
   return d;
 }
 
+// One warp's half of a tile of values, rows row0 .. row0 + 63, to f16; those from `rows` on hold no tokens and become zero (a page may hold
+// NaN there).  A lane takes 16 bytes of a row at a time, which become two pieces of a swizzled row.  For head_dim 128 a quarter warp
+// takes the first half of one row and the second half of the next: its loads are in different banks, and so are its stores,
+// whose pieces are XORed with numbers that differ in bit 0.  The loop is short code on purpose: unrolled it took 2900 cycles a half tile, nearly all
+// of them waits for instructions, which the softmax warps' long straight-line code keeps out of the instruction cache.
+template <int D>
+__device__ __forceinline__ void values_to_f16(uint32_t from, uint32_t to, int row0, int rows, int lane) {
+  constexpr int kPieces = D / 16, kRowsAt = 32 / kPieces;  // pieces of a row; rows that the warp takes at a time
+  constexpr uint32_t kAtomGroup = D / 64 * 1024;           // 8 rows of f16
+  if (rows < row0 + kTcKeys / 2) {
+    for (int i = max(rows, row0) * kPieces + lane; i < (row0 + kTcKeys / 2) * kPieces; i += 32)
+      asm volatile("st.shared.v4.b32 [%0], {%1,%1,%1,%1};" ::"r"(from + i * 16), "r"(0) : "memory");
+    __syncwarp();
+  }
+  const int odd = (lane >> 2) & 1;
+  const int c = D == 128 ? (lane & 3) + 4 * (((lane >> 3) & 1) ^ odd) : lane & 3;
+  const int lr = D == 128 ? 2 * (lane >> 4) + odd : lane >> 2;
+  const uint32_t half_off = (c >> 2) * 1024;
+  const int piece = (2 * c) & 7;
+  uint32_t src = from + (row0 + lr) * D + c * 16;
+  uint32_t w[4];
+  lds_words<16>(src, w);
+#pragma unroll 2
+  for (int r = row0 + lr; r < row0 + kTcKeys / 2; r += kRowsAt) {
+    uint32_t x[4], a[8];
+#pragma unroll
+    for (int k = 0; k < 4; ++k) x[k] = w[k];
+    src += kRowsAt * D;
+    if (r + kRowsAt < row0 + kTcKeys / 2) lds_words<16>(src, w);
+#pragma unroll
+    for (int k = 0; k < 4; ++k) e4m3x4_to_f16(x[k], a[2 * k], a[2 * k + 1]);
+    const uint32_t row = to + (r >> 3) * kAtomGroup + half_off;
+#pragma unroll
+    for (int k = 0; k < 2; ++k)
+      asm volatile("st.shared.v4.b32 [%0], {%1,%2,%3,%4};" ::"r"(row + swz128(r & 7, piece + k)), "r"(a[4 * k]), "r"(a[4 * k + 1]), "r"(a[4 * k + 2]),
+                   "r"(a[4 * k + 3])
+                   : "memory");
+  }
+  fence_proxy_async();  // the tensor core reads the tile, and the next copy writes the stage, through the async proxy
+  __syncwarp();
+}
+
 template <int D>
 __global__ void __launch_bounds__(kKv8PrefillThreads, 1)
 kv8_attn_prefill_kernel(const __grid_constant__ CUtensorMap k_map, const uint8_t* __restrict__ v_pool, const uint8_t* __restrict__ k_scale,
@@ -119,8 +162,8 @@ kv8_attn_prefill_kernel(const __grid_constant__ CUtensorMap k_map, const uint8_t
       mbar_init(bar_kfull + 8 * s, 1);
       mbar_init(bar_kempty + 8 * s, 1);
       mbar_init(bar_rawfull + 8 * s, 1);
-      mbar_init(bar_rawempty + 8 * s, 1);
-      mbar_init(bar_vfull + 8 * s, 1);
+      mbar_init(bar_rawempty + 8 * s, 2);
+      mbar_init(bar_vfull + 8 * s, 2);
       mbar_init(bar_vempty + 8 * s, 1);
       mbar_init(bar_sfull + 8 * s, 1);
       mbar_init(bar_odone + 8 * s, 1);
@@ -161,81 +204,48 @@ kv8_attn_prefill_kernel(const __grid_constant__ CUtensorMap k_map, const uint8_t
 
   if (warp < 4) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
-    if (warp == 0) {
-      // ------------------------------------------------- pages ------
-      // Lane i of the first 8 owns page i of a tile's keys, of the second 8 that of its values.
+    if (warp == 0 || warp == 3) {
+      // ------------------------------------------------- pages, V in f16 ------
+      // Warp 0 issues the copies of a key tile - lane i of the first 8 page i of its keys, of the second 8 that of its values - and then
+      // takes rows 64.. of the values of the tile before; warp 3 takes rows 0..63.
       const int pg = lane & 7;
       bool alive = true;
 #pragma unroll 1
-      for (int j = 0; j < n_tiles; ++j) {
-        const int st = j & 1;
-        // the last page stands in for those behind it, so that every stage is the same number of bytes
-        int page = __ldg(table_row + min((kt0 + j) * kTcPages + pg, last_page));
-        if (page < 0 || page >= num_blocks) {
-          set_error(err, kErrDevBadBlockId);
-          page = 0;
-        }
-        const size_t cell = static_cast<size_t>(page) * num_kv_heads + h;
-        if (alive) alive = mbar_wait(bar_kempty + 8 * st, ((j >> 1) & 1) ^ 1, err);
-        if (!__all_sync(0xffffffffu, alive)) break;
-        if (lane == 0) mbar_arrive_expect_tx(bar_kfull + 8 * st, Cfg::kTile8);
-        __syncwarp();
-        if (lane < kTcPages)
-          tma_load_2d(base + Cfg::kK + st * Cfg::kTile8 + pg * kPageBytes8, &k_map, bar_kfull + 8 * st, 0, static_cast<int>(cell) * kKvPage);
-        if (alive) alive = mbar_wait(bar_rawempty + 8 * st, ((j >> 1) & 1) ^ 1, err);
-        if (!__all_sync(0xffffffffu, alive)) break;
-        if (lane == 0) mbar_arrive_expect_tx(bar_rawfull + 8 * st, Cfg::kTile8);
-        __syncwarp();
-        if (lane >= 8 && lane < 16)
-          bulk_load(base + Cfg::kRaw + st * Cfg::kTile8 + pg * kPageBytes8, v_pool + cell * kPageBytes8, kPageBytes8, bar_rawfull + 8 * st);
-      }
-    } else if (warp == 3) {
-      // ------------------------------------------------- V in f16 ------
-      // A lane takes 16 bytes of a row at a time.  Their 32 bytes in f16 are two pieces of a swizzled row; the lanes of the second
-      // column half store theirs in the other order, so that a quarter warp's pieces lie in different banks.
-      constexpr int kPieces = D / 16, kRowsAt = 32 / kPieces;  // pieces of a row; rows that the warp takes at a time
-      const int c = lane % kPieces, lr = lane / kPieces;
-      const uint32_t half_off = (c >> 2) * 1024;
-      const int first_piece = (2 * c) & 7, swap = D == 128 ? c >> 2 : 0;
-      bool alive = true;
-#pragma unroll 1
-      for (int j = 0; j < n_tiles && alive; ++j) {
-        const int st = j & 1;
-        alive = mbar_wait(bar_rawfull + 8 * st, (j >> 1) & 1, err) && mbar_wait(bar_vempty + 8 * st, ((j >> 1) & 1) ^ 1, err);
-        if (!__all_sync(0xffffffffu, alive)) break;
-        const uint32_t from = base + Cfg::kRaw + st * Cfg::kTile8, to = base + Cfg::kV + st * Cfg::kTile16;
-        const int rows = last_pos - (kt0 + j) * kTcKeys + 1;  // of them hold tokens
-#pragma unroll 1
-        for (int r0 = 0; r0 < kTcKeys; r0 += 4 * kRowsAt) {
-          uint32_t w[4][4];
-#pragma unroll
-          for (int u = 0; u < 4; ++u) {
-            const int r = r0 + u * kRowsAt + lr;
-            asm volatile("ld.shared.v4.b32 {%0,%1,%2,%3}, [%4];"
-                         : "=r"(w[u][0]), "=r"(w[u][1]), "=r"(w[u][2]), "=r"(w[u][3]) : "r"(from + r * D + c * 16) : "memory");
-            if (r >= rows) w[u][0] = w[u][1] = w[u][2] = w[u][3] = 0u;
+      for (int j = 0; j < n_tiles + 1; ++j) {
+        if (warp == 0 && j < n_tiles) {
+          const int st = j & 1;
+          // the last page stands in for those behind it, so that every stage is the same number of bytes
+          int page = __ldg(table_row + min((kt0 + j) * kTcPages + pg, last_page));
+          if (page < 0 || page >= num_blocks) {
+            set_error(err, kErrDevBadBlockId);
+            page = 0;
           }
-#pragma unroll
-          for (int u = 0; u < 4; ++u) {
-            const int r = r0 + u * kRowsAt + lr;
-            uint32_t a[2][4];
-#pragma unroll
-            for (int k = 0; k < 4; ++k) e4m3x4_to_f16(w[u][k], a[k >> 1][(k & 1) * 2], a[k >> 1][(k & 1) * 2 + 1]);
-            const uint32_t row = to + (r >> 3) * kAtomGroup + half_off;
-#pragma unroll
-            for (int k = 0; k < 2; ++k) {
-              const int which = k ^ swap;
-              asm volatile("st.shared.v4.b32 [%0], {%1,%2,%3,%4};" ::"r"(row + swz128(r & 7, first_piece + which)), "r"(which ? a[1][0] : a[0][0]),
-                           "r"(which ? a[1][1] : a[0][1]), "r"(which ? a[1][2] : a[0][2]), "r"(which ? a[1][3] : a[0][3])
-                           : "memory");
-            }
-          }
+          const size_t cell = static_cast<size_t>(page) * num_kv_heads + h;
+          if (alive) alive = mbar_wait(bar_kempty + 8 * st, ((j >> 1) & 1) ^ 1, err);
+          if (!__all_sync(0xffffffffu, alive)) break;
+          if (lane == 0) mbar_arrive_expect_tx(bar_kfull + 8 * st, Cfg::kTile8);
+          __syncwarp();
+          if (lane < kTcPages)
+            tma_load_2d(base + Cfg::kK + st * Cfg::kTile8 + pg * kPageBytes8, &k_map, bar_kfull + 8 * st, 0, static_cast<int>(cell) * kKvPage);
+          if (alive) alive = mbar_wait(bar_rawempty + 8 * st, ((j >> 1) & 1) ^ 1, err);
+          if (!__all_sync(0xffffffffu, alive)) break;
+          if (lane == 0) mbar_arrive_expect_tx(bar_rawfull + 8 * st, Cfg::kTile8);
+          __syncwarp();
+          if (lane >= 8 && lane < 16)
+            bulk_load(base + Cfg::kRaw + st * Cfg::kTile8 + pg * kPageBytes8, v_pool + cell * kPageBytes8, kPageBytes8, bar_rawfull + 8 * st);
         }
-        fence_proxy_async();  // the tensor core reads the tile, and the next copy writes the stage, through the async proxy
-        __syncwarp();
-        if (lane == 0) {
-          mbar_arrive(bar_vfull + 8 * st);
-          mbar_arrive(bar_rawempty + 8 * st);
+        const int jv = warp == 0 ? j - 1 : j;
+        if (jv >= 0 && jv < n_tiles) {
+          const int st = jv & 1;
+          if (alive) alive = mbar_wait(bar_rawfull + 8 * st, (jv >> 1) & 1, err);
+          if (alive) alive = mbar_wait(bar_vempty + 8 * st, ((jv >> 1) & 1) ^ 1, err);
+          if (!__all_sync(0xffffffffu, alive)) break;
+          values_to_f16<D>(base + Cfg::kRaw + st * Cfg::kTile8, base + Cfg::kV + st * Cfg::kTile16, warp == 0 ? kTcKeys / 2 : 0,
+                           last_pos - (kt0 + jv) * kTcKeys + 1, lane);
+          if (lane == 0) {
+            mbar_arrive(bar_vfull + 8 * st);
+            mbar_arrive(bar_rawempty + 8 * st);
+          }
         }
       }
     } else if (warp == 1) {
@@ -249,19 +259,18 @@ kv8_attn_prefill_kernel(const __grid_constant__ CUtensorMap k_map, const uint8_t
           const int st = j & 1;
           alive = mbar_wait(bar_kfull + 8 * st, (j >> 1) & 1, err);
           const uint64_t b0 = desc_k8<D>(base + Cfg::kK + st * Cfg::kTile8);
-#pragma unroll
+#pragma unroll 1
           for (int t = 0; t < 2; ++t) {
-            if (j >= n_of[t]) continue;  // none of this tile's rows sees these keys
+            if (j >= (t ? n_of[1] : n_of[0])) continue;  // none of this tile's rows sees these keys
             if (alive) alive = mbar_wait(bar_sempty, (n & 1) ^ 1, err);
             if (!alive) break;
             ++n;
             tc_fence_after();
-#pragma unroll
-            for (int part = 0; part < 2; ++part) {
-              const uint64_t a0 = desc_k8<D>(base + Cfg::kQ + (2 * t + part) * Cfg::kTile8);
-#pragma unroll
-              for (int k = 0; k < D / 32; ++k) tc_mma_f8(tmem_s, a0 + 2 * k, b0 + 2 * k, idesc_s, part + k > 0 ? 1u : 0u);
-            }
+            uint64_t a = desc_k8<D>(base + Cfg::kQ + 2 * t * Cfg::kTile8);
+#pragma unroll 1
+            for (int part = 0; part < 2; ++part, a += Cfg::kTile8 >> 4)
+#pragma unroll 1
+              for (int k = 0; k < D / 32; ++k) tc_mma_f8(tmem_s, a + 2 * k, b0 + 2 * k, idesc_s, part + k > 0 ? 1u : 0u);
             tc_commit(bar_sfull + 8 * t);
           }
           tc_commit(bar_kempty + 8 * st);
@@ -275,19 +284,18 @@ kv8_attn_prefill_kernel(const __grid_constant__ CUtensorMap k_map, const uint8_t
       for (int j = 0; j < n_tiles && alive; ++j) {
         const int st = j & 1;
         alive = mbar_wait(bar_vfull + 8 * st, (j >> 1) & 1, err);
-#pragma unroll
+#pragma unroll 1
         for (int t = 0; t < 2; ++t) {
-          if (j >= n_of[t]) continue;
-#pragma unroll
-          for (int half = 0; half < 2; ++half) {
-            if (alive) alive = mbar_wait(bar_pfull + 16 * t + 8 * half, j & 1, err);
-            if (!alive) break;
-            tc_fence_after();
-#pragma unroll
-            for (int kk = half * 4; kk < half * 4 + 4; ++kk) {  // 16 keys each
-              const uint64_t b = umma_desc_mn128(base + Cfg::kV + st * Cfg::kTile16 + kk * kPageBytes16, 1024, kAtomGroup);
-              mma_f16_ts(tmem_o + t * kTcKeys, tmem_p + t * 64 + kk * 8, b, idesc_o, (j > 0 || kk > 0) ? 1u : 0u);
+          if (j >= (t ? n_of[1] : n_of[0])) continue;
+#pragma unroll 1
+          for (int kk = 0; kk < kTcPages; ++kk) {  // 16 keys each
+            if ((kk & 3) == 0) {
+              if (alive) alive = mbar_wait(bar_pfull + 16 * t + 2 * kk, j & 1, err);
+              if (!alive) break;
+              tc_fence_after();
             }
+            const uint64_t b = umma_desc_mn128(base + Cfg::kV + st * Cfg::kTile16 + kk * kPageBytes16, 1024, kAtomGroup);
+            mma_f16_ts(tmem_o + t * kTcKeys, tmem_p + t * 64 + kk * 8, b, idesc_o, (j > 0 || kk > 0) ? 1u : 0u);
           }
           tc_commit(bar_odone + 8 * t);
         }
@@ -316,20 +324,27 @@ kv8_attn_prefill_kernel(const __grid_constant__ CUtensorMap k_map, const uint8_t
     int kb = k_scale[static_cast<size_t>(id) * num_kv_heads + h], vb = v_scale[static_cast<size_t>(id) * num_kv_heads + h];
     id = page_id(1);
 
-    // Q tiles: neighbouring threads neighbouring pieces of 8 numbers of a row
-    for (int u = 0; u < own; ++u) {
-      uint4 v[D / 16];
-#pragma unroll
-      for (int k = 0; k < D / 16; ++k) {
-        const int i = threadIdx.x - 128 + k * 256, qr = i / (D / 8), qt_l = qr / gr, tok = t0 + u * QT + qt_l;
-        v[k] = make_uint4(0u, 0u, 0u, 0u);
-        if (qt_l < QT && tok < num_tokens)
-          v[k] = *reinterpret_cast<const uint4*>(q + (static_cast<size_t>(tok) * num_q_heads + h * gr + (qr - qt_l * gr)) * D + i % (D / 8) * 8);
-      }
-#pragma unroll
-      for (int k = 0; k < D / 16; ++k) {
-        const int i = threadIdx.x - 128 + k * 256, qr = i / (D / 8), ch = i % (D / 8);
-        const uint32_t x[4] = {v[k].x, v[k].y, v[k].z, v[k].w};
+    // Q tiles: neighbouring threads neighbouring pieces of 8 numbers of a row, 16 to 32 rows at a time and four such steps on their way.  One
+    // loop over all steps of both tiles: code that runs once has to be fetched first, and unrolled it was 16 KB.
+    {
+      constexpr int kSteps = D / 16;  // of a tile
+      const int ch = threadIdx.x % (D / 8), qr0 = (threadIdx.x - 128) / (D / 8);
+      auto load = [&](int step) {
+        const int qr = step % kSteps * (2048 / D) + qr0, qt_l = qr / gr, tok = t0 + step / kSteps * QT + qt_l;
+        uint4 x = make_uint4(0u, 0u, 0u, 0u);
+        if (step < own * kSteps && qt_l < QT && tok < num_tokens)
+          x = *reinterpret_cast<const uint4*>(q + (static_cast<size_t>(tok) * num_q_heads + h * gr + (qr - qt_l * gr)) * D + ch * 8);
+        return x;
+      };
+      uint4 v[4] = {load(0), load(1), load(2), load(3)};
+#pragma unroll 1
+      for (int step = 0; step < own * kSteps; ++step) {
+        const uint32_t x[4] = {v[0].x, v[0].y, v[0].z, v[0].w};
+        v[0] = v[1];
+        v[1] = v[2];
+        v[2] = v[3];
+        v[3] = load(step + 4);
+        const int u = step / kSteps, qr = step % kSteps * (2048 / D) + qr0;
         uint32_t top = 0;
 #pragma unroll
         for (int w = 0; w < 4; ++w) top = max(top, max((x[w] & 0x7fff0000u), (x[w] & 0x7fffu) << 16));
@@ -419,7 +434,7 @@ kv8_attn_prefill_kernel(const __grid_constant__ CUtensorMap k_map, const uint8_t
           // a row that has seen no key yet holds exact zeros
           const float alpha = m_new == -INFINITY ? 1.f : fast_exp2(m_run - m_new);
           l_run *= alpha;
-#pragma unroll
+#pragma unroll 1
           for (int c0 = 0; c0 < D; c0 += 32) {
             uint32_t o[32];
             tmem_ld32(o_acc + c0, o);
