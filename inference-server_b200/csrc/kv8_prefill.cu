@@ -126,6 +126,28 @@ __device__ __forceinline__ void values_to_f16(uint32_t from, uint32_t to, int ro
   __syncwarp();
 }
 
+// Two fp32 numbers in one instruction.
+__device__ __forceinline__ uint64_t pair_of(float lo, float hi) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(lo), "f"(hi));
+  return r;
+}
+__device__ __forceinline__ float2 halves(uint64_t v) {
+  float2 r;
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(v));
+  return r;
+}
+__device__ __forceinline__ uint64_t fma_pair(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t d;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
+  return d;
+}
+__device__ __forceinline__ uint64_t add_pair(uint64_t a, uint64_t b) {
+  uint64_t d;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+  return d;
+}
+
 template <int D>
 __global__ void __launch_bounds__(kKv8PrefillThreads, 1)
 kv8_attn_prefill_kernel(const __grid_constant__ CUtensorMap k_map, const uint8_t* __restrict__ v_pool, const uint8_t* __restrict__ k_scale,
@@ -454,21 +476,26 @@ kv8_attn_prefill_kernel(const __grid_constant__ CUtensorMap k_map, const uint8_t
 #pragma unroll
         for (int p = 0; p < 4; ++p) {
           const float4 w = sc[half * 4 + p];
-          const float f = f_q * w.x, off = w.y - mb;
-          float sum[2];
+          const uint64_t f = pair_of(f_q * w.x, f_q * w.x), off = pair_of(w.y - mb, w.y - mb);
+          uint64_t sum[2];
 #pragma unroll
           for (int ch = 0; ch < 2; ++ch) {
             // asked here, needed behind this half: P was last read by the product of the tile before; the next S
             if (p == 2 && ch == 1 && half == 0 && i > 0) p_free = mbar_test(odone, (i - 1) & 1);
             if (p == 2 && ch == 1 && half == 1) s_ready = mbar_test(sfull, (i + 1) & 1);
-            float e[8];
+            const float* x = s + half * 64 + p * 16 + ch * 8;
+            uint64_t e[4];
 #pragma unroll
-            for (int k = 0; k < 8; ++k) e[k] = fast_exp2(fmaf(s[half * 64 + p * 16 + ch * 8 + k], f, off));
-            sum[ch] = ((e[0] + e[1]) + (e[2] + e[3])) + ((e[4] + e[5]) + (e[6] + e[7]));
-#pragma unroll
-            for (int k = 0; k < 4; ++k) pk[p * 8 + ch * 4 + k] = pack_f16x2(e[2 * k], e[2 * k + 1]);
+            for (int k = 0; k < 4; ++k) {
+              const float2 t2 = halves(fma_pair(pair_of(x[2 * k], x[2 * k + 1]), f, off));
+              const float lo = fast_exp2(t2.x), hi = fast_exp2(t2.y);
+              pk[p * 8 + ch * 4 + k] = pack_f16x2(lo, hi);
+              e[k] = pair_of(lo, hi);
+            }
+            sum[ch] = add_pair(add_pair(e[0], e[1]), add_pair(e[2], e[3]));
           }
-          l_run = fmaf(sum[0] + sum[1], w.z, l_run);
+          const float2 both = halves(add_pair(sum[0], sum[1]));
+          l_run = fmaf(both.x + both.y, w.z, l_run);
         }
         if (half == 0 && !__all_sync(0xffffffffu, p_free) && alive) alive = mbar_wait(odone, (i - 1) & 1, err);
         tc_fence_after();
