@@ -21,8 +21,12 @@ def _ptr(t: torch.Tensor | None):
     return None if t is None else t.data_ptr()
 
 
+# The handle without a Stream object around it: 0.1 us in place of 3 in calls whose kernels take 4.
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+
+
 def _stream() -> int:
-    return torch.cuda.current_stream().cuda_stream
+    return torch.cuda.current_stream().cuda_stream if _raw_stream is None else _raw_stream(torch.cuda.current_device())
 
 
 def _need(t: torch.Tensor, name: str, dtype=None):
@@ -202,14 +206,15 @@ class KvSlotMap(NamedTuple):
     supply_used: torch.Tensor
 
 
-def _on_current_device(t: torch.Tensor, *others: torch.Tensor) -> None:
+_device_index = torch.Tensor.get_device
+
+
+def _on_current_device(*operands: torch.Tensor) -> None:
     """The kernels run on the current device's current stream: operands of another device are an error and not a fault."""
-    device = t.device
-    if device.index != torch.cuda.current_device():
-        raise ValueError(f"operands are on {device}, the current device is cuda:{torch.cuda.current_device()}")
-    for o in others:
-        if o.device != device:
-            raise ValueError(f"operands are on {device} and {o.device}")
+    if set(map(_device_index, operands)) != {torch.cuda.current_device()}:
+        for t in operands:
+            if t.get_device() != torch.cuda.current_device():
+                raise ValueError(f"an operand is on {t.device}, the current device is cuda:{torch.cuda.current_device()}")
 
 
 def _status_word(status: torch.Tensor | None) -> None:
@@ -227,14 +232,18 @@ def kv8_pools(num_blocks: int, num_kv_heads: int, head_dim: int, device="cuda"):
 
 
 def _kv8_cache(k_pool, v_pool, k_scale, v_scale) -> tuple[int, int, int]:
-    _need(k_pool, "k_pool", KV8_DTYPE)
-    _need(v_pool, "v_pool", KV8_DTYPE)
-    _need(k_scale, "k_scale", KV8_SCALE_DTYPE)
-    _need(v_scale, "v_scale", KV8_SCALE_DTYPE)
-    if k_pool.dim() != 4 or k_pool.shape[2] != 16:
-        raise ValueError(f"k_pool must be [num_blocks, kv_heads, 16, head_dim], got {list(k_pool.shape)}")
-    nb, Hkv, _, D = k_pool.shape
-    if v_pool.shape != k_pool.shape or k_scale.shape != (nb, Hkv) or v_scale.shape != (nb, Hkv):
+    shape = k_pool.shape
+    if not (k_pool.dtype is KV8_DTYPE and v_pool.dtype is KV8_DTYPE and k_scale.dtype is KV8_SCALE_DTYPE and v_scale.dtype is KV8_SCALE_DTYPE
+            and k_pool.is_contiguous() and v_pool.is_contiguous() and k_scale.is_contiguous() and v_scale.is_contiguous()
+            and k_pool.is_cuda and v_pool.is_cuda and k_scale.is_cuda and v_scale.is_cuda):
+        _need(k_pool, "k_pool", KV8_DTYPE)
+        _need(v_pool, "v_pool", KV8_DTYPE)
+        _need(k_scale, "k_scale", KV8_SCALE_DTYPE)
+        _need(v_scale, "v_scale", KV8_SCALE_DTYPE)
+    if len(shape) != 4 or shape[2] != 16:
+        raise ValueError(f"k_pool must be [num_blocks, kv_heads, 16, head_dim], got {list(shape)}")
+    nb, Hkv, _, D = shape
+    if v_pool.shape != shape or k_scale.shape != (nb, Hkv) or v_scale.shape != (nb, Hkv):
         raise ValueError("pools and scales do not match each other")
     return nb, Hkv, D
 
@@ -255,7 +264,7 @@ def kv_slot_map(ctx_lens, new_lens, block_table, supply, supply_used, num_rows: 
         raise ValueError("lengths, block table or supply_used do not match")
     if R < 0:
         raise ValueError(f"{R} rows")
-    m = KvSlotMap(*torch.empty(2 * B + 2 + 3 * R, dtype=torch.int32, device=ctx_lens.device).split((B, B + 1, R, R, R, 1)))
+    m = KvSlotMap(*torch.split_with_sizes(ctx_lens.new_empty(2 * B + 2 + 3 * R), (B, B + 1, R, R, R, 1)))
     rc = _lib.load().b200_kv_slot_map(
         _ptr(ctx_lens), _ptr(new_lens), _ptr(block_table), _ptr(supply), _ptr(supply_used), supply.numel(), _ptr(m.lens),
         _ptr(m.row_start), _ptr(m.row_seq), _ptr(m.positions), _ptr(m.slots), _ptr(m.supply_used), _ptr(status), B, R,
@@ -291,6 +300,15 @@ def kv8_append(k_new, v_new, k_pool, v_pool, k_scale, v_scale, slots, status: to
     check(rc, "b200_kv8_append")
 
 
+def _attn_out(q: torch.Tensor, out: torch.Tensor | None) -> torch.Tensor:
+    if out is None:
+        return torch.empty_like(q)
+    _need(out, "out", torch.bfloat16)
+    if out.shape != q.shape:
+        raise ValueError("out does not match q")
+    return out
+
+
 def kv8_attn_workspace(batch: int, num_q_heads: int, num_kv_heads: int, head_dim: int, max_pages: int, device,
                        split_tokens: int = 0) -> torch.Tensor:
     """Workspace of `kv8_attn_decode`, starting with the status word; kept for all steps of a batch shape."""
@@ -311,20 +329,13 @@ def kv8_attn_decode(q, k_pool, v_pool, k_scale, v_scale, block_table, ctx_lens, 
     B, Hq, _ = q.shape
     if block_table.dim() != 2 or block_table.shape[0] != B or ctx_lens.shape != (B,):
         raise ValueError("block_table / ctx_lens batch mismatch")
-    if out is None:
-        out = torch.empty_like(q)
-    else:
-        _need(out, "out", torch.bfloat16)
-        if out.shape != q.shape:
-            raise ValueError("out does not match q")
-    _on_current_device(q, k_pool, v_pool, k_scale, v_scale, block_table, ctx_lens, out)
+    out = _attn_out(q, out)
     if B == 0:
         return out
     if workspace is None:
         workspace = kv8_attn_workspace(B, Hq, Hkv, D, block_table.shape[1], q.device, int(split_tokens))
-    else:
-        _need(workspace, "workspace", torch.uint8)
-        _on_current_device(workspace)
+    _need(workspace, "workspace", torch.uint8)
+    _on_current_device(q, k_pool, v_pool, k_scale, v_scale, block_table, ctx_lens, out, workspace)
     rc = _lib.load().b200_kv8_attn_decode(
         _ptr(q), _ptr(k_pool), _ptr(v_pool), _ptr(k_scale), _ptr(v_scale), _ptr(block_table), _ptr(ctx_lens), _ptr(out),
         _ptr(workspace), workspace.numel(), B, Hq, Hkv, D, nb, block_table.shape[1], float(scale), int(split_tokens), _stream())
@@ -351,20 +362,13 @@ def kv8_attn_prefill(q, k_pool, v_pool, k_scale, v_scale, table_row, first_pos: 
     if table_row.dim() != 1:
         raise ValueError("table_row must be one row of a block table")
     R, Hq, _ = q.shape
-    if out is None:
-        out = torch.empty_like(q)
-    else:
-        _need(out, "out", torch.bfloat16)
-        if out.shape != q.shape:
-            raise ValueError("out does not match q")
-    _on_current_device(q, k_pool, v_pool, k_scale, v_scale, table_row, out)
+    out = _attn_out(q, out)
     if R == 0:
         return out
     if workspace is None:
         workspace = kv8_attn_prefill_workspace(R, int(first_pos), Hq, Hkv, D, q.device)
-    else:
-        _need(workspace, "workspace", torch.uint8)
-        _on_current_device(workspace)
+    _need(workspace, "workspace", torch.uint8)
+    _on_current_device(q, k_pool, v_pool, k_scale, v_scale, table_row, out, workspace)
     rc = _lib.load().b200_kv8_attn_prefill(
         _ptr(q), _ptr(k_pool), _ptr(v_pool), _ptr(k_scale), _ptr(v_scale), _ptr(table_row), _ptr(out), _ptr(workspace), workspace.numel(),
         R, int(first_pos), Hq, Hkv, D, nb, table_row.numel(), float(scale), _stream())
