@@ -245,8 +245,8 @@ int b200_kv_append(const void* k_new, const void* v_new, void* k_pool, void* v_p
  * are left as they were.  Numbers are rounded to nearest even; infinities and NaN become NaN.
  *
  * b200_kv8_attn_decode: softmax(q K^T * scale) V, one query row per sequence over its pages.  q, out [batch, num_q_heads, head_dim] bf16, any
- * number of query heads per kv head.  scale > 0.  workspace: b200_kv8_attn_workspace_bytes bytes, 16-byte aligned, starting with the status word;
- * calls that share it must not overlap.  split_tokens: tokens per CTA, a multiple of 16; 0: the library's choice, the same for
+ * number of query heads per kv head.  scale > 0.  The pages of all rows are cut into equal runs, one per CTA.  workspace:
+ * b200_kv8_attn_workspace_bytes bytes, 16-byte aligned, starting with the status word; calls that share it must not overlap.  split_tokens: tokens of a run at least, a multiple of 16; 0: the library's choice, the same for
  * both calls.  A row without tokens is zero.  Pages behind a row's last token are not read, and what the last page
  * holds behind it does not matter, NaN included.
  *

@@ -113,8 +113,7 @@ inline AttnWorkspace carve(void* ws, int batch, int hq, int D, int max_splits) {
 // Argument checks that the attention entry points of the 8-bit page cache share; joining their partials (kv8_decode.cu).
 int check_kv8(const char* name, int rows, int hq, int hkv, int head_dim, int num_blocks, int max_pages, const void* q, const void* k_pool,
               const void* v_pool, const void* out, float scale);
-int launch_kv8_join(int head_dim, const AttnWorkspace& w, const int* ctx_lens, void* out, int rows, int hq, int max_splits, int split_tokens,
-                    int max_ctx, cudaStream_t st);
+int launch_kv8_join(int head_dim, const AttnWorkspace& w, void* out, int rows, int hq, int parts, cudaStream_t st);
 
 }  // namespace b200
 

@@ -10,21 +10,31 @@
 // the largest is between 2^6 and 2^14; those below 2^-14 lose bits.  Queries are multiplied by a power of two that brings the largest of a kv group to 2^14 and become f16: what loses bits
 // is 2^-28 of the largest.  Sums are fp32.  With |ev| <= 32 the sums p_t 2^-ev stay below 2^14 * 2^32 * tokens.
 //
-//   grid   (batch, splits, groups of kv heads x slices of 16 query heads); block = one consumer warp per kv head + a producer warp.  A
-//          CTA owns `split_tokens` tokens of a sequence; the kv heads of a page are adjacent, so a page is one contiguous read of
-//          16 * HKV * D bytes for the keys and one for the values.
-//   load   TMA boxes of 128-byte rows with 128-byte swizzle into a ring of stages of PPS pages.
+//   work   The pages of all rows, one row after the other, are cut into equal runs, one per CTA (2 per SM for 4 kv heads of 128), wherever
+//          that falls in a row: every CTA streams the same number of bytes without a break, whatever the rows' lengths, and there are no
+//          waves.  Each CTA finds its run by itself from the lengths (a scan of at most a few KB).  It meets at most one row that began in a
+//          run before and one that goes on in the next; those give fp32 partials (o, m, l), all others are written at once.
+//          (Splits of 512 tokens, a CTA each, took 113 us and their join 9 for 256 rows of 512 to 4096 tokens; the last wave was a
+//          seventh of it.)
+//   grid   (runs, groups of kv heads x slices of 16 query heads); block = one consumer warp per kv head + a producer warp.
+//   load   The kv heads of a page are adjacent, so a page is one contiguous read of 16 * HKV * D bytes for the keys and one for the values:
+//          TMA boxes of 128-byte rows with 128-byte swizzle into a ring of stages of PPS pages.  The producer also brings the pages' scales
+//          and, a row ahead, the queries.
 //   math   transposed: S^T = K Q^T and O^T = V^T P^T with mma.sync m16n8k16, so that the 16 rows of the tile are tokens, or columns of V,
 //          and not the few heads of a group: 16 MMAs per page, half of what the other orientation needs, and 32 accumulators a thread.
 //          The order of head_dim in the products is free, so a thread's A operands come from its own 16-byte pieces of K rows without a
 //          transposition; those of V^T take bytes of two tokens and one column together with one byte permutation per four bytes of
 //          each.  P^T comes from S^T by one movmatrix per 8 x 8 tile.
 //   max    lazy, against 2^8: whether any score of the page outgrew its row's reference is one vote; only then are there shuffles.
-//   out    a sequence that fits one split is written by its CTA.  Otherwise fp32 partials (o, m, l), joined by a second kernel.
+//   join   A second kernel joins the parts of the rows that lie in more than one run, in their order.  (Joining in here by the warp that is last
+//          to finish a row - a fence, a counter, and the parts from L2 in code that runs once - took 5 us for two parts and 10 for 13;
+//          the second kernel, launched ahead, takes 1 to 1.5.)
 //
 // Bank conflicts: a token's row is 128 bytes, its 16-byte pieces XORed with the row number.  A quarter warp reads K pieces of two
 // neighbouring g = lane / 4, so their rows must differ in bit 2; it reads V pieces of four tq = lane % 4, whose rows must differ in
 // bits 1 and 2.  Row g of a tile is therefore token g ^ 4 (g & 1) of its eight.
+
+#include <algorithm>
 
 #include "host.h"
 #include "kv8.cuh"
@@ -49,6 +59,37 @@ __device__ __forceinline__ uint32_t transpose_8x8(uint32_t x) {
   return y;
 }
 
+// CTAs that an SM holds: as many as leave each enough of the ring, and of the registers, to keep its share of the memory busy.
+constexpr int kv8_ctas_per_sm(int head_dim, int hkv, int nt) {
+  return hkv == 1 ? (nt == 1 ? 6 : 5) : hkv == 2 ? (nt == 1 ? 4 : 3) : hkv == 4 ? 2 : 1;
+}
+
+// Workspace: the status word, per row where its parts are, then the parts: (m, l) and the unnormalised output per (run, which of its two
+// open rows, query head).
+struct Kv8Workspace {
+  int* err;
+  int2* rows;  // run of the first part (its sign: the run's second open row), number of parts
+  float2* ml;
+  float* o;
+  size_t bytes;
+};
+static Kv8Workspace carve_kv8(void* ws, int batch, int runs, int hq, int D) {
+  Kv8Workspace w;
+  uint8_t* p = static_cast<uint8_t*>(ws);
+  w.err = reinterpret_cast<int*>(p);
+  size_t off = 256;
+  w.rows = reinterpret_cast<int2*>(p + off);
+  off += (static_cast<size_t>(batch) * sizeof(int2) + 255) & ~size_t(255);
+  w.ml = reinterpret_cast<float2*>(p + off);
+  off += (static_cast<size_t>(runs) * 2 * hq * sizeof(float2) + 255) & ~size_t(255);
+  w.o = reinterpret_cast<float*>(p + off);
+  off += static_cast<size_t>(runs) * 2 * hq * D * sizeof(float);
+  w.bytes = off;
+  return w;
+}
+
+__device__ __forceinline__ int kv8_length(int L, int max_pages) { return min(max(L, 0), max_pages * kKvPage); }
+__device__ __forceinline__ int kv8_pages(int L, int max_pages) { return (kv8_length(L, max_pages) + kKvPage - 1) / kKvPage; }
 // D: head_dim.  HKV: kv heads = consumer warps.  NT: tiles of 8 query heads per kv head.  PPS: pages per stage.
 template <int D, int HKV, int NT, int PPS, int STAGES>
 struct Kv8Cfg {
@@ -56,8 +97,77 @@ struct Kv8Cfg {
   static constexpr int kHeadBytes = kKvPage * D;
   static constexpr int kPageBytes = HKV * kHeadBytes;      // keys, or values, of a page's kv heads
   static constexpr int kStageBytes = PPS * 2 * kPageBytes;  // page by page: keys, values
-  static constexpr int kRingBytes = STAGES * kStageBytes;
-  static constexpr int kSmemBytes = kRingBytes + 1024 /* alignment slack */ + 16 * STAGES /* barriers */;
+  static constexpr int kQ = STAGES * kStageBytes;
+  static constexpr int kScales = kQ + HKV * 8 * NT * D * 2;    // [stages][PPS][keys, values][8] bytes
+  static constexpr int kBars = kScales + STAGES * PPS * 2 * 8;
+  static constexpr int kSmemBytes = kBars + 16 * (STAGES + 1) + 1024 /* alignment slack */;
+};
+template <int BYTES> struct Kv8Word { using T = uint32_t; };
+template <> struct Kv8Word<1> { using T = uint8_t; };
+template <> struct Kv8Word<2> { using T = uint16_t; };
+template <> struct Kv8Word<8> { using T = uint2; };
+
+// A warp's walk over the rows of its CTA's run.  The lengths of 32 rows at a time are held by the lanes.
+struct Kv8Walk {
+  const int* ctx_lens;
+  int batch, max_pages, base, held;  // held: length of row base + lane
+  int total, per, begin, end;        // all pages; pages of a run; the run
+  int at, row, off;                  // the cursor: the row and the page of it that it is at
+
+  // Finds the run: every lane sums the pages of neighbouring rows, then a scan over the lanes.
+  __device__ __forceinline__ void start(const int* lens, int rows, int table_pages, int min_run, int lane, int* err) {
+    ctx_lens = lens;
+    batch = rows;
+    max_pages = table_pages;
+    const int each = (batch + 31) / 32, lo = min(lane * each, batch), hi = min(lo + each, batch);
+    int mine = 0;
+#pragma unroll 8
+    for (int b = lo; b < hi; ++b) {
+      const int L = ctx_lens[b];
+      if (L < 0 || L > max_pages * kKvPage) set_error(err, kErrDevBadCtxLen);
+      mine += kv8_pages(L, max_pages);
+    }
+    int upto = mine;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int up = __shfl_up_sync(0xffffffffu, upto, o);
+      if (lane >= o) upto += up;
+    }
+    total = __shfl_sync(0xffffffffu, upto, 31);  // < 2^31: no more than entries of the table
+    per = max(min_run, static_cast<int>((static_cast<unsigned>(total) + gridDim.x - 1) / gridDim.x));
+    const long long first = static_cast<long long>(blockIdx.x) * per;
+    begin = at = static_cast<int>(min(first, static_cast<long long>(total)));
+    end = static_cast<int>(min(first + per, static_cast<long long>(total)));
+    const unsigned past = __ballot_sync(0xffffffffu, begin < upto);  // the first of these lanes has the row
+    int before = upto - mine, b = lo;
+    if (begin >= before && begin < upto)
+      for (int pages; before + (pages = kv8_pages(ctx_lens[b], max_pages)) <= begin; ++b) before += pages;
+    const int from = past ? __ffs(past) - 1 : 0;
+    row = __shfl_sync(0xffffffffu, b, from);
+    off = begin - __shfl_sync(0xffffffffu, before, from);
+  }
+  __device__ __forceinline__ void fetch(int lane) {
+    base = row;
+    held = row + lane < batch ? ctx_lens[row + lane] : 0;
+  }
+  // The next part: row, its length L, first page off, number of pages n; false at the end of the run.
+  __device__ __forceinline__ bool next(int lane, int& L, int& n) {
+    while (at < end && row < batch) {
+      if (row - base >= 32) fetch(lane);
+      L = kv8_length(__shfl_sync(0xffffffffu, held, row - base), max_pages);
+      const int pages = (L + kKvPage - 1) / kKvPage;
+      n = min(pages - off, end - at);
+      if (n > 0) return true;
+      ++row;
+      off = 0;
+    }
+    return false;
+  }
+  __device__ __forceinline__ void advance(int n) {
+    at += n;
+    ++row;
+    off = 0;
+  }
 };
 
 template <int D, int HKV, int NT, int PPS, int STAGES, int CTAS>
@@ -65,79 +175,115 @@ __global__ void __launch_bounds__((HKV + 1) * 32, CTAS)
 kv8_attn_decode_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant__ CUtensorMap v_map,
                        const __nv_bfloat16* __restrict__ q, const uint8_t* __restrict__ k_scale, const uint8_t* __restrict__ v_scale,
                        const int* __restrict__ block_table, const int* __restrict__ ctx_lens, float* __restrict__ part_o,
-                       float2* __restrict__ part_ml, __nv_bfloat16* __restrict__ out, int* __restrict__ err, int num_q_heads,
-                       int num_kv_heads, int num_blocks, int max_pages, int split_tokens, int max_splits, float scale_log2) {
+                       float2* __restrict__ part_ml, int2* __restrict__ rows, __nv_bfloat16* __restrict__ out, int* __restrict__ err, int batch,
+                       int num_q_heads, int num_kv_heads, int num_blocks, int max_pages, int min_run, float scale_log2) {
 #ifdef B200_DEVICE_OK
-  grid_dep_wait();  // lengths, queries and the new tokens' pages come from the kernels before
-  grid_dep_launch();
   using Cfg = Kv8Cfg<D, HKV, NT, PPS, STAGES>;
+  using Word = typename Kv8Word<HKV>::T;
   extern __shared__ uint8_t smem_raw[];
   const uint32_t ring = (smem_u32(smem_raw) + 1023u) & ~1023u;
-  const uint32_t bars = ring + Cfg::kRingBytes;  // full[STAGES], empty[STAGES]
+  const uint32_t q_sm = ring + Cfg::kQ, scale_sm = ring + Cfg::kScales;
+  const uint32_t bars = ring + Cfg::kBars;  // full[STAGES], empty[STAGES], queries there, queries read
+  const uint32_t bar_q = bars + 16 * STAGES;
 
-  const int b = blockIdx.x, split = blockIdx.y;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int head_groups = num_kv_heads / HKV;
-  const int kv0 = static_cast<int>(blockIdx.z) % head_groups * HKV;   // first kv head of this CTA
-  const int q0 = static_cast<int>(blockIdx.z) / head_groups * (8 * NT);  // first query head of the group
+  const int kv0 = static_cast<int>(blockIdx.y) % head_groups * HKV;   // first kv head of this CTA
+  const int q0 = static_cast<int>(blockIdx.y) / head_groups * (8 * NT);  // first query head of the group
   const int group = num_q_heads / num_kv_heads;
   const int heads = min(group - q0, 8 * NT);  // query heads of a kv head here
-
-  int L = ctx_lens[b];
-  if (L < 0 || L > max_pages * kKvPage) {
-    if (threadIdx.x == 0) set_error(err, kErrDevBadCtxLen);
-    L = L < 0 ? 0 : max_pages * kKvPage;
-  }
-  const int start = split * split_tokens;
-  if (start >= L) {  // uniform for the whole CTA
-    if (L == 0 && split == 0 && blockIdx.z == 0)  // a row with no context attends to nothing: zeros
-      for (int i = threadIdx.x; i < num_q_heads * D; i += blockDim.x)
-        out[static_cast<size_t>(b) * num_q_heads * D + i] = __float2bfloat16(0.f);
-    return;
-  }
-  const int end = min(L, start + split_tokens);
-  const int npages = (end - start + kKvPage - 1) / kKvPage;
-  const int nstages = (npages + PPS - 1) / PPS;
-  const int* table_row = block_table + static_cast<size_t>(b) * max_pages + start / kKvPage;
 
   if (threadIdx.x == 0) {
     for (int s = 0; s < STAGES; ++s) {
       mbar_init(bars + 8 * s, 1);
       mbar_init(bars + 8 * (STAGES + s), HKV);
     }
+    mbar_init(bar_q, 1);
+    mbar_init(bar_q + 8, HKV);
     fence_mbar_init();
     fence_proxy_async();
   }
+  if (warp == HKV && lane == 0) {
+    tma_prefetch_desc(&k_map);
+    tma_prefetch_desc(&v_map);
+  }
   __syncthreads();
+  grid_dep_wait();  // lengths, queries and the new tokens' pages come from the kernels before
+  grid_dep_launch();
+
+  // Rows with no context attend to nothing: zeros, from the producer warp once it has nothing left to ask for.
+  auto zero_rows = [&]() {
+    if (blockIdx.y != 0) return;
+    for (int b = blockIdx.x; b < batch; b += gridDim.x)
+      if (ctx_lens[b] <= 0) {
+        uint4* to = reinterpret_cast<uint4*>(out + static_cast<size_t>(b) * num_q_heads * D);
+        for (int i = lane; i < num_q_heads * D / 8; i += 32) to[i] = make_uint4(0u, 0u, 0u, 0u);
+        if (lane == 0) rows[b] = make_int2(0, 0);
+      }
+  };
+  Kv8Walk walk;
+  walk.start(ctx_lens, batch, max_pages, min_run, lane, err);
+  if (walk.begin >= walk.total) {
+    if (warp == HKV) zero_rows();
+    return;
+  }
+  walk.fetch(lane);
+  int L = 0, n = 0;
+  int stage = 0;  // counts on over the parts
 
   if (warp == HKV) {
     // ------------------------------------------------------------ producer --
-    if (lane == 0) {
-      tma_prefetch_desc(&k_map);
-      tma_prefetch_desc(&v_map);
-    }
     const int lp = lane >> 1, lkv = lane & 1;  // lane -> (page of the stage, keys or values); one box each
-    int ids = 0;                               // page ids, 32 at a time, one per lane
-    for (int i = 0; i < nstages; ++i) {
-      const int p0 = i * PPS;
-      if ((p0 & 31) == 0) {
-        ids = p0 + lane < npages ? table_row[p0 + lane] : 0;
-        if (ids < 0 || ids >= num_blocks) {
+    bool alive = true;
+    for (int part = 0; walk.next(lane, L, n) && alive; ++part, walk.advance(n)) {
+      const int* table_row = block_table + static_cast<size_t>(walk.row) * max_pages + walk.off;
+      auto page_id = [&](int p) {
+        int id = p < n ? table_row[p] : 0;
+        if (id < 0 || id >= num_blocks) {
           set_error(err, kErrDevBadBlockId);
-          ids = 0;
+          id = 0;
         }
-      }
-      const int id = __shfl_sync(0xffffffffu, ids, (p0 + lp) & 31);
-      const int slot = i % STAGES;
-      const uint32_t phase = (i / STAGES) & 1;
-      if (!mbar_wait(bars + 8 * (STAGES + slot), phase ^ 1, err)) break;
-      const int pages = min(PPS, npages - p0);
-      if (lane == 0) mbar_arrive_expect_tx(bars + 8 * slot, pages * 2 * Cfg::kPageBytes);
+        return id;
+      };
+      int next_ids = page_id(lane), ids = 0;
+      alive = mbar_wait_warp(bar_q + 8, (part & 1) ^ 1, err);
+      if (!alive) break;
+      const uint32_t q_bytes = heads * D * 2;
+      if (lane == 0) mbar_arrive_expect_tx(bar_q, HKV * q_bytes);
       __syncwarp();
-      if (lp < pages)
-        tma_load_2d(ring + slot * Cfg::kStageBytes + lane * Cfg::kPageBytes, lkv ? &v_map : &k_map, bars + 8 * slot, 0,
-                    (id * num_kv_heads + kv0) * (Cfg::kHeadBytes / 128));
+      if (lane < HKV)
+        bulk_load(q_sm + lane * q_bytes, q + (static_cast<size_t>(walk.row) * num_q_heads + (kv0 + lane) * group + q0) * D, q_bytes, bar_q);
+      Word ks{}, vs{};
+      for (int p = 0; p < n; p += PPS, ++stage) {
+        if ((p & 31) == 0) {  // ids of 32 pages at a time, one per lane, asked for a batch ahead; their scales
+          ids = next_ids;
+          if (p + lane < n) {
+            const size_t cell = static_cast<size_t>(ids) * num_kv_heads + kv0;
+            ks = *reinterpret_cast<const Word*>(k_scale + cell);
+            vs = *reinterpret_cast<const Word*>(v_scale + cell);
+          }
+          next_ids = page_id(p + 32 + lane);
+        }
+        const int id = __shfl_sync(0xffffffffu, ids, (p + lp) & 31);
+        const int slot = stage % STAGES, pages = min(PPS, n - p);
+        alive = mbar_wait_warp(bars + 8 * (STAGES + slot), (stage / STAGES & 1) ^ 1, err);
+        if (!alive) break;
+        // The copies may end before the stage's bytes are announced: its phase cannot, without the arrival that comes with them.
+        // So they do not wait for the scales.
+        if (lp < pages)
+          tma_load_2d(ring + slot * Cfg::kStageBytes + lane * Cfg::kPageBytes, lkv ? &v_map : &k_map, bars + 8 * slot, 0,
+                      (id * num_kv_heads + kv0) * (Cfg::kHeadBytes / 128));
+        const int u = lane - (p & 31);
+        if (u >= 0 && u < pages) {
+          uint8_t* to = smem_raw + (scale_sm - smem_u32(smem_raw)) + (slot * PPS + u) * 16;
+          *reinterpret_cast<Word*>(to) = ks;
+          *reinterpret_cast<Word*>(to + 8) = vs;
+        }
+        __syncwarp();
+        if (lane == 0) mbar_arrive_expect_tx(bars + 8 * slot, pages * 2 * Cfg::kPageBytes);
+      }
     }
+    zero_rows();
     return;
   }
 
@@ -147,58 +293,6 @@ kv8_attn_decode_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_c
   constexpr int KS = D / 16;                       // k-steps of S^T
   constexpr int VB = D / 8;                        // bytes of a V row that a thread takes: columns g * VB ..
   constexpr int VW = VB / 4;                       // as words
-  const size_t row0 = static_cast<size_t>(b) * num_q_heads + kvh * group + q0;
-
-  // Scales of 32 pages at a time, one per lane, asked for a batch ahead.
-  auto page_id = [&](int p) {
-    const int id = p < npages ? table_row[p] : 0;
-    return id < 0 || id >= num_blocks ? 0 : id;  // the producer reports it
-  };
-  int ids = page_id(lane);
-  int ek = k_scale[static_cast<size_t>(ids) * num_kv_heads + kvh], ev = v_scale[static_cast<size_t>(ids) * num_kv_heads + kvh];
-  int ek_next = 0, ev_next = 0;
-  ids = page_id(32 + lane);
-
-  // Q^T fragments, f16.  k-step 4 c + w of thread tq: elements 64 c + 16 tq + 4 w + 0..3 of head_dim (16 tq + 4 w + .. for D = 64).
-  uint32_t qb[NT][KS][2];
-  float f_q;  // what a score is to be multiplied by, but for the page's scale
-  {
-    uint2 raw[NT][KS];
-    uint32_t top = 0;
-#pragma unroll
-    for (int n = 0; n < NT; ++n)
-#pragma unroll
-      for (int ks = 0; ks < KS; ++ks) {
-        raw[n][ks] = make_uint2(0u, 0u);
-        if (8 * n + g < heads)
-          raw[n][ks] = __ldg(reinterpret_cast<const uint2*>(q + (row0 + 8 * n + g) * D + (ks >> 2) * 64 + tq * 16 + (ks & 3) * 4));
-        const uint32_t a = raw[n][ks].x & 0x7fff7fffu, c = raw[n][ks].y & 0x7fff7fffu;
-        top = max(top, max(max(a >> 16, a & 0xffffu), max(c >> 16, c & 0xffffu)));
-      }
-    top = __reduce_max_sync(0xffffffffu, top);
-    // bf16 and fp32 have the same exponents, -127 (zeros) to 128 (infinities); tiny queries may stay below the top
-    const int shift = min(kKv8QueryTop - (static_cast<int>(top >> 7) - 127), 100);
-    const float by = power_of_two(shift);
-    f_q = scale_log2 * power_of_two(-shift);
-#pragma unroll
-    for (int n = 0; n < NT; ++n)
-#pragma unroll
-      for (int ks = 0; ks < KS; ++ks) {
-        const uint32_t x = raw[n][ks].x, y = raw[n][ks].y;
-        qb[n][ks][0] = pack_f16x2(__uint_as_float(x << 16) * by, __uint_as_float(x & 0xffff0000u) * by);
-        qb[n][ks][1] = pack_f16x2(__uint_as_float(y << 16) * by, __uint_as_float(y & 0xffff0000u) * by);
-      }
-  }
-
-  float o[NT][D / 16][4];  // O^T: rows g * VB + 2 j (+ 1), columns: heads 2 tq, 2 tq + 1
-  float m[NT][2], l[NT][2];
-#pragma unroll
-  for (int n = 0; n < NT; ++n) {
-    m[n][0] = m[n][1] = -INFINITY;
-    l[n][0] = l[n][1] = 0.f;
-#pragma unroll
-    for (int j = 0; j < D / 16; ++j) o[n][j][0] = o[n][j][1] = o[n][j][2] = o[n][j][3] = 0.f;
-  }
 
   // Address of a 16-byte piece of a token's row, relative to the head's page.
   auto piece = [](int token, int c) {
@@ -216,36 +310,70 @@ kv8_attn_decode_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_c
   // eight tokens on: the same piece, since eight rows (or four rows of two tokens, with bit 2 of the row) are one swizzle period
   constexpr uint32_t kEight = 8 * D;
 
-  bool alive = true;
-  for (int i = 0; i < nstages && alive; ++i) {
-    const int slot = i % STAGES;
-    const uint32_t phase = (i / STAGES) & 1;
-    const int p0 = i * PPS;
-    if ((p0 & 31) == 0) {
-      if (p0 > 0) {
-        ek = ek_next;
-        ev = ev_next;
-      }
-      if (p0 + 32 < npages) {
-        ek_next = k_scale[static_cast<size_t>(ids) * num_kv_heads + kvh];
-        ev_next = v_scale[static_cast<size_t>(ids) * num_kv_heads + kvh];
-        ids = page_id(p0 + 64 + lane);
-      }
+  bool alive = true;  // after a wait that ran out the warp goes through its parts without waiting, so that counters come out even
+#pragma unroll 1
+  for (int part = 0; walk.next(lane, L, n); ++part, walk.advance(n)) {
+    const size_t row0 = static_cast<size_t>(walk.row) * num_q_heads + kvh * group + q0;
+    // Q^T fragments, f16.  k-step 4 c + w of thread tq: elements 64 c + 16 tq + 4 w + 0..3 of head_dim (16 tq + 4 w + .. for D = 64).
+    uint32_t qb[NT][KS][2];
+    float f_q;  // what a score is to be multiplied by, but for the page's scale
+    {
+      if (alive) alive = mbar_wait_warp(bar_q, part & 1, err);
+      uint32_t top = 0;
+#pragma unroll
+      for (int t = 0; t < NT; ++t)
+#pragma unroll
+        for (int ks = 0; ks < KS; ++ks) {
+          qb[t][ks][0] = qb[t][ks][1] = 0u;
+          if (8 * t + g < heads)
+            lds_words<8>(q_sm + ((warp * heads + 8 * t + g) * D + (ks >> 2) * 64 + tq * 16 + (ks & 3) * 4) * 2, qb[t][ks]);
+          const uint32_t a = qb[t][ks][0] & 0x7fff7fffu, c = qb[t][ks][1] & 0x7fff7fffu;
+          top = max(top, max(max(a >> 16, a & 0xffffu), max(c >> 16, c & 0xffffu)));
+        }
+      __syncwarp();
+      if (lane == 0) mbar_arrive(bar_q + 8);
+      top = __reduce_max_sync(0xffffffffu, top);
+      // bf16 and fp32 have the same exponents, -127 (zeros) to 128 (infinities); tiny queries may stay below the top
+      const int shift = min(kKv8QueryTop - (static_cast<int>(top >> 7) - 127), 100);
+      const float by = power_of_two(shift);
+      f_q = scale_log2 * power_of_two(-shift);
+#pragma unroll
+      for (int t = 0; t < NT; ++t)
+#pragma unroll
+        for (int ks = 0; ks < KS; ++ks)
+#pragma unroll
+          for (int k = 0; k < 2; ++k)
+            qb[t][ks][k] = pack_f16x2(__uint_as_float(qb[t][ks][k] << 16) * by, __uint_as_float(qb[t][ks][k] & 0xffff0000u) * by);
     }
-    alive = mbar_wait(bars + 8 * slot, phase, err);
-    if (alive) {
+
+    float o[NT][D / 16][4];  // O^T: rows g * VB + 2 j (+ 1), columns: heads 2 tq, 2 tq + 1
+    float m[NT][2], l[NT][2];
+#pragma unroll
+    for (int t = 0; t < NT; ++t) {
+      m[t][0] = m[t][1] = -INFINITY;
+      l[t][0] = l[t][1] = 0.f;
+#pragma unroll
+      for (int j = 0; j < D / 16; ++j) o[t][j][0] = o[t][j][1] = o[t][j][2] = o[t][j][3] = 0.f;
+    }
+
+#pragma unroll 1
+    for (int p0 = 0; p0 < n; p0 += PPS, ++stage) {
+      const int slot = stage % STAGES;
+      const int left = L - (walk.off + p0) * kKvPage;  // tokens of the row from this stage on
+      if (alive) alive = mbar_wait_warp(bars + 8 * slot, stage / STAGES & 1, err);
       const uint32_t base = ring + slot * Cfg::kStageBytes + warp * Cfg::kHeadBytes;
-      float s[PPS][NT][4], lv[PPS];
+      float s[PPS][NT][4];
+      int ev[PPS];
 #pragma unroll
       for (int u = 0; u < PPS; ++u) {
 #pragma unroll
-        for (int n = 0; n < NT; ++n) s[u][n][0] = s[u][n][1] = s[u][n][2] = s[u][n][3] = -INFINITY;
-        lv[u] = 0.f;
-        if (u > 0 && p0 + u >= npages) continue;
+        for (int t = 0; t < NT; ++t) s[u][t][0] = s[u][t][1] = s[u][t][2] = s[u][t][3] = -INFINITY;
+        ev[u] = 0;
+        if (u > 0 && p0 + u >= n) continue;
         const uint32_t kb = base + u * 2 * Cfg::kPageBytes;
         float acc[NT][4];
 #pragma unroll
-        for (int n = 0; n < NT; ++n) acc[n][0] = acc[n][1] = acc[n][2] = acc[n][3] = 0.f;
+        for (int t = 0; t < NT; ++t) acc[t][0] = acc[t][1] = acc[t][2] = acc[t][3] = 0.f;
 #pragma unroll
         for (int c = 0; c < D / 64; ++c) {
           uint32_t x[4], y[4];
@@ -257,22 +385,26 @@ kv8_attn_decode_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_c
             e4m3x4_to_f16(x[w], a0, a2);
             e4m3x4_to_f16(y[w], a1, a3);
 #pragma unroll
-            for (int n = 0; n < NT; ++n) mma_f16_16816(acc[n], a0, a1, a2, a3, qb[n][c * 4 + w][0], qb[n][c * 4 + w][1]);
+            for (int t = 0; t < NT; ++t) mma_f16_16816(acc[t], a0, a1, a2, a3, qb[t][c * 4 + w][0], qb[t][c * 4 + w][1]);
           }
         }
-        const float f = f_q * power_of_two(scale_exponent(__shfl_sync(0xffffffffu, ek, (p0 + u) & 31)));
-        lv[u] = static_cast<float>(scale_exponent(__shfl_sync(0xffffffffu, ev, (p0 + u) & 31)));
-        const int t0 = start + (p0 + u) * kKvPage + tok;
+        int kbyte, vbyte;
+        asm volatile("ld.shared.u8 %0, [%1];" : "=r"(kbyte) : "r"(scale_sm + (slot * PPS + u) * 16 + warp));
+        asm volatile("ld.shared.u8 %0, [%1];" : "=r"(vbyte) : "r"(scale_sm + (slot * PPS + u) * 16 + 8 + warp));
+        const float f = f_q * power_of_two(scale_exponent(kbyte));
+        ev[u] = scale_exponent(vbyte);
+        const float lv = static_cast<float>(ev[u]);
+        const int here = left - u * kKvPage;  // tokens of this page, if fewer than 16
 #pragma unroll
-        for (int n = 0; n < NT; ++n)
+        for (int t = 0; t < NT; ++t)
 #pragma unroll
-          for (int k = 0; k < 4; ++k) s[u][n][k] = t0 + (k >> 1) * 8 < L ? fmaf(acc[n][k], f, lv[u]) : -INFINITY;
-        if (start + (p0 + u) * kKvPage + kKvPage > L) {
-          // the last page: what lies behind the last token may be NaN, which a weight of zero does not undo.  Nothing loads into
-          // this stage again.
+          for (int k = 0; k < 4; ++k) s[u][t][k] = tok + (k >> 1) * 8 < here ? fmaf(acc[t][k], f, lv) : -INFINITY;
+        if (here < kKvPage) {
+          // the last page: what lies behind the last token may be NaN, which a weight of zero does not undo
           const uint32_t vb = kb + Cfg::kPageBytes;
-          for (int t = L - (start + (p0 + u) * kKvPage); t < kKvPage; ++t)
-            if (lane < D / 4) asm volatile("st.shared.b32 [%0], %1;" ::"r"(vb + piece(t, lane >> 2) + (lane & 3) * 4), "r"(0) : "memory");
+          for (int x = here; x < kKvPage; ++x)
+            if (lane < D / 4) asm volatile("st.shared.b32 [%0], %1;" ::"r"(vb + piece(x, lane >> 2) + (lane & 3) * 4), "r"(0) : "memory");
+          fence_proxy_async();  // a later copy overwrites the stage
           __syncwarp();
         }
       }
@@ -281,49 +413,49 @@ kv8_attn_decode_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_c
       bool over = false;
       float top[NT][2];
 #pragma unroll
-      for (int n = 0; n < NT; ++n)
+      for (int t = 0; t < NT; ++t)
 #pragma unroll
         for (int k = 0; k < 2; ++k) {
-          float t = fmaxf(s[0][n][k], s[0][n][k + 2]);
+          float x = fmaxf(s[0][t][k], s[0][t][k + 2]);
 #pragma unroll
-          for (int u = 1; u < PPS; ++u) t = fmaxf(t, fmaxf(s[u][n][k], s[u][n][k + 2]));
-          top[n][k] = t;
-          over |= t > m[n][k] + kKv8RefSlack;
+          for (int u = 1; u < PPS; ++u) x = fmaxf(x, fmaxf(s[u][t][k], s[u][t][k + 2]));
+          top[t][k] = x;
+          over |= x > m[t][k] + kKv8RefSlack;
         }
       if (__any_sync(0xffffffffu, over)) {
 #pragma unroll
-        for (int n = 0; n < NT; ++n)
+        for (int t = 0; t < NT; ++t)
 #pragma unroll
           for (int k = 0; k < 2; ++k) {
-            float t = top[n][k];
+            float x = top[t][k];
 #pragma unroll
-            for (int x = 4; x < 32; x <<= 1) t = fmaxf(t, __shfl_xor_sync(0xffffffffu, t, x));
-            t = fmaxf(t, m[n][k]);
-            const float a = t == -INFINITY ? 1.f : fast_ex2(m[n][k] - t);  // still nothing but scores of -inf: sums are zero
-            m[n][k] = t;
-            l[n][k] *= a;
+            for (int d = 4; d < 32; d <<= 1) x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, d));
+            x = fmaxf(x, m[t][k]);
+            const float a = x == -INFINITY ? 1.f : fast_ex2(m[t][k] - x);  // still nothing but scores of -inf: sums are zero
+            m[t][k] = x;
+            l[t][k] *= a;
 #pragma unroll
             for (int j = 0; j < D / 16; ++j) {
-              o[n][j][k] *= a;
-              o[n][j][k + 2] *= a;
+              o[t][j][k] *= a;
+              o[t][j][k + 2] *= a;
             }
           }
       }
 
 #pragma unroll
       for (int u = 0; u < PPS; ++u) {
-        if (u > 0 && p0 + u >= npages) continue;
+        if (u > 0 && p0 + u >= n) continue;
         uint32_t pb[NT][2];
-        const float iv = power_of_two(-static_cast<int>(lv[u]));
+        const float iv = power_of_two(-ev[u]);
 #pragma unroll
-        for (int n = 0; n < NT; ++n) {
-          float p[4];
+        for (int t = 0; t < NT; ++t) {
+          float e[4];
 #pragma unroll
-          for (int k = 0; k < 4; ++k) p[k] = fast_ex2(s[u][n][k] - (m[n][k & 1] == -INFINITY ? 0.f : m[n][k & 1] - kKv8Lift));
-          l[n][0] = fmaf(p[0] + p[2], iv, l[n][0]);
-          l[n][1] = fmaf(p[1] + p[3], iv, l[n][1]);
-          pb[n][0] = transpose_8x8(pack_f16x2(p[0], p[1]));
-          pb[n][1] = transpose_8x8(pack_f16x2(p[2], p[3]));
+          for (int k = 0; k < 4; ++k) e[k] = fast_ex2(s[u][t][k] - (m[t][k & 1] == -INFINITY ? 0.f : m[t][k & 1] - kKv8Lift));
+          l[t][0] = fmaf(e[0] + e[2], iv, l[t][0]);
+          l[t][1] = fmaf(e[1] + e[3], iv, l[t][1]);
+          pb[t][0] = transpose_8x8(pack_f16x2(e[0], e[1]));
+          pb[t][1] = transpose_8x8(pack_f16x2(e[2], e[3]));
         }
         const uint32_t vb = base + u * 2 * Cfg::kPageBytes + Cfg::kPageBytes;
         uint32_t w00[VW], w01[VW], w10[VW], w11[VW];  // tokens tv, tv1, tv + 8, tv1 + 8
@@ -339,147 +471,165 @@ kv8_attn_decode_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_c
           e4m3x4_to_f16(__byte_perm(w10[w], w11[w], 0x5140), a[0][1], a[1][1]);
           e4m3x4_to_f16(__byte_perm(w10[w], w11[w], 0x7362), a[2][1], a[3][1]);
 #pragma unroll
-          for (int n = 0; n < NT; ++n) {
-            mma_f16_16816(o[n][2 * w], a[0][0], a[1][0], a[0][1], a[1][1], pb[n][0], pb[n][1]);
-            mma_f16_16816(o[n][2 * w + 1], a[2][0], a[3][0], a[2][1], a[3][1], pb[n][0], pb[n][1]);
+          for (int t = 0; t < NT; ++t) {
+            mma_f16_16816(o[t][2 * w], a[0][0], a[1][0], a[0][1], a[1][1], pb[t][0], pb[t][1]);
+            mma_f16_16816(o[t][2 * w + 1], a[2][0], a[3][0], a[2][1], a[3][1], pb[t][0], pb[t][1]);
           }
         }
       }
+      __syncwarp();
+      if (lane == 0) mbar_arrive(bars + 8 * (STAGES + slot));
     }
-    __syncwarp();
-    if (lane == 0) mbar_arrive(bars + 8 * (STAGES + slot));
-  }
 
-  const int nsplits = (L + split_tokens - 1) / split_tokens;
+    const int row_at = walk.at - walk.off;  // first page of the row among all pages
+    const int first_run = row_at / walk.per, parts = (row_at + (L + kKvPage - 1) / kKvPage - 1) / walk.per - first_run + 1;
+    // a part that begins with the run is the first of its two, one that does not is the second and the row's first part
+    const bool second = walk.at != walk.begin;
+    const size_t here = static_cast<size_t>(blockIdx.x) * 2 + second;
+    if (first_run == static_cast<int>(blockIdx.x) && blockIdx.y == 0 && threadIdx.x == 0)
+      rows[walk.row] = make_int2(first_run * 2 + second, parts);
 #pragma unroll
-  for (int n = 0; n < NT; ++n)
+    for (int t = 0; t < NT; ++t)
 #pragma unroll
-    for (int k = 0; k < 2; ++k) {
-      float sum = l[n][k];
+      for (int k = 0; k < 2; ++k) {
+        float sum = l[t][k];
 #pragma unroll
-      for (int x = 4; x < 32; x <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, x);
-      const int head = 8 * n + 2 * tq + k;
-      if (head >= heads) continue;
-      if (nsplits == 1) {
-        const float inv = 1.f / sum;
-        uint32_t r[VB / 2];
+        for (int x = 4; x < 32; x <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, x);
+        const int head = 8 * t + 2 * tq + k;
+        if (head >= heads) continue;
+        if (parts == 1) {
+          const float inv = 1.f / sum;
+          uint32_t r[VB / 2];
 #pragma unroll
-        for (int j = 0; j < D / 16; ++j) r[j] = pack_bf16x2(o[n][j][k] * inv, o[n][j][k + 2] * inv);
-        uint32_t* to = reinterpret_cast<uint32_t*>(out + (row0 + head) * D + g * VB);
+          for (int j = 0; j < D / 16; ++j) r[j] = pack_bf16x2(o[t][j][k] * inv, o[t][j][k + 2] * inv);
+          uint32_t* to = reinterpret_cast<uint32_t*>(out + (row0 + head) * D + g * VB);
 #pragma unroll
-        for (int j = 0; j < D / 16; j += 4) *reinterpret_cast<uint4*>(to + j) = make_uint4(r[j], r[j + 1], r[j + 2], r[j + 3]);
-      } else {
-        const size_t prow = (row0 + head) * max_splits + split;
-        float* to = part_o + prow * D + g * VB;
+          for (int j = 0; j < D / 16; j += 4) *reinterpret_cast<uint4*>(to + j) = make_uint4(r[j], r[j + 1], r[j + 2], r[j + 3]);
+        } else {
+          const size_t prow = here * num_q_heads + kvh * group + q0 + head;
+          float* to = part_o + prow * D + g * VB;
 #pragma unroll
-        for (int j = 0; j < D / 16; j += 2)
-          *reinterpret_cast<float4*>(to + 2 * j) = make_float4(o[n][j][k], o[n][j][k + 2], o[n][j + 1][k], o[n][j + 1][k + 2]);
-        if (g == 0) part_ml[prow] = make_float2(m[n][k], sum);
+          for (int j = 0; j < D / 16; j += 2)
+            *reinterpret_cast<float4*>(to + 2 * j) = make_float4(o[t][j][k], o[t][j][k + 2], o[t][j + 1][k], o[t][j + 1][k + 2]);
+          if (g == 0) part_ml[prow] = make_float2(m[t][k], sum);
+        }
       }
-    }
+  }
 #endif
 }
 
-// Joins the partials of one (row, query head): a CTA of four warps, warp w taking splits w, w + 4, ..., each lane D / 32
-// columns.  The sums over splits are taken in a fixed order.  Without lengths every row has max_splits of them, some perhaps empty (their
-// reference is -inf and their sums are not written).
-template <int D>
-__global__ void __launch_bounds__(128)
-kv8_attn_join_kernel(const float* __restrict__ part_o, const float2* __restrict__ part_ml, const int* __restrict__ ctx_lens,
-                     __nv_bfloat16* __restrict__ out, int num_q_heads, int max_splits, int split_tokens, int max_ctx) {
+// Joins the parts of one (row, query head): WARPS warps share them out, warp w taking parts w, w + WARPS, ..., eight at a time, each lane
+// D / 32 columns.  The sums over parts are taken in a fixed order.  With `rows` the parts are those of kv8_attn_decode_kernel;
+// without, every row has `parts` of them, side by side, some perhaps empty (their reference is -inf and their sums are not written).
+// One warp per row serves batches, whose rows have a handful of parts, and 16 a few rows of hundreds.
+template <int D, int WARPS>
+__global__ void __launch_bounds__(WARPS == 1 ? 128 : 32 * WARPS)
+kv8_attn_join_kernel(const float* __restrict__ part_o, const float2* __restrict__ part_ml, const int2* __restrict__ rows,
+                     __nv_bfloat16* __restrict__ out, int num_q_heads, int num_rows, int parts) {
   grid_dep_wait();
   grid_dep_launch();
   constexpr int V = D / 32;
-  __shared__ float o_sm[4][D];
-  __shared__ float ml_sm[4][2];
-  const size_t row = blockIdx.x;
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  int n = max_splits;
-  if (ctx_lens != nullptr) {
-    const int L = min(max(ctx_lens[row / num_q_heads], 0), max_ctx);
-    n = (L + split_tokens - 1) / split_tokens;
+  __shared__ float o_sm[WARPS][WARPS == 1 ? 1 : D];
+  __shared__ float ml_sm[WARPS][2];
+  const int lane = threadIdx.x & 31, warp = WARPS == 1 ? 0 : threadIdx.x >> 5;
+  const int row = WARPS == 1 ? static_cast<int>(blockIdx.x * 4 + (threadIdx.x >> 5)) : static_cast<int>(blockIdx.x);
+  if (row >= num_rows) return;  // WARPS > 1: never
+  int n = parts, first = row * parts, next = row * parts + 1, step = 1;  // part 0, then next, next + step, ...
+  if (rows != nullptr) {
+    const int2 at = rows[row / num_q_heads];
+    const int head = row % num_q_heads;
+    n = at.y;
     if (n <= 1) return;  // written by its one CTA
+    first = at.x * num_q_heads + head;
+    next = ((at.x | 1) + 1) * num_q_heads + head;  // the first part of the run after
+    step = 2 * num_q_heads;
   }
-  const size_t base = row * max_splits;
   float top = -INFINITY, den = 0.f, acc[V];
 #pragma unroll
   for (int j = 0; j < V; ++j) acc[j] = 0.f;
-  for (int s0 = warp; s0 < n; s0 += 16) {  // four splits of this warp at a time
-    float v[4][V];
-    float2 ml[4];
+#pragma unroll 1
+  for (int k0 = warp; k0 < n; k0 += 8 * WARPS) {
+    float v[8][V];
+    float2 ml[8];
 #pragma unroll
-    for (int u = 0; u < 4; ++u) {
+    for (int u = 0; u < 8; ++u) {
       ml[u] = make_float2(-INFINITY, 0.f);
-      const int s = s0 + 4 * u;
-      if (s < n) {
-        ml[u] = part_ml[base + s];
-        const float* from = part_o + (base + s) * D + lane * V;
 #pragma unroll
-        for (int j = 0; j < V; ++j) v[u][j] = from[j];
+      for (int j = 0; j < V; ++j) v[u][j] = 0.f;
+      const int k = k0 + u * WARPS;
+      if (k < n) {
+        const size_t from = k == 0 ? static_cast<size_t>(first) : static_cast<size_t>(next) + static_cast<size_t>(k - 1) * step;
+        ml[u] = part_ml[from];
+#pragma unroll
+        for (int j = 0; j < V; ++j) v[u][j] = part_o[from * D + lane * V + j];
       }
     }
+    float t = top;
 #pragma unroll
-    for (int u = 0; u < 4; ++u)
-#pragma unroll
-      for (int j = 0; j < V; ++j)
-        if (ml[u].x == -INFINITY) v[u][j] = 0.f;
-    const float t = fmaxf(fmaxf(top, fmaxf(ml[0].x, ml[1].x)), fmaxf(ml[2].x, ml[3].x));
+    for (int u = 0; u < 8; ++u) t = fmaxf(t, ml[u].x);
     const float ref = t == -INFINITY ? 0.f : t;
-    const float a = exp2f(top - ref);
+    const float a = fast_ex2(top - ref);
     top = t;
     den *= a;
 #pragma unroll
     for (int j = 0; j < V; ++j) acc[j] *= a;
 #pragma unroll
-    for (int u = 0; u < 4; ++u) {
-      const float w = exp2f(ml[u].x - ref);
-      den += w * ml[u].y;
+    for (int u = 0; u < 8; ++u) {
+      const float w = fast_ex2(ml[u].x - ref);
+      den = fmaf(w, ml[u].y, den);
 #pragma unroll
-      for (int j = 0; j < V; ++j) acc[j] += w * v[u][j];
+      for (int j = 0; j < V; ++j) acc[j] = fmaf(w, ml[u].x == -INFINITY ? 0.f : v[u][j], acc[j]);
     }
   }
+  if constexpr (WARPS == 1) {
+    const float inv = 1.f / den;
+    uint32_t* to = reinterpret_cast<uint32_t*>(out + static_cast<size_t>(row) * D + lane * V);
 #pragma unroll
-  for (int j = 0; j < V; ++j) o_sm[warp][lane * V + j] = acc[j];
-  if (lane == 0) {
-    ml_sm[warp][0] = top;
-    ml_sm[warp][1] = den;
-  }
-  __syncthreads();
-  const int d = threadIdx.x;
-  if (d >= D) return;
-  const float t = fmaxf(fmaxf(ml_sm[0][0], ml_sm[1][0]), fmaxf(ml_sm[2][0], ml_sm[3][0]));
-  const float ref = t == -INFINITY ? 0.f : t;
-  float num = 0.f, sum = 0.f;
+    for (int j = 0; j < V; j += 2) to[j / 2] = pack_bf16x2(acc[j] * inv, acc[j + 1] * inv);
+  } else {
 #pragma unroll
-  for (int w = 0; w < 4; ++w) {
-    const float x = exp2f(ml_sm[w][0] - ref);
-    num += x * o_sm[w][d];
-    sum += x * ml_sm[w][1];
+    for (int j = 0; j < V; ++j) o_sm[warp][lane * V + j] = acc[j];
+    if (lane == 0) {
+      ml_sm[warp][0] = top;
+      ml_sm[warp][1] = den;
+    }
+    __syncthreads();
+    const int d = threadIdx.x;
+    if (d >= D) return;
+    float t = ml_sm[0][0];
+#pragma unroll
+    for (int w = 1; w < WARPS; ++w) t = fmaxf(t, ml_sm[w][0]);
+    const float ref = t == -INFINITY ? 0.f : t;
+    float num = 0.f, sum = 0.f;
+#pragma unroll
+    for (int w = 0; w < WARPS; ++w) {
+      const float x = fast_ex2(ml_sm[w][0] - ref);
+      num += x * o_sm[w][d];
+      sum += x * ml_sm[w][1];
+    }
+    out[static_cast<size_t>(row) * D + d] = __float2bfloat16(num / sum);
   }
-  out[row * D + d] = __float2bfloat16(num / sum);
 }
 
-int launch_kv8_join(int head_dim, const AttnWorkspace& w, const int* ctx_lens, void* out, int rows, int hq, int max_splits, int split_tokens,
-                    int max_ctx, cudaStream_t st) {
-  B200_CUDA(launch_overlapped(head_dim == 128 ? kv8_attn_join_kernel<128> : kv8_attn_join_kernel<64>, dim3(rows * hq), dim3(128), 0, st, w.o,
-                              w.ml, ctx_lens, static_cast<__nv_bfloat16*>(out), hq, max_splits, split_tokens, max_ctx));
+template <int D>
+static int launch_join(const float* o, const float2* ml, const int2* rows, void* out, int hq, int num_rows, int parts, int most, cudaStream_t st) {
+  __nv_bfloat16* to = static_cast<__nv_bfloat16*>(out);
+  if (most <= 16)
+    B200_CUDA(launch_overlapped(kv8_attn_join_kernel<D, 1>, dim3((num_rows + 3) / 4), dim3(128), 0, st, o, ml, rows, to, hq, num_rows, parts));
+  else
+    B200_CUDA(launch_overlapped(kv8_attn_join_kernel<D, 16>, dim3(num_rows), dim3(512), 0, st, o, ml, rows, to, hq, num_rows, parts));
   return 0;
 }
-
-// Tokens per split where the caller names none.  Few rows: so that all CTAs are there at once and the GPU is full, but no fewer than 64
-// tokens; a full batch: 512, long enough that partials cost little and short enough that rows of different lengths even out.
-static int kv8_split_tokens(int batch, int head_ctas, int max_pages, int sms) {
-  const long long tokens = static_cast<long long>(max_pages) * kKvPage;
-  const long long ctas = 2ll * sms / (static_cast<long long>(batch) * head_ctas);
-  if (ctas < 2) return 512;
-  const long long split = ((tokens + ctas - 1) / ctas + kKvPage - 1) / kKvPage * kKvPage;
-  return static_cast<int>(split < 64 ? 64 : split > 512 && batch > 8 ? 512 : split);
+int launch_kv8_join(int head_dim, const AttnWorkspace& w, void* out, int rows, int hq, int parts, cudaStream_t st) {
+  return head_dim == 128 ? launch_join<128>(w.o, w.ml, nullptr, out, hq, rows * hq, parts, parts, st)
+                         : launch_join<64>(w.o, w.ml, nullptr, out, hq, rows * hq, parts, parts, st);
 }
 
+// How a call is laid out.  `min_run`: pages of a run at least.
 struct Kv8Plan {
-  int hkv, nt, slices, split, max_splits;
+  int hkv, nt, slices, runs, min_run;
 };
-static int kv8_plan(int batch, int hq, int hkv, int max_pages, int split_tokens, Kv8Plan* p) {
+static int kv8_plan(int batch, int hq, int hkv, int head_dim, int max_pages, int split_tokens, Kv8Plan* p) {
   const int group = hq / hkv;
   p->hkv = hkv % 8 == 0 ? 8 : hkv % 4 == 0 ? 4 : hkv % 2 == 0 ? 2 : 1;
   p->nt = group > 8 ? 2 : 1;
@@ -487,16 +637,19 @@ static int kv8_plan(int batch, int hq, int hkv, int max_pages, int split_tokens,
   int sms = 0;
   const int rc = device_sm_count(&sms);
   if (rc) return rc;
-  p->split = split_tokens > 0 ? split_tokens : kv8_split_tokens(batch, hkv / p->hkv * p->slices, max_pages, sms);
-  p->max_splits = static_cast<int>((static_cast<long long>(max_pages) * kKvPage + p->split - 1) / p->split);
+  const int y = hkv / p->hkv * p->slices, held = kv8_ctas_per_sm(head_dim, p->hkv, p->nt) * sms;
+  p->runs = y >= held ? 1 : held / y;
+  p->min_run = split_tokens > 0 ? split_tokens / kKvPage : 2;
   return 0;
 }
+
+constexpr int kKv8FewRows = 8;  // from this on a row has a handful of parts
 
 struct Kv8Args {
   const void *q, *k_pool, *v_pool, *k_scale, *v_scale;
   const int *table, *ctx;
   void* out;
-  AttnWorkspace w;
+  Kv8Workspace w;
   int batch, hq, hkv, num_blocks, max_pages;
   float scale;
   Kv8Plan plan;
@@ -506,6 +659,7 @@ struct Kv8Args {
 template <int D, int HKV, int NT, int PPS, int STAGES, int CTAS>
 static int launch_kv8_decode(const Kv8Args& a) {
   using Cfg = Kv8Cfg<D, HKV, NT, PPS, STAGES>;
+  static_assert(CTAS * (Cfg::kSmemBytes + 1024 + 128) <= 228 * 1024, "runs are cut for CTAS per SM");
   CUtensorMap kmap, vmap;
   const uint64_t rows = static_cast<uint64_t>(a.num_blocks) * a.hkv * (Cfg::kHeadBytes / 128);
   int rc = get_tensor_map_2d(a.k_pool, rows, 128, 1, Cfg::kPageBytes / 128, 128, &kmap);
@@ -515,23 +669,24 @@ static int launch_kv8_decode(const Kv8Args& a) {
   auto kernel = kv8_attn_decode_kernel<D, HKV, NT, PPS, STAGES, CTAS>;
   rc = ensure_dynamic_smem(reinterpret_cast<const void*>(kernel), Cfg::kSmemBytes);
   if (rc) return rc;
-  B200_CUDA(launch_overlapped(kernel, dim3(a.batch, a.plan.max_splits, a.hkv / HKV * a.plan.slices), dim3(Cfg::kThreads), Cfg::kSmemBytes,
-                              a.st, kmap, vmap, static_cast<const __nv_bfloat16*>(a.q), static_cast<const uint8_t*>(a.k_scale),
-                              static_cast<const uint8_t*>(a.v_scale), a.table, a.ctx, a.w.o, a.w.ml, static_cast<__nv_bfloat16*>(a.out),
-                              a.w.err, a.hq, a.hkv, a.num_blocks, a.max_pages, a.plan.split, a.plan.max_splits,
+  B200_CUDA(launch_overlapped(kernel, dim3(a.plan.runs, a.hkv / HKV * a.plan.slices), dim3(Cfg::kThreads), Cfg::kSmemBytes, a.st, kmap, vmap,
+                              static_cast<const __nv_bfloat16*>(a.q), static_cast<const uint8_t*>(a.k_scale),
+                              static_cast<const uint8_t*>(a.v_scale), a.table, a.ctx, a.w.o, a.w.ml, a.w.rows,
+                              static_cast<__nv_bfloat16*>(a.out), a.w.err, a.batch, a.hq, a.hkv, a.num_blocks, a.max_pages, a.plan.min_run,
                               a.scale * 1.4426950408889634f));
-  if (a.plan.max_splits > 1)
-    return launch_kv8_join(D, a.w, a.ctx, a.out, a.batch, a.hq, a.plan.max_splits, a.plan.split, a.max_pages * kKvPage, a.st);
-  return 0;
+  // parts of a row at most
+  const int most = static_cast<int>(std::min<long long>(a.plan.runs, static_cast<long long>(a.max_pages - 1) / a.plan.min_run + 2));
+  if (a.batch == 1 && a.max_pages <= a.plan.min_run) return 0;
+  return launch_join<D>(a.w.o, a.w.ml, a.w.rows, a.out, a.hq, a.batch * a.hq, 0, a.batch >= kKv8FewRows ? 1 : most, a.st);
 }
 
 template <int D, int NT>
 static int launch_kv8_heads(const Kv8Args& a) {
   switch (a.plan.hkv) {
-    case 1: return launch_kv8_decode<D, 1, NT, 2, 4, 6>(a);
-    case 2: return launch_kv8_decode<D, 2, NT, 2, 4, NT == 1 ? 4 : 3>(a);
-    case 4: return launch_kv8_decode<D, 4, NT, 2, 3, 2>(a);
-    default: return launch_kv8_decode<D, 8, NT, 1, D == 128 ? 6 : 8, 1>(a);
+    case 1: return launch_kv8_decode<D, 1, NT, 2, 4, kv8_ctas_per_sm(D, 1, NT)>(a);
+    case 2: return launch_kv8_decode<D, 2, NT, 2, D == 128 ? 3 : 4, kv8_ctas_per_sm(D, 2, NT)>(a);
+    case 4: return launch_kv8_decode<D, 4, NT, D == 128 && NT == 2 ? 1 : 2, D == 128 ? (NT == 2 ? 5 : 3) : 4, kv8_ctas_per_sm(D, 4, NT)>(a);
+    default: return launch_kv8_decode<D, 8, NT, 1, D == 128 ? 5 : 8, kv8_ctas_per_sm(D, 8, NT)>(a);
   }
 }
 
@@ -540,7 +695,7 @@ static int launch_kv8_heads(const Kv8Args& a) {
 using namespace b200;
 
 int b200::check_kv8(const char* name, int batch, int hq, int hkv, int head_dim, int num_blocks, int max_pages, const void* q,
-                     const void* k_pool, const void* v_pool, const void* out, float scale) {
+                    const void* k_pool, const void* v_pool, const void* out, float scale) {
   B200_REQUIRE(batch > 0 && hq > 0 && hkv > 0 && num_blocks > 0 && max_pages > 0, "%s: non-positive dimension", name);
   B200_REQUIRE(hq % hkv == 0, "%s: q heads %d not a multiple of kv heads %d", name, hq, hkv);
   B200_REQUIRE(head_dim == 64 || head_dim == 128, "%s: head_dim %d is neither 64 nor 128", name, head_dim);
@@ -559,8 +714,8 @@ extern "C" size_t b200_kv8_attn_workspace_bytes(int batch, int num_q_heads, int 
       num_q_heads % num_kv_heads != 0)
     return 256;
   Kv8Plan p;
-  if (kv8_plan(batch, num_q_heads, num_kv_heads, max_pages_per_seq, split_tokens, &p)) return 256;
-  return carve(nullptr, batch, num_q_heads, head_dim, p.max_splits).bytes;
+  if (kv8_plan(batch, num_q_heads, num_kv_heads, head_dim, max_pages_per_seq, split_tokens, &p)) return 256;
+  return carve_kv8(nullptr, batch, p.runs, num_q_heads, head_dim).bytes;
 }
 
 extern "C" int b200_kv8_attn_decode(const void* q, const void* k_pool, const void* v_pool, const void* k_scale, const void* v_scale,
@@ -575,12 +730,14 @@ extern "C" int b200_kv8_attn_decode(const void* q, const void* k_pool, const voi
   if (rc) return rc;
   Kv8Args a{q, k_pool, v_pool, k_scale, v_scale, block_table, ctx_lens, out, {}, batch, num_q_heads, num_kv_heads, num_blocks,
             max_pages_per_seq, scale, {}, as_stream(stream)};
-  rc = kv8_plan(batch, num_q_heads, num_kv_heads, max_pages_per_seq, split_tokens, &a.plan);
+  rc = kv8_plan(batch, num_q_heads, num_kv_heads, head_dim, max_pages_per_seq, split_tokens, &a.plan);
   if (rc) return rc;
-  B200_REQUIRE(a.plan.max_splits <= 65535 && num_kv_heads / a.plan.hkv * a.plan.slices <= 65535 &&
-                   static_cast<long long>(batch) * num_q_heads < (1ll << 31),
+  B200_REQUIRE(num_kv_heads / a.plan.hkv * a.plan.slices <= 65535 && static_cast<long long>(batch) * num_q_heads < (1ll << 31),
                "kv8_attn_decode: grid too large");
-  a.w = carve(workspace, batch, num_q_heads, head_dim, a.plan.max_splits);
+  B200_REQUIRE(static_cast<long long>(batch) * max_pages_per_seq < (1ll << 31), "kv8_attn_decode: the table has more than 2^31 entries");
+  B200_REQUIRE(reinterpret_cast<uintptr_t>(k_scale) % a.plan.hkv == 0 && reinterpret_cast<uintptr_t>(v_scale) % a.plan.hkv == 0,
+               "kv8_attn_decode: scales must be %d-byte aligned", a.plan.hkv);
+  a.w = carve_kv8(workspace, batch, a.plan.runs, num_q_heads, head_dim);
   if (workspace_bytes < a.w.bytes || (reinterpret_cast<uintptr_t>(workspace) & 15) != 0) {
     set_detail("kv8_attn_decode: workspace of %zu bytes at %p, %zu on a 16-byte boundary are needed", workspace_bytes, workspace, a.w.bytes);
     return -kErrWorkspace;

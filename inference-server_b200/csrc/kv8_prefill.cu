@@ -593,7 +593,7 @@ static int launch_kv8_prefill(const void* q, const void* k_pool, const void* v_p
                               static_cast<const uint8_t*>(v_scale), table_row, static_cast<const __nv_bfloat16*>(q),
                               static_cast<__nv_bfloat16*>(out), w.o, w.ml, w.err, num_tokens, first_pos, hq, hkv, num_blocks,
                               scale * 1.4426950408889634f, p.pairs, p.splits, p.split_tiles));
-  if (p.splits > 1) return launch_kv8_join(D, w, nullptr, out, num_tokens, hq, p.splits, 0, 0, st);
+  if (p.splits > 1) return launch_kv8_join(D, w, out, num_tokens, hq, p.splits, st);
   return 0;
 }
 

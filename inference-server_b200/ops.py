@@ -311,7 +311,7 @@ def _attn_out(q: torch.Tensor, out: torch.Tensor | None) -> torch.Tensor:
 
 def kv8_attn_workspace(batch: int, num_q_heads: int, num_kv_heads: int, head_dim: int, max_pages: int, device,
                        split_tokens: int = 0) -> torch.Tensor:
-    """Workspace of `kv8_attn_decode`, starting with the status word; kept for all steps of a batch shape."""
+    """Workspace of `kv8_attn_decode`, starting with the status word; kept for all steps.  Its size does not depend on the lengths."""
     n = _lib.load().b200_kv8_attn_workspace_bytes(batch, num_q_heads, num_kv_heads, head_dim, max_pages, split_tokens)
     return torch.zeros(n, dtype=torch.uint8, device=device)
 
@@ -319,7 +319,7 @@ def kv8_attn_workspace(batch: int, num_q_heads: int, num_kv_heads: int, head_dim
 def kv8_attn_decode(q, k_pool, v_pool, k_scale, v_scale, block_table, ctx_lens, scale: float, split_tokens: int = 0,
                     workspace: torch.Tensor | None = None, out: torch.Tensor | None = None) -> torch.Tensor:
     """`paged_attn_decode` over an 8-bit page cache: softmax(q K^T * scale) V for one bf16 query row [B, Hq, D] per sequence; head_dim 64
-    or 128, any head grouping.  `split_tokens` 0: the library's choice."""
+    or 128, any head grouping.  `split_tokens`: tokens that a CTA takes at least; 0: the library's choice."""
     nb, Hkv, D = _kv8_cache(k_pool, v_pool, k_scale, v_scale)
     _need(q, "q", torch.bfloat16)
     _need(block_table, "block_table", torch.int32)

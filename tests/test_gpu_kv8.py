@@ -287,6 +287,34 @@ def test_decode_batches(ops, B, top):
     check_attn(run_decode(ops, *case, lens, 0.09), *case, lens, 0.09)
 
 
+def test_decode_one_workspace_for_many_shapes(ops):
+    """Calls of other sizes and head shapes take turns with a workspace; parts of rows are counted in it."""
+    rng = np.random.default_rng(14)
+    shapes = [(8, 2, 64, [3000]), (32, 4, 128, [100, 700, 30]), (8, 2, 64, [900] * 40), (16, 1, 128, [2000, 0, 17, 5]), (32, 4, 128, [2500] * 9)]
+    cases = [attn_case(rng, lens, Hq, H, D, width=200) for Hq, H, D, lens in shapes]
+    n = max(ops.kv8_attn_workspace(len(lens), Hq, H, D, 200, DEV).numel() for Hq, H, D, lens in shapes)
+    ws = torch.zeros(n, dtype=torch.uint8, device=DEV)
+    first = []
+    for turn in range(3):
+        for i, (q, kc, ke, vc, ve, table) in enumerate(cases):
+            lens = shapes[i][3]
+            out = ops.kv8_attn_decode(q.to(DEV), plain.pool_of(kc), plain.pool_of(vc), plain.scale_of(ke), plain.scale_of(ve), torch.from_numpy(table).to(DEV),
+                                      ints(lens), 0.1, workspace=ws)
+            if turn == 0:
+                check_attn(out, q, kc, ke, vc, ve, table, lens, 0.1)
+                first.append(out)
+            assert torch.equal(out, first[i])
+    ops.read_status(ws, "turns")
+
+
+@pytest.mark.parametrize("lens", [[0, 0, 0], [0] * 300 + [33] + [0] * 300, [1] * 700, [16] * 37 + [0, 4000, 0] + [1] * 5, [5000] + [0] * 20, [15, 16, 17] * 333])
+def test_decode_runs_over_rows_of_all_lengths(ops, lens):
+    rng = np.random.default_rng(len(lens))
+    case = attn_case(rng, lens, 8, 2, 64)
+    for split in (0, 16):
+        check_attn(run_decode(ops, *case, lens, 0.1, split), *case, lens, 0.1)
+
+
 def test_decode_values_of_nan_and_what_they_reach(ops):
     rng = np.random.default_rng(11)
     lens = [40, 40]
