@@ -139,7 +139,7 @@ kv_slot_map_kernel(const int* __restrict__ ctx_lens, const int* __restrict__ new
 // ------------------------------------------------------------------- append --
 //
 // A run is a set of neighbouring rows whose slots lie in one page.  One warp takes a run's keys, or values, of one kv head: it holds up
-// to 16 rows in registers (a lane 4 or 2 neighbouring numbers of each), so that their largest magnitude and their rounding are one pass
+// to 16 rows in registers, 16 bytes a lane and load, so that their largest magnitude and their rounding are one pass
 // over memory, finds the page's scale and writes 8-bit rows.  Only where the scale of a page that already had tokens grows are its
 // earlier rows read, rounded anew and written back.  Nothing else of the page is touched.
 //
@@ -149,74 +149,69 @@ kv_slot_map_kernel(const int* __restrict__ ctx_lens, const int* __restrict__ new
 constexpr int kAppendWarps = 8;
 constexpr int kAppendMaxWindow = 16;  // a run that begins in a window lies within the 32 rows that a warp's lanes look at
 
-template <typename T, int PER>
+// 16 bytes of a row: 8 bf16 or 4 fp32 numbers.
+template <typename T>
 struct RowPiece {
-  static constexpr int kWords = PER * static_cast<int>(sizeof(T)) / 4;
-  uint32_t w[kWords];
-  __device__ __forceinline__ void load(const T* p) {
-    if constexpr (kWords == 4) {
-      const uint4 v = *reinterpret_cast<const uint4*>(p);
-      w[0] = v.x, w[1] = v.y, w[2] = v.z, w[3] = v.w;
-    } else if constexpr (kWords == 2) {
-      const uint2 v = *reinterpret_cast<const uint2*>(p);
-      w[0] = v.x, w[1] = v.y;
+  static constexpr int kNumbers = 16 / static_cast<int>(sizeof(T));
+  uint4 w;
+  __device__ __forceinline__ uint32_t word(int i) const { return i == 0 ? w.x : i == 1 ? w.y : i == 2 ? w.z : w.w; }
+  __device__ __forceinline__ float value(int i) const {
+    if constexpr (sizeof(T) == 4) return __uint_as_float(word(i));
+    else return __uint_as_float(i & 1 ? word(i / 2) & 0xffff0000u : word(i / 2) << 16);
+  }
+  // Bits of the largest magnitude as those of an fp32 number, infinities and NaN among them or not.
+  __device__ __forceinline__ uint32_t top() const {
+    if constexpr (sizeof(T) == 4) {
+      return max(max(w.x & 0x7fffffffu, w.y & 0x7fffffffu), max(w.z & 0x7fffffffu, w.w & 0x7fffffffu));
     } else {
-      w[0] = *reinterpret_cast<const uint32_t*>(p);
+      const uint32_t m = __vmaxu2(__vmaxu2(w.x & 0x7fff7fffu, w.y & 0x7fff7fffu), __vmaxu2(w.z & 0x7fff7fffu, w.w & 0x7fff7fffu));
+      return max(m >> 16, m & 0xffffu) << 16;
     }
   }
-  __device__ __forceinline__ float value(int i) const {
-    if constexpr (sizeof(T) == 4) return __uint_as_float(w[i]);
-    else return __uint_as_float(i & 1 ? w[i / 2] & 0xffff0000u : w[i / 2] << 16);
-  }
-  // bits of the largest finite magnitude
-  __device__ __forceinline__ uint32_t top() const {
+  __device__ __forceinline__ uint32_t finite_top() const {
     uint32_t m = 0;
 #pragma unroll
-    for (int i = 0; i < PER; ++i) {
+    for (int i = 0; i < kNumbers; ++i) {
       const uint32_t a = __float_as_uint(value(i)) & 0x7fffffffu;
       m = max(m, a < 0x7f800000u ? a : 0u);
     }
     return m;
   }
   // e4m3 codes of the numbers times `by`, which is a power of two: the product is exact, or underflows far below the smallest code.
-  // An infinity has no e4m3 number and must not look like one: it becomes NaN, as inf - inf.
-  __device__ __forceinline__ void store(uint8_t* to, float by) const {
-    float v[PER];
+  // An infinity has no e4m3 number and must not look like one: it becomes NaN where there may be any (`odd`).
+  __device__ __forceinline__ void store(uint8_t* to, float by, bool odd) const {
+    float v[kNumbers];
 #pragma unroll
-    for (int i = 0; i < PER; ++i) {
-      const float x = value(i);
-      v[i] = fabsf(x) < INFINITY ? x * by : NAN;
-    }
-    if constexpr (PER == 4) *reinterpret_cast<uint32_t*>(to) = to_e4m3x2(v[0], v[1]) | to_e4m3x2(v[2], v[3]) << 16;
-    else *reinterpret_cast<uint16_t*>(to) = static_cast<uint16_t>(to_e4m3x2(v[0], v[1]));
+    for (int i = 0; i < kNumbers; ++i) v[i] = value(i) * by;
+    if (odd)
+#pragma unroll
+      for (int i = 0; i < kNumbers; ++i) v[i] = fabsf(value(i)) < INFINITY ? v[i] : NAN;
+    const uint32_t lo = to_e4m3x2(v[0], v[1]) | to_e4m3x2(v[2], v[3]) << 16;
+    if constexpr (kNumbers == 8)
+      *reinterpret_cast<uint2*>(to) = make_uint2(lo, to_e4m3x2(v[4], v[5]) | to_e4m3x2(v[6], v[7]) << 16);
+    else *reinterpret_cast<uint32_t*>(to) = lo;
   }
 };
 
-// PER codes times `by`, rounded again.
-template <int PER>
-__device__ __forceinline__ void round_again(uint8_t* at, float by) {
+// Four codes times `by`, rounded again.
+__device__ __forceinline__ uint32_t round_again(uint32_t codes, float by) {
   uint32_t lo, hi;
-  if constexpr (PER == 4) {
-    e4m3x4_to_f16(*reinterpret_cast<const uint32_t*>(at), lo, hi);
-    const float2 a = __half22float2(*reinterpret_cast<const __half2*>(&lo)), b = __half22float2(*reinterpret_cast<const __half2*>(&hi));
-    *reinterpret_cast<uint32_t*>(at) = to_e4m3x2(a.x * by, a.y * by) | to_e4m3x2(b.x * by, b.y * by) << 16;
-  } else {
-    e4m3x4_to_f16(*reinterpret_cast<const uint16_t*>(at), lo, hi);
-    const float2 a = __half22float2(*reinterpret_cast<const __half2*>(&lo));
-    *reinterpret_cast<uint16_t*>(at) = static_cast<uint16_t>(to_e4m3x2(a.x * by, a.y * by));
-  }
+  e4m3x4_to_f16(codes, lo, hi);
+  const float2 a = __half22float2(*reinterpret_cast<const __half2*>(&lo)), b = __half22float2(*reinterpret_cast<const __half2*>(&hi));
+  return to_e4m3x2(a.x * by, a.y * by) | to_e4m3x2(b.x * by, b.y * by) << 16;
 }
 
 template <typename T, int D>
-__global__ void __launch_bounds__(kAppendWarps * 32)
+__global__ void __launch_bounds__(kAppendWarps * 32, D * sizeof(T) > 256 ? 2 : 4)
 kv8_append_kernel(const T* __restrict__ k_new, const T* __restrict__ v_new, long long k_stride, long long v_stride,
                   uint8_t* __restrict__ k_pool, uint8_t* __restrict__ v_pool, uint8_t* __restrict__ k_scale, uint8_t* __restrict__ v_scale,
                   const int* __restrict__ slots, int* __restrict__ err, int num_rows, int num_kv_heads, int num_blocks, int window) {
   grid_dep_wait();
   grid_dep_launch();
-  constexpr int PER = D / 32;
-  using Piece = RowPiece<T, PER>;
+  using Piece = RowPiece<T>;
+  constexpr int kLanes = D / Piece::kNumbers, kAtOnce = 32 / kLanes, kSteps = kKvPage / kAtOnce;  // lanes of a row; rows of a step
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int sub = lane / kLanes, col = lane % kLanes * Piece::kNumbers;
   const int row0 = blockIdx.x * window;  // lane l looks at row row0 - 1 + l
   const int my_row = row0 - 1 + lane;
   int slot = -1;
@@ -230,6 +225,7 @@ kv8_append_kernel(const T* __restrict__ k_new, const T* __restrict__ v_new, long
   unsigned starts = __ballot_sync(0xffffffffu, lane >= 1 && lane <= window && block >= 0 && block != left);
   const int items = 2 * num_kv_heads, total = __popc(starts) * items;
   int run = 0;  // of the lowest bit left in `starts`
+#pragma unroll 1
   for (int it = warp; it < total; it += kAppendWarps) {
     for (; run < it / items; ++run) starts &= starts - 1;
     const int first = __ffs(starts) - 1, item = it % items;
@@ -244,48 +240,74 @@ kv8_append_kernel(const T* __restrict__ k_new, const T* __restrict__ v_new, long
     const bool is_v = item >= num_kv_heads;
     const int h = is_v ? item - num_kv_heads : item;
     const long long stride = is_v ? v_stride : k_stride;
-    const T* src = (is_v ? v_new : k_new) + row * stride + h * D + lane * PER;
+    const T* src = (is_v ? v_new : k_new) + row * stride + h * D + col;
     const size_t cell = static_cast<size_t>(page) * num_kv_heads + h;
-    uint8_t* pool = (is_v ? v_pool : k_pool) + cell * (kKvPage * D) + lane * PER;
+    uint8_t* pool = (is_v ? v_pool : k_pool) + cell * (kKvPage * D) + col;
     uint8_t* scale = (is_v ? v_scale : k_scale) + cell;
     const int old = scale_exponent(*scale);
 
-    Piece x[kKvPage];
+    Piece x[kSteps];
     uint32_t top = 0;
 #pragma unroll
-    for (int i = 0; i < kKvPage; ++i)
-      if (i < n) x[i].load(src + i * stride);
-#pragma unroll
-    for (int i = 0; i < kKvPage; ++i)
-      if (i < n) top = max(top, x[i].top());
-    for (int i = kKvPage; i < n; ++i) {
-      Piece more;
-      more.load(src + i * stride);
-      top = max(top, more.top());
+    for (int s = 0; s < kSteps; ++s) {
+      const int i = s * kAtOnce + sub;
+      x[s].w = i < n ? *reinterpret_cast<const uint4*>(src + i * stride) : make_uint4(0u, 0u, 0u, 0u);
     }
-    int e = fit_exponent(__reduce_max_sync(0xffffffffu, top));
+#pragma unroll
+    for (int s = 0; s < kSteps; ++s) top = max(top, x[s].top());
+#pragma unroll 1
+    for (int i = kKvPage + sub; i < n; i += kAtOnce) top = max(top, Piece{*reinterpret_cast<const uint4*>(src + i * stride)}.top());
+    top = __reduce_max_sync(0xffffffffu, top);
+    const bool odd = top >= 0x7f800000u;
+    if (odd) {  // the largest finite magnitude instead
+      top = 0;
+#pragma unroll 1
+      for (int i = sub; i < n; i += kAtOnce) top = max(top, Piece{*reinterpret_cast<const uint4*>(src + i * stride)}.finite_top());
+      top = __reduce_max_sync(0xffffffffu, top);
+    }
+    int e = fit_exponent(top);
     if (low > 0 && old >= e) {
       e = old;
     } else {  // a new page, or a larger scale for one that has tokens
       const float by = power_of_two(old - e);
+      constexpr int kBatch = kSteps < 4 ? kSteps : 4;
+#pragma unroll 1
+      for (int r0 = sub; r0 < low; r0 += kBatch * kAtOnce) {
+        uint32_t codes[kBatch][Piece::kNumbers / 4];
 #pragma unroll
-      for (int i = 0; i < kKvPage - 1; ++i)
-        if (i < low) round_again<PER>(pool + i * D, by);
+        for (int s = 0; s < kBatch; ++s)
+          if (r0 + s * kAtOnce < low)
+#pragma unroll
+            for (int k = 0; k < Piece::kNumbers / 4; ++k)
+              codes[s][k] = *reinterpret_cast<const uint32_t*>(pool + (r0 + s * kAtOnce) * D + 4 * k);
+#pragma unroll
+        for (int s = 0; s < kBatch; ++s)
+          if (r0 + s * kAtOnce < low)
+#pragma unroll
+            for (int k = 0; k < Piece::kNumbers / 4; ++k)
+              *reinterpret_cast<uint32_t*>(pool + (r0 + s * kAtOnce) * D + 4 * k) = round_again(codes[s][k], by);
+      }
+      __syncwarp();
       if (lane == 0) *scale = static_cast<uint8_t>(e + 127);
     }
     const float by = power_of_two(-e);
+    // rows in rising order: of two that name one slot the later stays, whichever lanes hold them
 #pragma unroll
-    for (int i = 0; i < kKvPage; ++i) {
-      if (i < n) {
-        const int off = first + i < 32 ? __shfl_sync(0xffffffffu, slot, first + i) % kKvPage : slots[row + i] % kKvPage;
-        x[i].store(pool + off * D, by);
+    for (int s = 0; s < kSteps; ++s) {
+      const int i = s * kAtOnce + sub;
+      const int mine = __shfl_sync(0xffffffffu, slot, (first + i) & 31);
+      bool last = i < n;
+#pragma unroll
+      for (int d = 1; d < kAtOnce; ++d) {
+        const int other = __shfl_down_sync(0xffffffffu, mine, d * kLanes);
+        if (sub + d < kAtOnce && i + d < n && other == mine) last = false;
       }
+      if (last) x[s].store(pool + mine % kKvPage * D, by, odd);
+      if constexpr (kAtOnce > 1) __syncwarp();
     }
-    for (int i = kKvPage; i < n; ++i) {
-      Piece more;
-      more.load(src + i * stride);
-      more.store(pool + slots[row + i] % kKvPage * D, by);
-    }
+#pragma unroll 1
+    for (int i = kKvPage; i < n; ++i)
+      if (sub == 0) Piece{*reinterpret_cast<const uint4*>(src + i * stride)}.store(pool + slots[row + i] % kKvPage * D, by, odd);
   }
 }
 
@@ -345,7 +367,7 @@ extern "C" int b200_kv8_append(const void* k_new, const void* v_new, int64_t k_r
   B200_REQUIRE(dtype == 0 || dtype == 1, "kv8_append: dtype %d is neither 0 (bf16) nor 1 (f32)", dtype);
   B200_REQUIRE(static_cast<long long>(num_blocks) * kKvPage < (1ll << 31), "kv8_append: %d pages have more slots than 32 bits count", num_blocks);
   B200_REQUIRE(num_rows < (1 << 30) && num_kv_heads <= 1 << 20, "kv8_append: too many rows or heads");
-  const int align = head_dim / 32 * (dtype == 0 ? 2 : 4);  // bytes a lane loads at once
+  const int align = 16;  // bytes a lane loads at once
   const int elem = dtype == 0 ? 2 : 4;
   B200_REQUIRE(reinterpret_cast<uintptr_t>(k_new) % align == 0 && reinterpret_cast<uintptr_t>(v_new) % align == 0 &&
                    k_row_stride * elem % align == 0 && v_row_stride * elem % align == 0 && k_row_stride >= 0 && v_row_stride >= 0,

@@ -45,7 +45,7 @@ def test_append_refuses():
     refused(call(dim=96), "head_dim 96")
     refused(call(dtype=2), "dtype 2")
     refused(call(blocks=2 ** 27), "32 bits")
-    refused(call(kn=P + 4), "multiples of 8")
+    refused(call(kn=P + 8), "multiples of 16")
     refused(call(dtype=1, vs=514), "multiples of 16")
     refused(call(ks=-512), "multiples")
     refused(call(vp=P + 8), "16-byte aligned")
