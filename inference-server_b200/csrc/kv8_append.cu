@@ -159,17 +159,14 @@ struct RowPiece {
     if constexpr (sizeof(T) == 4) return __uint_as_float(word(i));
     else return __uint_as_float(i & 1 ? word(i / 2) & 0xffff0000u : word(i / 2) << 16);
   }
-  // Bits of the largest magnitude as those of an fp32 number, infinities and NaN among them or not.
-  __device__ __forceinline__ uint32_t top() const {
-    if constexpr (sizeof(T) == 4) {
-      return max(max(w.x & 0x7fffffffu, w.y & 0x7fffffffu), max(w.z & 0x7fffffffu, w.w & 0x7fffffffu));
-    } else {
-      const uint32_t m = __vmaxu2(__vmaxu2(w.x & 0x7fff7fffu, w.y & 0x7fff7fffu), __vmaxu2(w.z & 0x7fff7fffu, w.w & 0x7fff7fffu));
-      return max(m >> 16, m & 0xffffu) << 16;
-    }
+  // Largest magnitudes so far, infinities and NaN among them: bits of an fp32 number, or of two bf16 numbers side by side.
+  __device__ __forceinline__ uint32_t top(uint32_t m) const {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) m = sizeof(T) == 4 ? max(m, word(i) & 0x7fffffffu) : __vmaxu2(m, word(i) & 0x7fff7fffu);
+    return m;
   }
-  __device__ __forceinline__ uint32_t finite_top() const {
-    uint32_t m = 0;
+  __device__ __forceinline__ static uint32_t top_of(uint32_t m) { return sizeof(T) == 4 ? m : max(m >> 16, m & 0xffffu) << 16; }
+  __device__ __forceinline__ uint32_t finite_top(uint32_t m) const {
 #pragma unroll
     for (int i = 0; i < kNumbers; ++i) {
       const uint32_t a = __float_as_uint(value(i)) & 0x7fffffffu;
@@ -178,18 +175,22 @@ struct RowPiece {
     return m;
   }
   // e4m3 codes of the numbers times `by`, which is a power of two: the product is exact, or underflows far below the smallest code.
-  // An infinity has no e4m3 number and must not look like one: it becomes NaN where there may be any (`odd`).
-  __device__ __forceinline__ void store(uint8_t* to, float by, bool odd) const {
-    float v[kNumbers];
+  // An infinity has no e4m3 number and must not look like one: where there may be any (`ODD`) it becomes NaN.
+  template <bool ODD>
+  __device__ __forceinline__ void store(uint8_t* to, float by) const {
+    uint32_t codes[kNumbers / 4];
 #pragma unroll
-    for (int i = 0; i < kNumbers; ++i) v[i] = value(i) * by;
-    if (odd)
+    for (int k = 0; k < kNumbers / 4; ++k) {
+      float v[4];
 #pragma unroll
-      for (int i = 0; i < kNumbers; ++i) v[i] = fabsf(value(i)) < INFINITY ? v[i] : NAN;
-    const uint32_t lo = to_e4m3x2(v[0], v[1]) | to_e4m3x2(v[2], v[3]) << 16;
-    if constexpr (kNumbers == 8)
-      *reinterpret_cast<uint2*>(to) = make_uint2(lo, to_e4m3x2(v[4], v[5]) | to_e4m3x2(v[6], v[7]) << 16);
-    else *reinterpret_cast<uint32_t*>(to) = lo;
+      for (int i = 0; i < 4; ++i) {
+        const float x = value(4 * k + i);
+        v[i] = ODD && !(fabsf(x) < INFINITY) ? NAN : x * by;
+      }
+      codes[k] = to_e4m3x2(v[0], v[1]) | to_e4m3x2(v[2], v[3]) << 16;
+    }
+    if constexpr (kNumbers == 8) *reinterpret_cast<uint2*>(to) = make_uint2(codes[0], codes[1]);
+    else *reinterpret_cast<uint32_t*>(to) = codes[0];
   }
 };
 
@@ -232,10 +233,19 @@ kv8_append_kernel(const T* __restrict__ k_new, const T* __restrict__ v_new, long
     const int page = __shfl_sync(0xffffffffu, block, first);
     const unsigned same = __ballot_sync(0xffffffffu, block == page) >> first;
     int n = __ffs(~same) - 1;  // rows of the run among those of the lanes; first >= 1, so a bit of `same` is clear
-    int low = __reduce_min_sync(0xffffffffu, lane >= first && lane < first + n ? slot % kKvPage : kKvPage);
-    const int row = row0 - 1 + first;
-    if (first + n == 32)  // slots named more than once can make a run longer than a page
-      for (; row + n < num_rows && slots[row + n] >= 0 && slots[row + n] / kKvPage == page; ++n) low = min(low, slots[row + n] % kKvPage);
+    const int row = row0 - 1 + first, low0 = __shfl_sync(0xffffffffu, slot, first);
+    // The usual run names one slot after the other.
+    const bool inside = lane >= first && lane < first + n;
+    bool plain = __all_sync(0xffffffffu, !inside || slot - lane == low0 - first) && n <= kKvPage;
+    int low = low0 % kKvPage;
+    if (!plain || first + n == 32) {
+      low = __reduce_min_sync(0xffffffffu, inside ? slot % kKvPage : kKvPage);
+      // slots named more than once can make a run longer than a page
+      for (; row + n < num_rows && slots[row + n] >= 0 && slots[row + n] / kKvPage == page; ++n) {
+        low = min(low, slots[row + n] % kKvPage);
+        plain = false;
+      }
+    }
 
     const bool is_v = item >= num_kv_heads;
     const int h = is_v ? item - num_kv_heads : item;
@@ -250,19 +260,19 @@ kv8_append_kernel(const T* __restrict__ k_new, const T* __restrict__ v_new, long
     uint32_t top = 0;
 #pragma unroll
     for (int s = 0; s < kSteps; ++s) {
-      const int i = s * kAtOnce + sub;
-      x[s].w = i < n ? *reinterpret_cast<const uint4*>(src + i * stride) : make_uint4(0u, 0u, 0u, 0u);
+      x[s].w = make_uint4(0u, 0u, 0u, 0u);
+      if (s * kAtOnce + sub < n) x[s].w = *reinterpret_cast<const uint4*>(src + (s * kAtOnce + sub) * stride);
     }
 #pragma unroll
-    for (int s = 0; s < kSteps; ++s) top = max(top, x[s].top());
+    for (int s = 0; s < kSteps; ++s) top = x[s].top(top);
 #pragma unroll 1
-    for (int i = kKvPage + sub; i < n; i += kAtOnce) top = max(top, Piece{*reinterpret_cast<const uint4*>(src + i * stride)}.top());
-    top = __reduce_max_sync(0xffffffffu, top);
-    const bool odd = top >= 0x7f800000u;
-    if (odd) {  // the largest finite magnitude instead
+    for (int i = kKvPage + sub; i < n; i += kAtOnce) top = Piece{*reinterpret_cast<const uint4*>(src + i * stride)}.top(top);
+    top = __reduce_max_sync(0xffffffffu, Piece::top_of(top));
+    if (top >= 0x7f800000u) {  // the largest finite magnitude instead
+      plain = false;
       top = 0;
 #pragma unroll 1
-      for (int i = sub; i < n; i += kAtOnce) top = max(top, Piece{*reinterpret_cast<const uint4*>(src + i * stride)}.finite_top());
+      for (int i = sub; i < n; i += kAtOnce) top = Piece{*reinterpret_cast<const uint4*>(src + i * stride)}.finite_top(top);
       top = __reduce_max_sync(0xffffffffu, top);
     }
     int e = fit_exponent(top);
@@ -291,23 +301,17 @@ kv8_append_kernel(const T* __restrict__ k_new, const T* __restrict__ v_new, long
       if (lane == 0) *scale = static_cast<uint8_t>(e + 127);
     }
     const float by = power_of_two(-e);
-    // rows in rising order: of two that name one slot the later stays, whichever lanes hold them
+    if (plain) {
+      uint8_t* to = pool + (low + sub) * D;
 #pragma unroll
-    for (int s = 0; s < kSteps; ++s) {
-      const int i = s * kAtOnce + sub;
-      const int mine = __shfl_sync(0xffffffffu, slot, (first + i) & 31);
-      bool last = i < n;
-#pragma unroll
-      for (int d = 1; d < kAtOnce; ++d) {
-        const int other = __shfl_down_sync(0xffffffffu, mine, d * kLanes);
-        if (sub + d < kAtOnce && i + d < n && other == mine) last = false;
-      }
-      if (last) x[s].store(pool + mine % kKvPage * D, by, odd);
-      if constexpr (kAtOnce > 1) __syncwarp();
-    }
+      for (int s = 0; s < kSteps; ++s)
+        if (s * kAtOnce + sub < n) x[s].template store<false>(to + s * kAtOnce * D, by);
+    } else {  // one row after the other: of those that name one slot the last stays
 #pragma unroll 1
-    for (int i = kKvPage; i < n; ++i)
-      if (sub == 0) Piece{*reinterpret_cast<const uint4*>(src + i * stride)}.store(pool + slots[row + i] % kKvPage * D, by, odd);
+      for (int i = 0; i < n; ++i) {
+        if (sub == 0) Piece{*reinterpret_cast<const uint4*>(src + i * stride)}.template store<true>(pool + slots[row + i] % kKvPage * D, by);
+      }
+    }
   }
 }
 
