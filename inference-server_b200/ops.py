@@ -209,12 +209,19 @@ class KvSlotMap(NamedTuple):
 _device_index = torch.Tensor.get_device
 
 
-def _on_current_device(*operands: torch.Tensor) -> None:
-    """The kernels run on the current device's current stream: operands of another device are an error and not a fault."""
-    if set(map(_device_index, operands)) != {torch.cuda.current_device()}:
+def _stream_of(*operands: torch.Tensor) -> int:
+    """The current stream of the device that all operands are on.  The kernels run on the current device: operands of another are an error
+    and not a fault."""
+    devices = set(map(_device_index, operands))
+    here = devices.pop()
+    if here < 0 or devices:
         for t in operands:
-            if t.get_device() != torch.cuda.current_device():
-                raise ValueError(f"an operand is on {t.device}, the current device is cuda:{torch.cuda.current_device()}")
+            if not t.is_cuda:
+                raise ValueError("operands must be CUDA tensors (this path has no CPU implementation)")
+        raise ValueError(f"operands are on {sorted({str(t.device) for t in operands})}")
+    if here != torch.cuda.current_device():
+        raise ValueError(f"operands are on cuda:{here}, the current device is cuda:{torch.cuda.current_device()}")
+    return torch.cuda.current_stream().cuda_stream if _raw_stream is None else _raw_stream(here)
 
 
 def _status_word(status: torch.Tensor | None) -> None:
@@ -234,18 +241,16 @@ def kv8_pools(num_blocks: int, num_kv_heads: int, head_dim: int, device="cuda"):
 def _kv8_cache(k_pool, v_pool, k_scale, v_scale) -> tuple[int, int, int]:
     shape = k_pool.shape
     if not (k_pool.dtype is KV8_DTYPE and v_pool.dtype is KV8_DTYPE and k_scale.dtype is KV8_SCALE_DTYPE and v_scale.dtype is KV8_SCALE_DTYPE
-            and k_pool.is_contiguous() and v_pool.is_contiguous() and k_scale.is_contiguous() and v_scale.is_contiguous()
-            and k_pool.is_cuda and v_pool.is_cuda and k_scale.is_cuda and v_scale.is_cuda):
+            and k_pool.is_contiguous() and v_pool.is_contiguous() and k_scale.is_contiguous() and v_scale.is_contiguous()):
         _need(k_pool, "k_pool", KV8_DTYPE)
         _need(v_pool, "v_pool", KV8_DTYPE)
         _need(k_scale, "k_scale", KV8_SCALE_DTYPE)
         _need(v_scale, "v_scale", KV8_SCALE_DTYPE)
     if len(shape) != 4 or shape[2] != 16:
         raise ValueError(f"k_pool must be [num_blocks, kv_heads, 16, head_dim], got {list(shape)}")
-    nb, Hkv, _, D = shape
-    if v_pool.shape != shape or k_scale.shape != (nb, Hkv) or v_scale.shape != (nb, Hkv):
+    if v_pool.shape != shape or k_scale.shape != shape[:2] or v_scale.shape != shape[:2]:
         raise ValueError("pools and scales do not match each other")
-    return nb, Hkv, D
+    return shape[0], shape[1], shape[3]
 
 
 def kv_slot_map(ctx_lens, new_lens, block_table, supply, supply_used, num_rows: int, num_blocks: int,
@@ -254,22 +259,28 @@ def kv_slot_map(ctx_lens, new_lens, block_table, supply, supply_used, num_rows: 
     need are taken from `supply` [any], free page ids, from entry supply_used [1] on, and entered into block_table [B, max_pages] in
     place.  `num_rows`: rows of the pass, at least the sum of new_lens; rows behind the last token get slot -1.  Slots are
     page * 16 + position % 16, for `kv8_append` or any other cache of 16-token pages; page ids outside [0, num_blocks) are findings."""
-    for t, name in ((ctx_lens, "ctx_lens"), (new_lens, "new_lens"), (block_table, "block_table"), (supply, "supply"),
-                    (supply_used, "supply_used")):
-        _need(t, name, torch.int32)
-    _status_word(status)
-    _on_current_device(ctx_lens, new_lens, block_table, supply, supply_used)
-    B, R = ctx_lens.shape[0], int(num_rows)
-    if ctx_lens.dim() != 1 or new_lens.shape != ctx_lens.shape or block_table.dim() != 2 or block_table.shape[0] != B or supply_used.numel() != 1:
+    for t in (ctx_lens, new_lens, block_table, supply, supply_used):
+        if t.dtype is not torch.int32 or not t.is_contiguous():
+            raise ValueError("lengths, block table, supply and supply_used must be contiguous int32 tensors")
+    stream = _stream_of(ctx_lens, new_lens, block_table, supply, supply_used)
+    if status is not None:
+        _status_word(status)
+        _stream_of(ctx_lens, status)
+    table = block_table.shape
+    B, R = table[0], int(num_rows)
+    if len(table) != 2 or ctx_lens.shape != table[:1] or new_lens.shape != table[:1] or supply_used.numel() != 1:
         raise ValueError("lengths, block table or supply_used do not match")
     if R < 0:
         raise ValueError(f"{R} rows")
+    # one allocation; views are made in one go
     m = KvSlotMap(*torch.split_with_sizes(ctx_lens.new_empty(2 * B + 2 + 3 * R), (B, B + 1, R, R, R, 1)))
+    lens = m.lens.data_ptr()
+    rows = lens + 4 * (2 * B + 1)
     rc = _lib.load().b200_kv_slot_map(
-        _ptr(ctx_lens), _ptr(new_lens), _ptr(block_table), _ptr(supply), _ptr(supply_used), supply.numel(), _ptr(m.lens),
-        _ptr(m.row_start), _ptr(m.row_seq), _ptr(m.positions), _ptr(m.slots), _ptr(m.supply_used), _ptr(status), B, R,
-        int(num_blocks), block_table.shape[1], _stream())
-    check(rc, "b200_kv_slot_map")
+        ctx_lens.data_ptr(), new_lens.data_ptr(), block_table.data_ptr(), supply.data_ptr(), supply_used.data_ptr(), supply.numel(), lens,
+        lens + 4 * B, rows, rows + 4 * R, rows + 8 * R, rows + 12 * R, _ptr(status), B, R, int(num_blocks), table[1], stream)
+    if rc:
+        check(rc, "b200_kv_slot_map")
     return m
 
 
@@ -279,34 +290,44 @@ def kv8_append(k_new, v_new, k_pool, v_pool, k_scale, v_scale, slots, status: to
     by side, in order.  The scale of a page is the smallest power of two for which its largest number fits; see the header
     for how it grows."""
     nb, Hkv, D = _kv8_cache(k_pool, v_pool, k_scale, v_scale)
-    _need(slots, "slots", torch.int32)
-    _status_word(status)
-    if k_new.dtype not in DTYPE_CODE or v_new.dtype != k_new.dtype:
-        raise ValueError(f"k_new and v_new must be bfloat16 or float32, got {k_new.dtype} and {v_new.dtype}")
+    if slots.dtype is not torch.int32 or not slots.is_contiguous():
+        raise ValueError("slots must be a contiguous int32 tensor")
+    dtype, shape = k_new.dtype, k_new.shape
+    if dtype not in DTYPE_CODE or v_new.dtype is not dtype:
+        raise ValueError(f"k_new and v_new must be bfloat16 or float32, got {dtype} and {v_new.dtype}")
     R = slots.numel()
-    for t, name in ((k_new, "k_new"), (v_new, "v_new")):
-        if not t.is_cuda:
-            raise ValueError(f"{name} must be a CUDA tensor (this path has no CPU implementation)")
-        if t.shape != (R, Hkv, D):
-            raise ValueError(f"{name} must be [{R}, {Hkv}, {D}], got {list(t.shape)}")
-        if R > 0 and (t.stride(2) != 1 or (Hkv > 1 and t.stride(1) != D) or (R > 1 and t.stride(0) < Hkv * D)):
-            raise ValueError(f"{name} may be strided in its rows only")
-    _on_current_device(k_pool, v_pool, k_scale, v_scale, k_new, v_new, slots)
+    if shape != (R, Hkv, D) or v_new.shape != shape:
+        raise ValueError(f"k_new and v_new must be [{R}, {Hkv}, {D}], got {list(shape)} and {list(v_new.shape)}")
+    stream = _stream_of(k_pool, v_pool, k_scale, v_scale, k_new, v_new, slots)
+    if status is not None:
+        _status_word(status)
+        _stream_of(slots, status)
     if R == 0:
         return
+    for t in (k_new, v_new):
+        if not t.is_contiguous() and (t.stride(2) != 1 or (Hkv > 1 and t.stride(1) != D) or (R > 1 and t.stride(0) < Hkv * D)):
+            raise ValueError("k_new and v_new may be strided in their rows only")
     rc = _lib.load().b200_kv8_append(
-        _ptr(k_new), _ptr(v_new), k_new.stride(0), v_new.stride(0), _ptr(k_pool), _ptr(v_pool), _ptr(k_scale), _ptr(v_scale),
-        _ptr(slots), _ptr(status), R, Hkv, D, nb, DTYPE_CODE[k_new.dtype], _stream())
-    check(rc, "b200_kv8_append")
+        k_new.data_ptr(), v_new.data_ptr(), k_new.stride(0), v_new.stride(0), k_pool.data_ptr(), v_pool.data_ptr(), k_scale.data_ptr(),
+        v_scale.data_ptr(), slots.data_ptr(), _ptr(status), R, Hkv, D, nb, DTYPE_CODE[dtype], stream)
+    if rc:
+        check(rc, "b200_kv8_append")
 
 
-def _attn_out(q: torch.Tensor, out: torch.Tensor | None) -> torch.Tensor:
+def _kv8_queries(q, out, index, workspace, D: int, what: str):
+    """Checks that the two attention calls share; rows and heads of q, and an `out` if none is given."""
+    shape = q.shape
+    if len(shape) != 3 or shape[2] != D:
+        raise ValueError(f"q must be [{what}, heads, {D}], got {list(shape)}")
+    if q.dtype is not torch.bfloat16 or not q.is_contiguous() or index.dtype is not torch.int32 or not index.is_contiguous():
+        raise ValueError("q must be contiguous bfloat16, block table and lengths contiguous int32 tensors")
+    if workspace is not None and (workspace.dtype is not torch.uint8 or not workspace.is_contiguous()):
+        raise ValueError("workspace must be a contiguous uint8 tensor")
     if out is None:
-        return torch.empty_like(q)
-    _need(out, "out", torch.bfloat16)
-    if out.shape != q.shape:
-        raise ValueError("out does not match q")
-    return out
+        out = torch.empty_like(q)
+    elif out.dtype is not torch.bfloat16 or not out.is_contiguous() or out.shape != shape:
+        raise ValueError("out must be a contiguous bfloat16 tensor of q's shape")
+    return shape[0], shape[1], out
 
 
 def kv8_attn_workspace(batch: int, num_q_heads: int, num_kv_heads: int, head_dim: int, max_pages: int, device,
@@ -321,25 +342,20 @@ def kv8_attn_decode(q, k_pool, v_pool, k_scale, v_scale, block_table, ctx_lens, 
     """`paged_attn_decode` over an 8-bit page cache: softmax(q K^T * scale) V for one bf16 query row [B, Hq, D] per sequence; head_dim 64
     or 128, any head grouping.  `split_tokens`: tokens that a CTA takes at least; 0: the library's choice."""
     nb, Hkv, D = _kv8_cache(k_pool, v_pool, k_scale, v_scale)
-    _need(q, "q", torch.bfloat16)
-    _need(block_table, "block_table", torch.int32)
-    _need(ctx_lens, "ctx_lens", torch.int32)
-    if q.dim() != 3 or q.shape[2] != D:
-        raise ValueError(f"q must be [batch, heads, {D}], got {list(q.shape)}")
-    B, Hq, _ = q.shape
-    if block_table.dim() != 2 or block_table.shape[0] != B or ctx_lens.shape != (B,):
-        raise ValueError("block_table / ctx_lens batch mismatch")
-    out = _attn_out(q, out)
+    B, Hq, out = _kv8_queries(q, out, block_table, workspace, D, "batch")
+    table = block_table.shape
+    if len(table) != 2 or table[0] != B or ctx_lens.shape != table[:1] or ctx_lens.dtype is not torch.int32 or not ctx_lens.is_contiguous():
+        raise ValueError("block_table [batch, pages] and ctx_lens [batch] int32 must match q")
+    stream = _stream_of(q, k_pool, v_pool, k_scale, v_scale, block_table, ctx_lens, out, q if workspace is None else workspace)
     if B == 0:
         return out
     if workspace is None:
-        workspace = kv8_attn_workspace(B, Hq, Hkv, D, block_table.shape[1], q.device, int(split_tokens))
-    _need(workspace, "workspace", torch.uint8)
-    _on_current_device(q, k_pool, v_pool, k_scale, v_scale, block_table, ctx_lens, out, workspace)
+        workspace = kv8_attn_workspace(B, Hq, Hkv, D, table[1], q.device, int(split_tokens))
     rc = _lib.load().b200_kv8_attn_decode(
-        _ptr(q), _ptr(k_pool), _ptr(v_pool), _ptr(k_scale), _ptr(v_scale), _ptr(block_table), _ptr(ctx_lens), _ptr(out),
-        _ptr(workspace), workspace.numel(), B, Hq, Hkv, D, nb, block_table.shape[1], float(scale), int(split_tokens), _stream())
-    check(rc, "b200_kv8_attn_decode")
+        q.data_ptr(), k_pool.data_ptr(), v_pool.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), block_table.data_ptr(), ctx_lens.data_ptr(),
+        out.data_ptr(), workspace.data_ptr(), workspace.numel(), B, Hq, Hkv, D, nb, table[1], float(scale), int(split_tokens), stream)
+    if rc:
+        check(rc, "b200_kv8_attn_decode")
     return out
 
 
@@ -352,27 +368,22 @@ def kv8_attn_prefill_workspace(num_tokens: int, first_pos: int, num_q_heads: int
 def kv8_attn_prefill(q, k_pool, v_pool, k_scale, v_scale, table_row, first_pos: int, scale: float, workspace: torch.Tensor | None = None,
                      out: torch.Tensor | None = None) -> torch.Tensor:
     """`paged_attn_prefill` over an 8-bit page cache: causal attention of consecutive prompt tokens of one sequence, q [R, Hq, D] bf16 at
-    positions first_pos .. first_pos + R - 1, keys and values already in their slots; table_row [max_pages] int32.  head_dim 64 or 128, up to 128 query
-    heads per kv head.  Few rows over many keys are shared out along the keys and joined in the workspace."""
+    positions first_pos .. first_pos + R - 1, keys and values already in their slots; table_row [max_pages] int32.  head_dim 64 or 128,
+    up to 128 query heads per kv head.  Few rows over many keys are shared out along the keys and joined in the workspace."""
     nb, Hkv, D = _kv8_cache(k_pool, v_pool, k_scale, v_scale)
-    _need(q, "q", torch.bfloat16)
-    _need(table_row, "table_row", torch.int32)
-    if q.dim() != 3 or q.shape[2] != D:
-        raise ValueError(f"q must be [tokens, heads, {D}], got {list(q.shape)}")
+    R, Hq, out = _kv8_queries(q, out, table_row, workspace, D, "tokens")
     if table_row.dim() != 1:
         raise ValueError("table_row must be one row of a block table")
-    R, Hq, _ = q.shape
-    out = _attn_out(q, out)
+    stream = _stream_of(q, k_pool, v_pool, k_scale, v_scale, table_row, out, q if workspace is None else workspace)
     if R == 0:
         return out
     if workspace is None:
         workspace = kv8_attn_prefill_workspace(R, int(first_pos), Hq, Hkv, D, q.device)
-    _need(workspace, "workspace", torch.uint8)
-    _on_current_device(q, k_pool, v_pool, k_scale, v_scale, table_row, out, workspace)
     rc = _lib.load().b200_kv8_attn_prefill(
-        _ptr(q), _ptr(k_pool), _ptr(v_pool), _ptr(k_scale), _ptr(v_scale), _ptr(table_row), _ptr(out), _ptr(workspace), workspace.numel(),
-        R, int(first_pos), Hq, Hkv, D, nb, table_row.numel(), float(scale), _stream())
-    check(rc, "b200_kv8_attn_prefill")
+        q.data_ptr(), k_pool.data_ptr(), v_pool.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), table_row.data_ptr(), out.data_ptr(),
+        workspace.data_ptr(), workspace.numel(), R, int(first_pos), Hq, Hkv, D, nb, table_row.numel(), float(scale), stream)
+    if rc:
+        check(rc, "b200_kv8_attn_prefill")
     return out
 
 
