@@ -15,13 +15,17 @@
 //
 //   grid     (CTAs of tiles, late ones first) x splits of the keys x kv heads.  The keys are split where the tiles alone leave SMs idle; fp32
 //            partials are then joined by kv8_attn_join_kernel.
-//   warp 0   producer: per key tile, 8 pages of keys by TMA and 8 of values as plain bulk copies, two stages each.
-//   warps 0, 3   half of a tile's values each: 16 bytes of a row to 16 f16 numbers; zero for what lies behind the last token, where a page
-//            may hold NaN.
+//   warp 0   producer: per key tile, 8 pages of keys by TMA into three stages and 8 of values as plain bulk copies into two.  It does nothing
+//            else: when it converted values too, it asked for keys so late that S waited for memory.
 //   warp 1   S issuer (one thread), warp 2 P V issuer (one thread).
-//   warps 4-7, 8-11   first the queries of both tiles (bf16 to hi and lo, a row's top by shuffles), then the softmax of tile 0 and of tile 1,
+//   warps 4-7    a quarter of a tile's values each: 16 bytes of a row to 16 f16 numbers; zero for what lies behind the last token, where a page
+//            may hold NaN.  One such warp per scheduler: with two of them on two, the softmax warps beside them held up the others.
+//   warps 8-11, 12-15   first the queries of both tiles (bf16 to hi and lo, a row's top by shuffles), then the softmax of tile 0 and of tile 1,
 //            a thread per score row; the scales of a key tile's 8 pages come to each warp by its own lanes, two key tiles
-//            ahead (ids) and one (scales), and from a corner of shared memory to all lanes.
+//            ahead (ids) and one (scales), and from a corner of shared memory to all lanes.  (Two threads per row, 16 softmax warps, and one
+//            predicate per key tile between them: 296 us where a thread per row took 276.)
+//   A CTA with one tile of rows takes every second key tile of it on the other tile's warps, with an accumulator and reference of their own,
+//   and adds the two up at the end.
 //
 // Every mbarrier wait is bounded; a wait that runs out records kErrDevWaitTimeout and the thread stops waiting but keeps the loop
 // structure, so the kernel ends.
@@ -35,7 +39,9 @@
 
 namespace b200 {
 
-constexpr int kKv8PrefillThreads = 384;
+constexpr int kKv8SoftmaxWarps = 8;
+constexpr int kKv8PrefillThreads = (8 + kKv8SoftmaxWarps) * 32;
+constexpr int kKv8KStages = 3;
 constexpr float kKv8PLift = 6.f;  // weights are taken times 2^6, at most 2^14 with the slack of kTcRescaleLog2
 
 template <int D>
@@ -43,13 +49,14 @@ struct Kv8PrefillCfg {
   static constexpr int kTile8 = kTcKeys * D;                 // bytes of 128 rows in 8 bits
   static constexpr int kTile16 = 2 * kTile8;
   static constexpr int kQ = 0;                                // [2 tiles][hi, lo]
-  static constexpr int kK = kQ + 4 * kTile8;                  // [2 stages]
-  static constexpr int kRaw = kK + 2 * kTile8;                // [2 stages] values as they are
-  static constexpr int kV = kRaw + 2 * kTile8;                // [2 stages] values in f16
-  static constexpr int kScales = kV + 2 * kTile16;            // [8 warps][2][8 pages] float4
-  static constexpr int kRowScale = kScales + 8 * 2 * 8 * 16;  // [2 tiles][128] float
-  static constexpr int kSums = kRowScale + 2 * 128 * 4;       // [128] float
-  static constexpr int kBars = kSums + 128 * 4;
+  static constexpr int kK = kQ + 4 * kTile8;                   // [kKv8KStages]
+  static constexpr int kRaw = kK + kKv8KStages * kTile8;       // [2 stages] values as they are
+  static constexpr int kV = kRaw + 2 * kTile8;                 // [2 stages] values in f16
+  static constexpr int kScales = kV + 2 * kTile16;             // [8 warps][2][8 pages] float4
+  static constexpr int kRowScale = kScales + 8 * 2 * 8 * 16;   // [2 tiles][128] float
+  static constexpr int kSums = kRowScale + 2 * 128 * 4;        // the same
+  static constexpr int kRefs = kSums + 2 * 128 * 4;            // the same
+  static constexpr int kBars = kRefs + 2 * 128 * 4;
   static constexpr int kSmemBytes = kBars + 256 + 1024 /* alignment slack */;
 };
 
@@ -84,17 +91,17 @@ __device__ __forceinline__ float max_of_3(float a, float b, float c) {
   return d;
 }
 
-// One warp's half of a tile of values, rows row0 .. row0 + 63, to f16; those from `rows` on hold no tokens and become zero (a page may hold
+// One warp's quarter of a tile of values, rows row0 .. row0 + 31, to f16; those from `rows` on hold no tokens and become zero (a page may hold
 // NaN there).  A lane takes 16 bytes of a row at a time, which become two pieces of a swizzled row.  For head_dim 128 a quarter warp
 // takes the first half of one row and the second half of the next: its loads are in different banks, and so are its stores,
-// whose pieces are XORed with numbers that differ in bit 0.  The loop is short code on purpose: unrolled it took 2900 cycles a half tile, nearly all
+// whose pieces are XORed with numbers that differ in bit 0.  The loop is short code on purpose: unrolled, half a tile took 2900 cycles, nearly all
 // of them waits for instructions, which the softmax warps' long straight-line code keeps out of the instruction cache.
 template <int D>
 __device__ __forceinline__ void values_to_f16(uint32_t from, uint32_t to, int row0, int rows, int lane) {
   constexpr int kPieces = D / 16, kRowsAt = 32 / kPieces;  // pieces of a row; rows that the warp takes at a time
   constexpr uint32_t kAtomGroup = D / 64 * 1024;           // 8 rows of f16
-  if (rows < row0 + kTcKeys / 2) {
-    for (int i = max(rows, row0) * kPieces + lane; i < (row0 + kTcKeys / 2) * kPieces; i += 32)
+  if (rows < row0 + kTcKeys / 4) {
+    for (int i = max(rows, row0) * kPieces + lane; i < (row0 + kTcKeys / 4) * kPieces; i += 32)
       asm volatile("st.shared.v4.b32 [%0], {%1,%1,%1,%1};" ::"r"(from + i * 16), "r"(0) : "memory");
     __syncwarp();
   }
@@ -107,12 +114,12 @@ __device__ __forceinline__ void values_to_f16(uint32_t from, uint32_t to, int ro
   uint32_t w[4];
   lds_words<16>(src, w);
 #pragma unroll 2
-  for (int r = row0 + lr; r < row0 + kTcKeys / 2; r += kRowsAt) {
+  for (int r = row0 + lr; r < row0 + kTcKeys / 4; r += kRowsAt) {
     uint32_t x[4], a[8];
 #pragma unroll
     for (int k = 0; k < 4; ++k) x[k] = w[k];
     src += kRowsAt * D;
-    if (r + kRowsAt < row0 + kTcKeys / 2) lds_words<16>(src, w);
+    if (r + kRowsAt < row0 + kTcKeys / 4) lds_words<16>(src, w);
 #pragma unroll
     for (int k = 0; k < 4; ++k) e4m3x4_to_f16(x[k], a[2 * k], a[2 * k + 1]);
     const uint32_t row = to + (r >> 3) * kAtomGroup + half_off;
@@ -124,28 +131,6 @@ __device__ __forceinline__ void values_to_f16(uint32_t from, uint32_t to, int ro
   }
   fence_proxy_async();  // the tensor core reads the tile, and the next copy writes the stage, through the async proxy
   __syncwarp();
-}
-
-// Two fp32 numbers in one instruction.
-__device__ __forceinline__ uint64_t pair_of(float lo, float hi) {
-  uint64_t r;
-  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(lo), "f"(hi));
-  return r;
-}
-__device__ __forceinline__ float2 halves(uint64_t v) {
-  float2 r;
-  asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(v));
-  return r;
-}
-__device__ __forceinline__ uint64_t fma_pair(uint64_t a, uint64_t b, uint64_t c) {
-  uint64_t d;
-  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
-  return d;
-}
-__device__ __forceinline__ uint64_t add_pair(uint64_t a, uint64_t b) {
-  uint64_t d;
-  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
-  return d;
 }
 
 template <int D>
@@ -165,34 +150,37 @@ kv8_attn_prefill_kernel(const __grid_constant__ CUtensorMap k_map, const uint8_t
   const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u;
   uint8_t* base_ptr = smem_raw + (base - smem_u32(smem_raw));
   const uint32_t bars = base + Cfg::kBars;
-  const uint32_t bar_kfull = bars, bar_kempty = bars + 16;        // [2 stages] each
-  const uint32_t bar_rawfull = bars + 32, bar_rawempty = bars + 48;
-  const uint32_t bar_vfull = bars + 64, bar_vempty = bars + 80;
-  const uint32_t bar_q = bars + 96;                               // Q written
-  const uint32_t bar_sempty = bars + 104;                         // S read
-  const uint32_t bar_sfull = bars + 112;                          // [2 tiles] S written, for this tile
-  const uint32_t bar_odone = bars + 128;                          // [2 tiles] O += P V finished
-  const uint32_t bar_pfull = bars + 144;                          // [2 tiles][2 halves of 64 keys] P written, O rescaled
-  uint32_t* tmem_base_sm = reinterpret_cast<uint32_t*>(base_ptr + Cfg::kBars + 192);
+  const uint32_t bar_kfull = bars, bar_kempty = bars + 32;        // [3 stages] each
+  const uint32_t bar_rawfull = bars + 64, bar_rawempty = bars + 80;  // [2 stages] each
+  const uint32_t bar_vfull = bars + 96, bar_vempty = bars + 112;
+  const uint32_t bar_q = bars + 128;                              // Q written
+  const uint32_t bar_sempty = bars + 136;                         // S read
+  const uint32_t bar_sfull = bars + 144;                          // [2 tiles] S written, for this tile
+  const uint32_t bar_odone = bars + 160;                          // [2 tiles] O += P V finished
+  const uint32_t bar_pfull = bars + 176;                          // [2 tiles][2 halves of 64 keys] P written, O rescaled
+  uint32_t* tmem_base_sm = reinterpret_cast<uint32_t*>(base_ptr + Cfg::kBars + 240);
   float* row_scale = reinterpret_cast<float*>(base_ptr + Cfg::kRowScale);
   float* sums = reinterpret_cast<float*>(base_ptr + Cfg::kSums);
+  float* refs = reinterpret_cast<float*>(base_ptr + Cfg::kRefs);
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   if (threadIdx.x == 32) tma_prefetch_desc(&k_map);
   if (threadIdx.x == 0) {
     for (int s = 0; s < 2; ++s) {
-      mbar_init(bar_kfull + 8 * s, 1);
-      mbar_init(bar_kempty + 8 * s, 1);
       mbar_init(bar_rawfull + 8 * s, 1);
-      mbar_init(bar_rawempty + 8 * s, 2);
-      mbar_init(bar_vfull + 8 * s, 2);
+      mbar_init(bar_rawempty + 8 * s, 4);
+      mbar_init(bar_vfull + 8 * s, 4);
       mbar_init(bar_vempty + 8 * s, 1);
       mbar_init(bar_sfull + 8 * s, 1);
       mbar_init(bar_odone + 8 * s, 1);
       mbar_init(bar_pfull + 16 * s, 4);
       mbar_init(bar_pfull + 16 * s + 8, 4);
     }
-    mbar_init(bar_q, 8);
+    for (int s = 0; s < kKv8KStages; ++s) {
+      mbar_init(bar_kfull + 8 * s, 1);
+      mbar_init(bar_kempty + 8 * s, 1);
+    }
+    mbar_init(bar_q, kKv8SoftmaxWarps);
     mbar_init(bar_sempty, 4);
     fence_mbar_init();
     fence_proxy_async();
@@ -210,95 +198,90 @@ kv8_attn_prefill_kernel(const __grid_constant__ CUtensorMap k_map, const uint8_t
   const int t0 = ((num_tokens + QT - 1) / QT - own - cta - min(cta, pairs)) * QT;
   const int t_end = min(t0 + own * QT, num_tokens);
   const int last_pos = first_pos + t_end - 1;
-  // key tiles of this CTA: kt0 ..; each tile of rows takes the first n_of[] of them
+  // key tiles of this CTA: kt0 ..; a tile of rows takes the first n_of[] of them, or, alone, accumulator 0 the even and 1 the odd ones
   const int kt0 = split * split_tiles;
   const int n_tiles = max(0, min(last_pos / kTcKeys + 1, kt0 + split_tiles) - kt0);
-  int n_of[2];
-#pragma unroll
-  for (int t = 0; t < 2; ++t) {
-    const int first = t0 + t * QT;
-    n_of[t] = first < t_end ? max(0, min(n_tiles, (first_pos + min(first + QT, t_end) - 1) / kTcKeys + 1 - kt0)) : 0;
+  int n_of[2] = {(n_tiles + 1) / 2, n_tiles / 2};
+  if (own == 2) {
+    n_of[0] = max(0, min(n_tiles, (first_pos + t0 + QT - 1) / kTcKeys + 1 - kt0));
+    n_of[1] = n_tiles;
   }
+  const int stride = own == 2 ? 1 : 2;  // key tiles from one of an accumulator to its next
   const int last_page = last_pos / kKvPage;
 
   grid_dep_wait();  // set-up done; Q and this chunk's pages come from the kernels before
   grid_dep_launch();
 
   if (warp < 4) {
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
-    if (warp == 0 || warp == 3) {
-      // ------------------------------------------------- pages, V in f16 ------
-      // Warp 0 issues the copies of a key tile - lane i of the first 8 page i of its keys, of the second 8 that of its values - and then
-      // takes rows 64.. of the values of the tile before; warp 3 takes rows 0..63.
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 40;");
+    if (warp == 0) {
+      // ------------------------------------------------- pages ------
+      // Lane i of the first 8 owns page i of a tile's keys, of the second 8 that of its values.
       const int pg = lane & 7;
       bool alive = true;
+      int next = __ldg(table_row + min(kt0 * kTcPages + pg, last_page)), ks = 0, kphase = 1;
 #pragma unroll 1
-      for (int j = 0; j < n_tiles + 1; ++j) {
-        if (warp == 0 && j < n_tiles) {
-          const int st = j & 1;
-          // the last page stands in for those behind it, so that every stage is the same number of bytes
-          int page = __ldg(table_row + min((kt0 + j) * kTcPages + pg, last_page));
-          if (page < 0 || page >= num_blocks) {
-            set_error(err, kErrDevBadBlockId);
-            page = 0;
-          }
-          const size_t cell = static_cast<size_t>(page) * num_kv_heads + h;
-          if (alive) alive = mbar_wait(bar_kempty + 8 * st, ((j >> 1) & 1) ^ 1, err);
-          if (!__all_sync(0xffffffffu, alive)) break;
-          if (lane == 0) mbar_arrive_expect_tx(bar_kfull + 8 * st, Cfg::kTile8);
-          __syncwarp();
-          if (lane < kTcPages)
-            tma_load_2d(base + Cfg::kK + st * Cfg::kTile8 + pg * kPageBytes8, &k_map, bar_kfull + 8 * st, 0, static_cast<int>(cell) * kKvPage);
-          if (alive) alive = mbar_wait(bar_rawempty + 8 * st, ((j >> 1) & 1) ^ 1, err);
-          if (!__all_sync(0xffffffffu, alive)) break;
-          if (lane == 0) mbar_arrive_expect_tx(bar_rawfull + 8 * st, Cfg::kTile8);
-          __syncwarp();
-          if (lane >= 8 && lane < 16)
-            bulk_load(base + Cfg::kRaw + st * Cfg::kTile8 + pg * kPageBytes8, v_pool + cell * kPageBytes8, kPageBytes8, bar_rawfull + 8 * st);
+      for (int j = 0; j < n_tiles && alive; ++j) {
+        // the last page stands in for those behind it, so that every stage is the same number of bytes
+        int page = next;
+        next = __ldg(table_row + min((kt0 + j + 1) * kTcPages + pg, last_page));
+        if (page < 0 || page >= num_blocks) {
+          set_error(err, kErrDevBadBlockId);
+          page = 0;
         }
-        const int jv = warp == 0 ? j - 1 : j;
-        if (jv >= 0 && jv < n_tiles) {
-          const int st = jv & 1;
-          if (alive) alive = mbar_wait(bar_rawfull + 8 * st, (jv >> 1) & 1, err);
-          if (alive) alive = mbar_wait(bar_vempty + 8 * st, ((jv >> 1) & 1) ^ 1, err);
-          if (!__all_sync(0xffffffffu, alive)) break;
-          values_to_f16<D>(base + Cfg::kRaw + st * Cfg::kTile8, base + Cfg::kV + st * Cfg::kTile16, warp == 0 ? kTcKeys / 2 : 0,
-                           last_pos - (kt0 + jv) * kTcKeys + 1, lane);
-          if (lane == 0) {
-            mbar_arrive(bar_vfull + 8 * st);
-            mbar_arrive(bar_rawempty + 8 * st);
-          }
+        const size_t cell = static_cast<size_t>(page) * num_kv_heads + h;
+        alive = mbar_wait_warp(bar_kempty + 8 * ks, kphase, err);
+        if (!alive) break;
+        if (lane == 0) mbar_arrive_expect_tx(bar_kfull + 8 * ks, Cfg::kTile8);
+        __syncwarp();
+        if (lane < kTcPages)
+          tma_load_2d(base + Cfg::kK + ks * Cfg::kTile8 + pg * kPageBytes8, &k_map, bar_kfull + 8 * ks, 0, static_cast<int>(cell) * kKvPage);
+        if (++ks == kKv8KStages) {
+          ks = 0;
+          kphase ^= 1;
         }
+        const int st = j & 1;
+        alive = mbar_wait_warp(bar_rawempty + 8 * st, ((j >> 1) & 1) ^ 1, err);
+        if (!alive) break;
+        if (lane == 0) mbar_arrive_expect_tx(bar_rawfull + 8 * st, Cfg::kTile8);
+        __syncwarp();
+        if (lane >= 8 && lane < 16)
+          bulk_load(base + Cfg::kRaw + st * Cfg::kTile8 + pg * kPageBytes8, v_pool + cell * kPageBytes8, kPageBytes8, bar_rawfull + 8 * st);
       }
     } else if (warp == 1) {
       // ------------------------------------------------- S = Q K^T ------
       if (elect_one()) {
         constexpr uint32_t idesc_s = umma_idesc_f8(kTcRows, kTcKeys);
         bool alive = mbar_wait(bar_q, 0, err);
-        uint32_t n = 0;
+        uint32_t n = 0, st = 0, phase = 0;
 #pragma unroll 1
         for (int j = 0; j < n_tiles && alive; ++j) {
-          const int st = j & 1;
-          alive = mbar_wait(bar_kfull + 8 * st, (j >> 1) & 1, err);
+          alive = mbar_wait(bar_kfull + 8 * st, phase, err);
           const uint64_t b0 = desc_k8<D>(base + Cfg::kK + st * Cfg::kTile8);
 #pragma unroll 1
           for (int t = 0; t < 2; ++t) {
-            if (j >= (t ? n_of[1] : n_of[0])) continue;  // none of this tile's rows sees these keys
+            // none of this tile's rows sees these keys, or they are the other accumulator's
+            if (own == 2 ? j >= (t ? n_of[1] : n_of[0]) : (j & 1) != t) continue;
             if (alive) alive = mbar_wait(bar_sempty, (n & 1) ^ 1, err);
             if (!alive) break;
             ++n;
             tc_fence_after();
-            uint64_t a = desc_k8<D>(base + Cfg::kQ + 2 * t * Cfg::kTile8);
-#pragma unroll 1
-            for (int part = 0; part < 2; ++part, a += Cfg::kTile8 >> 4)
-#pragma unroll 1
-              for (int k = 0; k < D / 32; ++k) tc_mma_f8(tmem_s, a + 2 * k, b0 + 2 * k, idesc_s, part + k > 0 ? 1u : 0u);
+            const uint64_t a0 = desc_k8<D>(base + Cfg::kQ + 2 * (own == 2 ? t : 0) * Cfg::kTile8);
+#pragma unroll
+            for (int k = 0; k < D / 16; ++k) {  // hi, then lo
+              constexpr int kSteps = D / 32;
+              tc_mma_f8(tmem_s, a0 + (k / kSteps * (Cfg::kTile8 >> 4) + k % kSteps * 2), b0 + k % kSteps * 2, idesc_s, k > 0 ? 1u : 0u);
+            }
             tc_commit(bar_sfull + 8 * t);
           }
           tc_commit(bar_kempty + 8 * st);
+          if (++st == kKv8KStages) {
+            st = 0;
+            phase ^= 1;
+          }
         }
       }
-    } else if (elect_one()) {
+    } else if (warp == 2 && elect_one()) {
       // ------------------------------------------------- O += P V ------
       constexpr uint32_t idesc_o = idesc_f16_mn(kTcRows, D);
       bool alive = true;
@@ -308,49 +291,74 @@ kv8_attn_prefill_kernel(const __grid_constant__ CUtensorMap k_map, const uint8_t
         alive = mbar_wait(bar_vfull + 8 * st, (j >> 1) & 1, err);
 #pragma unroll 1
         for (int t = 0; t < 2; ++t) {
-          if (j >= (t ? n_of[1] : n_of[0])) continue;
-#pragma unroll 1
-          for (int kk = 0; kk < kTcPages; ++kk) {  // 16 keys each
-            if ((kk & 3) == 0) {
-              if (alive) alive = mbar_wait(bar_pfull + 16 * t + 2 * kk, j & 1, err);
-              if (!alive) break;
-              tc_fence_after();
-            }
-            const uint64_t b = umma_desc_mn128(base + Cfg::kV + st * Cfg::kTile16 + kk * kPageBytes16, 1024, kAtomGroup);
-            mma_f16_ts(tmem_o + t * kTcKeys, tmem_p + t * 64 + kk * 8, b, idesc_o, (j > 0 || kk > 0) ? 1u : 0u);
+          if (own == 2 ? j >= (t ? n_of[1] : n_of[0]) : (j & 1) != t) continue;
+          const int i = own == 2 ? j : j >> 1;
+          const uint64_t b0 = umma_desc_mn128(base + Cfg::kV + st * Cfg::kTile16, 1024, kAtomGroup);
+#pragma unroll
+          for (int half = 0; half < 2; ++half) {
+            if (alive) alive = mbar_wait(bar_pfull + 16 * t + 8 * half, i & 1, err);
+            if (!alive) break;
+            tc_fence_after();
+#pragma unroll
+            for (int kk = half * 4; kk < half * 4 + 4; ++kk)  // 16 keys each
+              mma_f16_ts(tmem_o + t * kTcKeys, tmem_p + t * 64 + kk * 8, b0 + kk * (kPageBytes16 >> 4), idesc_o, (i > 0 || kk > 0) ? 1u : 0u);
           }
           tc_commit(bar_odone + 8 * t);
         }
         tc_commit(bar_vempty + 8 * st);
       }
     }
+  } else if (warp < 8) {
+    // ------------------------------------------------- V in f16 ------
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 40;");
+    bool alive = true;
+#pragma unroll 1
+    for (int j = 0; j < n_tiles && alive; ++j) {
+      const int st = j & 1;
+      alive = mbar_wait_warp(bar_rawfull + 8 * st, (j >> 1) & 1, err) && mbar_wait_warp(bar_vempty + 8 * st, ((j >> 1) & 1) ^ 1, err);
+      if (!alive) break;
+      values_to_f16<D>(base + Cfg::kRaw + st * Cfg::kTile8, base + Cfg::kV + st * Cfg::kTile16, (warp - 4) * (kTcKeys / 4),
+                       last_pos - (kt0 + j) * kTcKeys + 1, lane);
+      if (lane == 0) {
+        mbar_arrive(bar_vfull + 8 * st);
+        mbar_arrive(bar_rawempty + 8 * st);
+      }
+    }
   } else {
     // -------------------------------------------------------- softmax ------
-    asm volatile("setmaxnreg.inc.sync.aligned.u32 224;");
-    const int t = (warp >> 2) - 1;           // tile of rows
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 216;");
+    const int t = (warp - 8) >> 2;           // tile of rows, or accumulator
     const int quarter = warp & 3;            // TMEM lanes this warp may touch
     const int r = quarter * 32 + lane;       // score row
     const uint32_t lane_off = static_cast<uint32_t>(quarter * 32) << 16;
     const uint32_t s_acc = tmem_s + lane_off, o_acc = tmem_o + t * kTcKeys + lane_off, p_tm = tmem_p + t * 64 + lane_off;
     const uint32_t sfull = bar_sfull + 8 * t, odone = bar_odone + 8 * t, pfull = bar_pfull + 16 * t;
-    const int tt0 = t0 + t * QT, rt = r / gr, n_own = t ? n_of[1] : n_of[0];
+    const int tile = own == 2 ? t : 0, tt0 = t0 + tile * QT, rt = r / gr, n_own = t ? n_of[1] : n_of[0];
     const int pos = first_pos + min(tt0 + rt, min(tt0 + QT, num_tokens) - 1);  // the last key this row may see
+    const int first_tile = kt0 + (own == 2 ? 0 : t);
 
     // Scales of the pages of a key tile: lane i of 8 asks for those of page i.
     const int pg = lane & 7;
-    auto page_id = [&](int j) {
-      const int id = j < n_own ? __ldg(table_row + min((kt0 + j) * kTcPages + pg, last_page)) : 0;
-      return id < 0 || id >= num_blocks ? 0 : id;  // the producer reports it
+    // (Loads that stay where they are written: left to itself the compiler moves them down to where they are needed.)
+    auto page_id = [&](int i) {
+      int id;
+      asm volatile("ld.global.nc.b32 %0, [%1];" : "=r"(id) : "l"(table_row + min((first_tile + i * stride) * kTcPages + pg, last_page)));
+      return id;
     };
-    int id = page_id(0);
-    int kb = k_scale[static_cast<size_t>(id) * num_kv_heads + h], vb = v_scale[static_cast<size_t>(id) * num_kv_heads + h];
+    int id = page_id(0), kb, vb;
+    auto ask_scales = [&]() {
+      const size_t cell = static_cast<size_t>(id < 0 || id >= num_blocks ? 0 : id) * num_kv_heads + h;  // the producer reports it
+      asm volatile("ld.global.nc.u8 %0, [%1];" : "=r"(kb) : "l"(k_scale + cell));
+      asm volatile("ld.global.nc.u8 %0, [%1];" : "=r"(vb) : "l"(v_scale + cell));
+    };
+    ask_scales();
     id = page_id(1);
 
-    // Q tiles: neighbouring threads neighbouring pieces of 8 numbers of a row, 16 to 32 rows at a time and four such steps on their way.  One
+    // Q tiles: neighbouring threads neighbouring pieces of 8 numbers of a row, 16 or 32 rows at a time and four such steps on their way.  One
     // loop over all steps of both tiles: code that runs once has to be fetched first, and unrolled it was 16 KB.
     {
       constexpr int kSteps = D / 16;  // of a tile
-      const int ch = threadIdx.x % (D / 8), qr0 = (threadIdx.x - 128) / (D / 8);
+      const int ch = threadIdx.x % (D / 8), qr0 = (threadIdx.x - 256) / (D / 8);
       auto load = [&](int step) {
         const int qr = step % kSteps * (2048 / D) + qr0, qt_l = qr / gr, tok = t0 + step / kSteps * QT + qt_l;
         uint4 x = make_uint4(0u, 0u, 0u, 0u);
@@ -402,25 +410,14 @@ kv8_attn_prefill_kernel(const __grid_constant__ CUtensorMap k_map, const uint8_t
     fence_proxy_async();  // the tensor core reads Q through the async proxy
     asm volatile("bar.sync 1, 256;" ::: "memory");
     if (lane == 0) mbar_arrive(bar_q);
-    const float f_q = own > t ? row_scale[t * kTcRows + r] : 1.f;
-    float4* scales = reinterpret_cast<float4*>(base_ptr + Cfg::kScales) + (warp - 4) * 16;
+    const float f_q = row_scale[tile * kTcRows + r];
+    float4* scales = reinterpret_cast<float4*>(base_ptr + Cfg::kScales) + (warp - 8) * 16;
 
     float m_run = -INFINITY, l_run = 0.f;
     bool alive = true, s_ready = false;
-    int kbase = kt0 * kTcKeys;
+    int kbase = first_tile * kTcKeys;
 #pragma unroll 1
-    for (int i = 0; i < n_own; ++i, kbase += kTcKeys) {
-      {
-        const int ev = scale_exponent(vb);
-        if (lane < 8) scales[(i & 1) * 8 + pg] = make_float4(power_of_two(scale_exponent(kb)), static_cast<float>(ev), power_of_two(-ev), 0.f);
-        __syncwarp();
-        if (i + 1 < n_own) {
-          kb = k_scale[static_cast<size_t>(id) * num_kv_heads + h];
-          vb = v_scale[static_cast<size_t>(id) * num_kv_heads + h];
-          id = page_id(i + 2);
-        }
-      }
-      const float4* sc = scales + (i & 1) * 8;
+    for (int i = 0; i < n_own; ++i, kbase += stride * kTcKeys) {
       if (!__all_sync(0xffffffffu, s_ready) && alive) alive = mbar_wait(sfull, i & 1, err);
       tc_fence_after();
       float s[128];
@@ -428,8 +425,24 @@ kv8_attn_prefill_kernel(const __grid_constant__ CUtensorMap k_map, const uint8_t
         uint32_t (&raw)[4][32] = *reinterpret_cast<uint32_t(*)[4][32]>(s);
 #pragma unroll
         for (int c = 0; c < 4; ++c) tmem_ld32(s_acc + c * 32, raw[c]);
-        tmem_ld_wait();
       }
+      // while S is on its way: the pages' scales, and the next key tile's are asked for
+      const float4* sc = scales + (i & 1) * 8;
+      float f[8], lv[8];
+      {
+        const int ev = scale_exponent(vb);
+        if (lane < 8) scales[(i & 1) * 8 + pg] = make_float4(power_of_two(scale_exponent(kb)), static_cast<float>(ev), power_of_two(-ev), 0.f);
+        __syncwarp();
+        ask_scales();  // of the next key tile; past the last one those of the last page
+        id = page_id(i + 2);
+#pragma unroll
+        for (int p = 0; p < 8; ++p) {
+          const float2 w = *reinterpret_cast<const float2*>(sc + p);
+          f[p] = f_q * w.x;
+          lv[p] = w.y;
+        }
+      }
+      tmem_ld_wait();
       tc_fence_before();
       __syncwarp();
       if (lane == 0) mbar_arrive(bar_sempty);  // S is the other tile's now
@@ -445,7 +458,7 @@ kv8_attn_prefill_kernel(const __grid_constant__ CUtensorMap k_map, const uint8_t
         const float* x = s + 16 * p;
         const float a = max_of_3(max_of_3(x[0], x[1], x[2]), x[3], x[4]), b = max_of_3(max_of_3(x[5], x[6], x[7]), x[8], x[9]);
         const float c = max_of_3(max_of_3(x[10], x[11], x[12]), x[13], x[14]);
-        m_new = fmaxf(m_new, fmaf(max_of_3(max_of_3(a, b, c), x[15], x[15]), f_q * sc[p].x, sc[p].y));
+        m_new = fmaxf(m_new, fmaf(max_of_3(max_of_3(a, b, c), x[15], x[15]), f[p], lv[p]));
       }
       const bool need = m_new - m_run > kTcRescaleLog2;  // true on the first tile (m_run = -inf)
       if (__any_sync(0xffffffffu, need)) {
@@ -475,27 +488,21 @@ kv8_attn_prefill_kernel(const __grid_constant__ CUtensorMap k_map, const uint8_t
         uint32_t pk[32];
 #pragma unroll
         for (int p = 0; p < 4; ++p) {
-          const float4 w = sc[half * 4 + p];
-          const uint64_t f = pair_of(f_q * w.x, f_q * w.x), off = pair_of(w.y - mb, w.y - mb);
-          uint64_t sum[2];
+          const float factor = f[half * 4 + p], off = lv[half * 4 + p] - mb;
+          float sum[2];
 #pragma unroll
           for (int ch = 0; ch < 2; ++ch) {
             // asked here, needed behind this half: P was last read by the product of the tile before; the next S
             if (p == 2 && ch == 1 && half == 0 && i > 0) p_free = mbar_test(odone, (i - 1) & 1);
             if (p == 2 && ch == 1 && half == 1) s_ready = mbar_test(sfull, (i + 1) & 1);
-            const float* x = s + half * 64 + p * 16 + ch * 8;
-            uint64_t e[4];
+            float e[8];
 #pragma unroll
-            for (int k = 0; k < 4; ++k) {
-              const float2 t2 = halves(fma_pair(pair_of(x[2 * k], x[2 * k + 1]), f, off));
-              const float lo = fast_exp2(t2.x), hi = fast_exp2(t2.y);
-              pk[p * 8 + ch * 4 + k] = pack_f16x2(lo, hi);
-              e[k] = pair_of(lo, hi);
-            }
-            sum[ch] = add_pair(add_pair(e[0], e[1]), add_pair(e[2], e[3]));
+            for (int k = 0; k < 8; ++k) e[k] = fast_exp2(fmaf(s[half * 64 + p * 16 + ch * 8 + k], factor, off));
+            sum[ch] = ((e[0] + e[1]) + (e[2] + e[3])) + ((e[4] + e[5]) + (e[6] + e[7]));
+#pragma unroll
+            for (int k = 0; k < 4; ++k) pk[p * 8 + ch * 4 + k] = pack_f16x2(e[2 * k], e[2 * k + 1]);
           }
-          const float2 both = halves(add_pair(sum[0], sum[1]));
-          l_run = fmaf(both.x + both.y, w.z, l_run);
+          l_run = fmaf(sum[0] + sum[1], sc[half * 4 + p].z, l_run);
         }
         if (half == 0 && !__all_sync(0xffffffffu, p_free) && alive) alive = mbar_wait(odone, (i - 1) & 1, err);
         tc_fence_after();
@@ -506,41 +513,62 @@ kv8_attn_prefill_kernel(const __grid_constant__ CUtensorMap k_map, const uint8_t
         if (lane == 0) mbar_arrive(pfull + 8 * half);
       }
     }
-    // ---- epilogue, once the product of the last key tile has finished.  The warps of a CTA with one tile share its columns.
-    const int e = own == 2 ? t : 0, cols = own == 2 ? D : D / 2, col0 = own == 2 ? 0 : t * (D / 2), n_e = e ? n_of[1] : n_of[0];
-    const int tok = t0 + e * QT + rt;
+    // ---- epilogue, once the products of the last key tiles have finished.  The warps of a CTA with one tile take half of the columns each, for
+    // the sum of both accumulators.
+    sums[t * kTcRows + r] = l_run;
+    refs[t * kTcRows + r] = m_run;
+    asm volatile("bar.sync 1, 256;" ::: "memory");
+    const int tok = tt0 + rt;
     const bool real = rt < QT && tok < t_end;
     const size_t oidx = static_cast<size_t>(tok) * num_q_heads + h * gr + (r - rt * gr);
-    float l = l_run;
-    if (splits > 1 && real && e == t) part_ml[oidx * splits + split] = make_float2(m_run, l);
+    const bool second = own == 1 && n_of[1] > 0;  // there is an accumulator 1 to be added
+    float l = l_run, w0 = 1.f, w1 = 0.f;
     if (own == 1) {
-      if (t == 0) sums[r] = l;
-      asm volatile("bar.sync 1, 256;" ::: "memory");
-      l = sums[r];
+      const float m0 = refs[r], m1 = refs[kTcRows + r];
+      m_run = fmaxf(m0, m1);
+      const float ref = m_run == -INFINITY ? 0.f : m_run;
+      w0 = fast_exp2(m0 - ref);
+      w1 = fast_exp2(m1 - ref);
+      l = w0 * sums[r] + w1 * sums[kTcRows + r];
     }
+    if (splits > 1 && real && (own == 2 || t == 0)) part_ml[oidx * splits + split] = make_float2(m_run, l);
+    const int n_e = own == 2 ? n_own : n_of[0];
     if (n_e > 0) {
-      if (alive) alive = mbar_wait(bar_odone + 8 * e, (n_e - 1) & 1, err);
+      const uint32_t acc = own == 2 ? o_acc : tmem_o + lane_off;
+      const int cols = own == 2 ? D : D / 2, col0 = own == 2 ? 0 : t * (D / 2);
+      if (alive) alive = mbar_wait(own == 2 ? odone : bar_odone, (n_e - 1) & 1, err);
+      if (second && alive) alive = mbar_wait(bar_odone + 8, (n_of[1] - 1) & 1, err);
       tc_fence_after();
-      const float inv = 1.f / l;
+      const float inv = splits > 1 ? 1.f : 1.f / l, none = 0.f * l;  // none: 0, or NaN where the row's sum is
 #pragma unroll 1
-      for (int c0 = 0; c0 < cols; c0 += 32) {
+      for (int c0 = col0; c0 < col0 + cols; c0 += 32) {
         uint32_t o[32];
-        tmem_ld32(tmem_o + e * kTcKeys + lane_off + col0 + c0, o);
+        tmem_ld32(acc + c0, o);
         tmem_ld_wait();
+        // the weight of an accumulator that holds nothing is 0, but what it holds may not be a number
+#pragma unroll
+        for (int c = 0; c < 32; ++c) o[c] = __float_as_uint(w0 == 0.f ? none : __uint_as_float(o[c]) * (w0 * inv));
+        if (second) {
+          uint32_t o1[32];
+          tmem_ld32(acc + kTcKeys + c0, o1);
+          tmem_ld_wait();
+#pragma unroll
+          for (int c = 0; c < 32; ++c)
+            if (w1 != 0.f) o[c] = __float_as_uint(fmaf(__uint_as_float(o1[c]), w1 * inv, __uint_as_float(o[c])));
+        }
         if (real && alive) {
           if (splits > 1) {
-            float4* to = reinterpret_cast<float4*>(part_o + (oidx * splits + split) * D + col0 + c0);
+            uint4* to = reinterpret_cast<uint4*>(part_o + (oidx * splits + split) * D + c0);
 #pragma unroll
-            for (int c = 0; c < 8; ++c)
-              to[c] = make_float4(__uint_as_float(o[4 * c]), __uint_as_float(o[4 * c + 1]), __uint_as_float(o[4 * c + 2]), __uint_as_float(o[4 * c + 3]));
+            for (int c = 0; c < 8; ++c) to[c] = make_uint4(o[4 * c], o[4 * c + 1], o[4 * c + 2], o[4 * c + 3]);
           } else {
-            uint4* to = reinterpret_cast<uint4*>(out + oidx * D + col0 + c0);
+            uint4* to = reinterpret_cast<uint4*>(out + oidx * D + c0);
 #pragma unroll
             for (int c = 0; c < 4; ++c) {
-              uint32_t w[4];
+              uint32_t x[4];
 #pragma unroll
-              for (int k = 0; k < 4; ++k) w[k] = pack_bf16x2(__uint_as_float(o[8 * c + 2 * k]) * inv, __uint_as_float(o[8 * c + 2 * k + 1]) * inv);
-              to[c] = make_uint4(w[0], w[1], w[2], w[3]);
+              for (int k = 0; k < 4; ++k) x[k] = pack_bf16x2(__uint_as_float(o[8 * c + 2 * k]), __uint_as_float(o[8 * c + 2 * k + 1]));
+              to[c] = make_uint4(x[0], x[1], x[2], x[3]);
             }
           }
         }
