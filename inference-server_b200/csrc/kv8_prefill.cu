@@ -354,56 +354,63 @@ kv8_attn_prefill_kernel(const __grid_constant__ CUtensorMap k_map, const uint8_t
     ask_scales();
     id = page_id(1);
 
-    // Q tiles: neighbouring threads neighbouring pieces of 8 numbers of a row, 16 or 32 rows at a time and four such steps on their way.  One
-    // loop over all steps of both tiles: code that runs once has to be fetched first, and unrolled it was 16 KB.
+    // Q tiles: 32 numbers of a row per thread and step, the next step's on their way.  (8 numbers, with three times the shuffles and a
+    // quarter of the work side by side, took 5200 cycles a tile.)  One loop over the steps of both tiles: code that runs once has to be
+    // fetched first.
     {
-      constexpr int kSteps = D / 16;  // of a tile
-      const int ch = threadIdx.x % (D / 8), qr0 = (threadIdx.x - 256) / (D / 8);
+      constexpr int kOfRow = D / 32, kRows = 256 / kOfRow, kSteps = kTcRows / kRows;  // threads of a row; rows of a step; steps of a tile
+      const int ch = threadIdx.x % kOfRow, qr0 = (threadIdx.x - 256) / kOfRow;
+      uint4 v[4];
       auto load = [&](int step) {
-        const int qr = step % kSteps * (2048 / D) + qr0, qt_l = qr / gr, tok = t0 + step / kSteps * QT + qt_l;
-        uint4 x = make_uint4(0u, 0u, 0u, 0u);
-        if (step < own * kSteps && qt_l < QT && tok < num_tokens)
-          x = *reinterpret_cast<const uint4*>(q + (static_cast<size_t>(tok) * num_q_heads + h * gr + (qr - qt_l * gr)) * D + ch * 8);
-        return x;
+        const int qr = step % kSteps * kRows + qr0, qt_l = qr / gr, tok = t0 + step / kSteps * QT + qt_l;
+        const bool there = step < own * kSteps && qt_l < QT && tok < num_tokens;
+        const uint4* from = reinterpret_cast<const uint4*>(q + (static_cast<size_t>(tok) * num_q_heads + h * gr + (qr - qt_l * gr)) * D + ch * 32);
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          v[k] = make_uint4(0u, 0u, 0u, 0u);
+          if (there) v[k] = from[k];
+        }
       };
-      uint4 v[4] = {load(0), load(1), load(2), load(3)};
+      load(0);
 #pragma unroll 1
       for (int step = 0; step < own * kSteps; ++step) {
-        const uint32_t x[4] = {v[0].x, v[0].y, v[0].z, v[0].w};
-        v[0] = v[1];
-        v[1] = v[2];
-        v[2] = v[3];
-        v[3] = load(step + 4);
-        const int u = step / kSteps, qr = step % kSteps * (2048 / D) + qr0;
+        const int u = step / kSteps, qr = step % kSteps * kRows + qr0;
+        uint32_t x[16];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) x[4 * k] = v[k].x, x[4 * k + 1] = v[k].y, x[4 * k + 2] = v[k].z, x[4 * k + 3] = v[k].w;
+        load(step + 1);
         uint32_t top = 0;
 #pragma unroll
-        for (int w = 0; w < 4; ++w) top = max(top, max((x[w] & 0x7fff0000u), (x[w] & 0x7fffu) << 16));
+        for (int k = 0; k < 16; ++k) top = __vmaxu2(top, x[k] & 0x7fff7fffu);
+        top = max(top >> 16, top & 0xffffu) << 16;
 #pragma unroll
-        for (int o = 1; o < D / 8; o <<= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
+        for (int o = 1; o < kOfRow; o <<= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
         // the exponent that brings the row's top to (224, 448]; tiny rows may stay below, a row with an infinity is all NaN
         const int e = max(static_cast<int>(top >> 23) - 127 - 8 + ((top & 0x7fffffu) > 0x600000u ? 1 : 0), -100);
         const float by = top < 0x7f800000u ? power_of_two(-e) : NAN;
-        uint32_t hi[2], lo[2];
+        uint32_t hi[8], lo[8];
 #pragma unroll
-        for (int w = 0; w < 2; ++w) {
+        for (int k = 0; k < 8; ++k) {
           uint32_t pair[2], rest_of[2];
 #pragma unroll
           for (int p = 0; p < 2; ++p) {
-            const float a = __uint_as_float(x[2 * w + p] << 16) * by, b = __uint_as_float(x[2 * w + p] & 0xffff0000u) * by;
+            const float a = __uint_as_float(x[2 * k + p] << 16) * by, b = __uint_as_float(x[2 * k + p] & 0xffff0000u) * by;
             pair[p] = to_e4m3x2(a, b);
             uint32_t near, unused;
             e4m3x4_to_f16(pair[p], near, unused);
             const float2 n2 = __half22float2(*reinterpret_cast<const __half2*>(&near));
             rest_of[p] = to_e4m3x2(a - n2.x, b - n2.y);
           }
-          hi[w] = pair[0] | pair[1] << 16;
-          lo[w] = rest_of[0] | rest_of[1] << 16;
+          hi[k] = pair[0] | pair[1] << 16;
+          lo[k] = rest_of[0] | rest_of[1] << 16;
         }
-        uint32_t at;
-        if constexpr (D == 128) at = (qr >> 3) * 1024 + swz128(qr & 7, ch >> 1) + (ch & 1) * 8;
-        else at = qr * 64 + (((ch >> 1) ^ ((qr >> 1) & 3)) << 4) + (ch & 1) * 8;
-        *reinterpret_cast<uint2*>(base_ptr + Cfg::kQ + 2 * u * Cfg::kTile8 + at) = make_uint2(hi[0], hi[1]);
-        *reinterpret_cast<uint2*>(base_ptr + Cfg::kQ + (2 * u + 1) * Cfg::kTile8 + at) = make_uint2(lo[0], lo[1]);
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+          const uint32_t at = D == 128 ? (qr >> 3) * 1024 + swz128(qr & 7, 2 * ch + k) : qr * 64 + (((2 * ch + k) ^ ((qr >> 1) & 3)) << 4);
+          uint8_t* to = base_ptr + Cfg::kQ + 2 * u * Cfg::kTile8 + at;
+          *reinterpret_cast<uint4*>(to) = make_uint4(hi[4 * k], hi[4 * k + 1], hi[4 * k + 2], hi[4 * k + 3]);
+          *reinterpret_cast<uint4*>(to + Cfg::kTile8) = make_uint4(lo[4 * k], lo[4 * k + 1], lo[4 * k + 2], lo[4 * k + 3]);
+        }
         if (ch == 0) row_scale[u * kTcRows + qr] = fmaxf(scale_log2 * power_of_two(min(e, 120)), 0x1p-90f);
       }
     }
