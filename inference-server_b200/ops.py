@@ -206,29 +206,25 @@ class KvSlotMap(NamedTuple):
     supply_used: torch.Tensor
 
 
-_device_index = torch.Tensor.get_device
+_native = None
 
 
-def _stream_of(*operands: torch.Tensor) -> int:
-    """The current stream of the device that all operands are on.  The kernels run on the current device: operands of another are an error
-    and not a fault."""
-    devices = set(map(_device_index, operands))
-    here = devices.pop()
-    if here < 0 or devices:
-        for t in operands:
-            if not t.is_cuda:
-                raise ValueError("operands must be CUDA tensors (this path has no CPU implementation)")
-        raise ValueError(f"operands are on {sorted({str(t.device) for t in operands})}")
-    if here != torch.cuda.current_device():
-        raise ValueError(f"operands are on cuda:{here}, the current device is cuda:{torch.cuda.current_device()}")
-    return torch.cuda.current_stream().cuda_stream if _raw_stream is None else _raw_stream(here)
-
-
-def _status_word(status: torch.Tensor | None) -> None:
-    if status is not None:
-        _need(status, "status")
-        if status.numel() * status.element_size() < 4:
-            raise ValueError("status holds less than a 4-byte word")
+def _load_native():
+    """The native binding of this section's operators (csrc/kv8_bind.cpp), tied to the loaded library.  It checks the operands - types, shapes,
+    strides, all on the current device - and raises ValueError, makes the outputs and calls the C ABI on the current stream."""
+    global _native
+    import ctypes
+    import importlib
+    lib = _lib.load()
+    try:
+        module = importlib.import_module("._kv8", __package__)
+    except ImportError as e:
+        raise RuntimeError("the native binding _kv8.so is missing or does not load; build it with `python inference-server_b200/build.py`") from e
+    names = ("b200_kv_slot_map", "b200_kv8_append", "b200_kv8_attn_workspace_bytes", "b200_kv8_attn_decode", "b200_kv8_attn_prefill_workspace_bytes",
+             "b200_kv8_attn_prefill")
+    module.bind(check, *(ctypes.cast(getattr(lib, n), ctypes.c_void_p).value for n in names))
+    _native = module
+    return module
 
 
 def kv8_pools(num_blocks: int, num_kv_heads: int, head_dim: int, device="cuda"):
@@ -238,50 +234,13 @@ def kv8_pools(num_blocks: int, num_kv_heads: int, head_dim: int, device="cuda"):
     return *pools, *scales
 
 
-def _kv8_cache(k_pool, v_pool, k_scale, v_scale) -> tuple[int, int, int]:
-    shape = k_pool.shape
-    if not (k_pool.dtype is KV8_DTYPE and v_pool.dtype is KV8_DTYPE and k_scale.dtype is KV8_SCALE_DTYPE and v_scale.dtype is KV8_SCALE_DTYPE
-            and k_pool.is_contiguous() and v_pool.is_contiguous() and k_scale.is_contiguous() and v_scale.is_contiguous()):
-        _need(k_pool, "k_pool", KV8_DTYPE)
-        _need(v_pool, "v_pool", KV8_DTYPE)
-        _need(k_scale, "k_scale", KV8_SCALE_DTYPE)
-        _need(v_scale, "v_scale", KV8_SCALE_DTYPE)
-    if len(shape) != 4 or shape[2] != 16:
-        raise ValueError(f"k_pool must be [num_blocks, kv_heads, 16, head_dim], got {list(shape)}")
-    if v_pool.shape != shape or k_scale.shape != shape[:2] or v_scale.shape != shape[:2]:
-        raise ValueError("pools and scales do not match each other")
-    return shape[0], shape[1], shape[3]
-
-
 def kv_slot_map(ctx_lens, new_lens, block_table, supply, supply_used, num_rows: int, num_blocks: int,
                 status: torch.Tensor | None = None) -> KvSlotMap:
     """Where the new tokens of a pass go, worked out on the GPU: sequence b has ctx_lens[b] tokens and gets new_lens[b] more.  Pages they
     need are taken from `supply` [any], free page ids, from entry supply_used [1] on, and entered into block_table [B, max_pages] in
     place.  `num_rows`: rows of the pass, at least the sum of new_lens; rows behind the last token get slot -1.  Slots are
     page * 16 + position % 16, for `kv8_append` or any other cache of 16-token pages; page ids outside [0, num_blocks) are findings."""
-    for t in (ctx_lens, new_lens, block_table, supply, supply_used):
-        if t.dtype is not torch.int32 or not t.is_contiguous():
-            raise ValueError("lengths, block table, supply and supply_used must be contiguous int32 tensors")
-    stream = _stream_of(ctx_lens, new_lens, block_table, supply, supply_used)
-    if status is not None:
-        _status_word(status)
-        _stream_of(ctx_lens, status)
-    table = block_table.shape
-    B, R = table[0], int(num_rows)
-    if len(table) != 2 or ctx_lens.shape != table[:1] or new_lens.shape != table[:1] or supply_used.numel() != 1:
-        raise ValueError("lengths, block table or supply_used do not match")
-    if R < 0:
-        raise ValueError(f"{R} rows")
-    # one allocation; views are made in one go
-    m = KvSlotMap(*torch.split_with_sizes(ctx_lens.new_empty(2 * B + 2 + 3 * R), (B, B + 1, R, R, R, 1)))
-    lens = m.lens.data_ptr()
-    rows = lens + 4 * (2 * B + 1)
-    rc = _lib.load().b200_kv_slot_map(
-        ctx_lens.data_ptr(), new_lens.data_ptr(), block_table.data_ptr(), supply.data_ptr(), supply_used.data_ptr(), supply.numel(), lens,
-        lens + 4 * B, rows, rows + 4 * R, rows + 8 * R, rows + 12 * R, _ptr(status), B, R, int(num_blocks), table[1], stream)
-    if rc:
-        check(rc, "b200_kv_slot_map")
-    return m
+    return KvSlotMap(*(_native or _load_native()).slot_map(ctx_lens, new_lens, block_table, supply, supply_used, num_rows, num_blocks, status))
 
 
 def kv8_append(k_new, v_new, k_pool, v_pool, k_scale, v_scale, slots, status: torch.Tensor | None = None) -> None:
@@ -289,45 +248,7 @@ def kv8_append(k_new, v_new, k_pool, v_pool, k_scale, v_scale, slots, status: to
     slots [R] int32 = page * 16 + offset, as `kv_slot_map` gives them; negative: the row goes nowhere.  Rows of one page stand side
     by side, in order.  The scale of a page is the smallest power of two for which its largest number fits; see the header
     for how it grows."""
-    nb, Hkv, D = _kv8_cache(k_pool, v_pool, k_scale, v_scale)
-    if slots.dtype is not torch.int32 or not slots.is_contiguous():
-        raise ValueError("slots must be a contiguous int32 tensor")
-    dtype, shape = k_new.dtype, k_new.shape
-    if dtype not in DTYPE_CODE or v_new.dtype is not dtype:
-        raise ValueError(f"k_new and v_new must be bfloat16 or float32, got {dtype} and {v_new.dtype}")
-    R = slots.numel()
-    if shape != (R, Hkv, D) or v_new.shape != shape:
-        raise ValueError(f"k_new and v_new must be [{R}, {Hkv}, {D}], got {list(shape)} and {list(v_new.shape)}")
-    stream = _stream_of(k_pool, v_pool, k_scale, v_scale, k_new, v_new, slots)
-    if status is not None:
-        _status_word(status)
-        _stream_of(slots, status)
-    if R == 0:
-        return
-    for t in (k_new, v_new):
-        if not t.is_contiguous() and (t.stride(2) != 1 or (Hkv > 1 and t.stride(1) != D) or (R > 1 and t.stride(0) < Hkv * D)):
-            raise ValueError("k_new and v_new may be strided in their rows only")
-    rc = _lib.load().b200_kv8_append(
-        k_new.data_ptr(), v_new.data_ptr(), k_new.stride(0), v_new.stride(0), k_pool.data_ptr(), v_pool.data_ptr(), k_scale.data_ptr(),
-        v_scale.data_ptr(), slots.data_ptr(), _ptr(status), R, Hkv, D, nb, DTYPE_CODE[dtype], stream)
-    if rc:
-        check(rc, "b200_kv8_append")
-
-
-def _kv8_queries(q, out, index, workspace, D: int, what: str):
-    """Checks that the two attention calls share; rows and heads of q, and an `out` if none is given."""
-    shape = q.shape
-    if len(shape) != 3 or shape[2] != D:
-        raise ValueError(f"q must be [{what}, heads, {D}], got {list(shape)}")
-    if q.dtype is not torch.bfloat16 or not q.is_contiguous() or index.dtype is not torch.int32 or not index.is_contiguous():
-        raise ValueError("q must be contiguous bfloat16, block table and lengths contiguous int32 tensors")
-    if workspace is not None and (workspace.dtype is not torch.uint8 or not workspace.is_contiguous()):
-        raise ValueError("workspace must be a contiguous uint8 tensor")
-    if out is None:
-        out = torch.empty_like(q)
-    elif out.dtype is not torch.bfloat16 or not out.is_contiguous() or out.shape != shape:
-        raise ValueError("out must be a contiguous bfloat16 tensor of q's shape")
-    return shape[0], shape[1], out
+    (_native or _load_native()).append(k_new, v_new, k_pool, v_pool, k_scale, v_scale, slots, status)
 
 
 def kv8_attn_workspace(batch: int, num_q_heads: int, num_kv_heads: int, head_dim: int, max_pages: int, device,
@@ -341,22 +262,7 @@ def kv8_attn_decode(q, k_pool, v_pool, k_scale, v_scale, block_table, ctx_lens, 
                     workspace: torch.Tensor | None = None, out: torch.Tensor | None = None) -> torch.Tensor:
     """`paged_attn_decode` over an 8-bit page cache: softmax(q K^T * scale) V for one bf16 query row [B, Hq, D] per sequence; head_dim 64
     or 128, any head grouping.  `split_tokens`: tokens that a CTA takes at least; 0: the library's choice."""
-    nb, Hkv, D = _kv8_cache(k_pool, v_pool, k_scale, v_scale)
-    B, Hq, out = _kv8_queries(q, out, block_table, workspace, D, "batch")
-    table = block_table.shape
-    if len(table) != 2 or table[0] != B or ctx_lens.shape != table[:1] or ctx_lens.dtype is not torch.int32 or not ctx_lens.is_contiguous():
-        raise ValueError("block_table [batch, pages] and ctx_lens [batch] int32 must match q")
-    stream = _stream_of(q, k_pool, v_pool, k_scale, v_scale, block_table, ctx_lens, out, q if workspace is None else workspace)
-    if B == 0:
-        return out
-    if workspace is None:
-        workspace = kv8_attn_workspace(B, Hq, Hkv, D, table[1], q.device, int(split_tokens))
-    rc = _lib.load().b200_kv8_attn_decode(
-        q.data_ptr(), k_pool.data_ptr(), v_pool.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), block_table.data_ptr(), ctx_lens.data_ptr(),
-        out.data_ptr(), workspace.data_ptr(), workspace.numel(), B, Hq, Hkv, D, nb, table[1], float(scale), int(split_tokens), stream)
-    if rc:
-        check(rc, "b200_kv8_attn_decode")
-    return out
+    return (_native or _load_native()).decode(q, k_pool, v_pool, k_scale, v_scale, block_table, ctx_lens, scale, split_tokens, workspace, out)
 
 
 def kv8_attn_prefill_workspace(num_tokens: int, first_pos: int, num_q_heads: int, num_kv_heads: int, head_dim: int, device) -> torch.Tensor:
@@ -370,21 +276,7 @@ def kv8_attn_prefill(q, k_pool, v_pool, k_scale, v_scale, table_row, first_pos: 
     """`paged_attn_prefill` over an 8-bit page cache: causal attention of consecutive prompt tokens of one sequence, q [R, Hq, D] bf16 at
     positions first_pos .. first_pos + R - 1, keys and values already in their slots; table_row [max_pages] int32.  head_dim 64 or 128,
     up to 128 query heads per kv head.  Few rows over many keys are shared out along the keys and joined in the workspace."""
-    nb, Hkv, D = _kv8_cache(k_pool, v_pool, k_scale, v_scale)
-    R, Hq, out = _kv8_queries(q, out, table_row, workspace, D, "tokens")
-    if table_row.dim() != 1:
-        raise ValueError("table_row must be one row of a block table")
-    stream = _stream_of(q, k_pool, v_pool, k_scale, v_scale, table_row, out, q if workspace is None else workspace)
-    if R == 0:
-        return out
-    if workspace is None:
-        workspace = kv8_attn_prefill_workspace(R, int(first_pos), Hq, Hkv, D, q.device)
-    rc = _lib.load().b200_kv8_attn_prefill(
-        q.data_ptr(), k_pool.data_ptr(), v_pool.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), table_row.data_ptr(), out.data_ptr(),
-        workspace.data_ptr(), workspace.numel(), R, int(first_pos), Hq, Hkv, D, nb, table_row.numel(), float(scale), stream)
-    if rc:
-        check(rc, "b200_kv8_attn_prefill")
-    return out
+    return (_native or _load_native()).prefill(q, k_pool, v_pool, k_scale, v_scale, table_row, first_pos, scale, workspace, out)
 
 
 # ---------------------------------------------------------- dense projections
