@@ -518,37 +518,47 @@ kv8_attn_decode_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_c
 #endif
 }
 
-// Joins the parts of one (row, query head): WARPS warps share them out, warp w taking parts w, w + WARPS, ..., eight at a time, each lane
-// D / 32 columns.  The sums over parts are taken in a fixed order.  With `rows` the parts are those of kv8_attn_decode_kernel;
+// Where the parts of a (row, query head) are: part 0, then `next`, `next` + `step`, ...  With `rows` they are those of kv8_attn_decode_kernel;
 // without, every row has `parts` of them, side by side, some perhaps empty (their reference is -inf and their sums are not written).
-// One warp per row serves batches, whose rows have a handful of parts, and 16 a few rows of hundreds.
-template <int D, int WARPS>
-__global__ void __launch_bounds__(WARPS == 1 ? 128 : 32 * WARPS)
+struct Kv8Parts {
+  int n;
+  long long first, next;
+  int step;
+  __device__ __forceinline__ Kv8Parts(const int2* rows, int row, int num_q_heads, int parts) {
+    if (rows == nullptr) {
+      n = parts;
+      first = static_cast<long long>(row) * parts;
+      next = first + 1;
+      step = 1;
+    } else {
+      const int2 at = rows[row / num_q_heads];
+      const int head = row % num_q_heads;
+      n = at.y;
+      first = static_cast<long long>(at.x) * num_q_heads + head;
+      next = static_cast<long long>((at.x | 1) + 1) * num_q_heads + head;  // the first part of the run after
+      step = 2 * num_q_heads;
+    }
+  }
+  __device__ __forceinline__ size_t at(int k) const { return static_cast<size_t>(k == 0 ? first : next + static_cast<long long>(k - 1) * step); }
+};
+
+// Joins the parts of one (row, query head) per warp, eight at a time, each lane D / 32 columns: for batches, whose rows have a handful.
+template <int D>
+__global__ void __launch_bounds__(128)
 kv8_attn_join_kernel(const float* __restrict__ part_o, const float2* __restrict__ part_ml, const int2* __restrict__ rows,
                      __nv_bfloat16* __restrict__ out, int num_q_heads, int num_rows, int parts) {
   grid_dep_wait();
   grid_dep_launch();
   constexpr int V = D / 32;
-  __shared__ float o_sm[WARPS][WARPS == 1 ? 1 : D];
-  __shared__ float ml_sm[WARPS][2];
-  const int lane = threadIdx.x & 31, warp = WARPS == 1 ? 0 : threadIdx.x >> 5;
-  const int row = WARPS == 1 ? static_cast<int>(blockIdx.x * 4 + (threadIdx.x >> 5)) : static_cast<int>(blockIdx.x);
-  if (row >= num_rows) return;  // WARPS > 1: never
-  int n = parts, first = row * parts, next = row * parts + 1, step = 1;  // part 0, then next, next + step, ...
-  if (rows != nullptr) {
-    const int2 at = rows[row / num_q_heads];
-    const int head = row % num_q_heads;
-    n = at.y;
-    if (n <= 1) return;  // written by its one CTA
-    first = at.x * num_q_heads + head;
-    next = ((at.x | 1) + 1) * num_q_heads + head;  // the first part of the run after
-    step = 2 * num_q_heads;
-  }
+  const int lane = threadIdx.x & 31, row = static_cast<int>(blockIdx.x * 4 + (threadIdx.x >> 5));
+  if (row >= num_rows) return;
+  const Kv8Parts where(rows, row, num_q_heads, parts);
+  if (rows != nullptr && where.n <= 1) return;  // written by its one CTA
   float top = -INFINITY, den = 0.f, acc[V];
 #pragma unroll
   for (int j = 0; j < V; ++j) acc[j] = 0.f;
 #pragma unroll 1
-  for (int k0 = warp; k0 < n; k0 += 8 * WARPS) {
+  for (int k0 = 0; k0 < where.n; k0 += 8) {
     float v[8][V];
     float2 ml[8];
 #pragma unroll
@@ -556,9 +566,8 @@ kv8_attn_join_kernel(const float* __restrict__ part_o, const float2* __restrict_
       ml[u] = make_float2(-INFINITY, 0.f);
 #pragma unroll
       for (int j = 0; j < V; ++j) v[u][j] = 0.f;
-      const int k = k0 + u * WARPS;
-      if (k < n) {
-        const size_t from = k == 0 ? static_cast<size_t>(first) : static_cast<size_t>(next) + static_cast<size_t>(k - 1) * step;
+      if (k0 + u < where.n) {
+        const size_t from = where.at(k0 + u);
         ml[u] = part_ml[from];
 #pragma unroll
         for (int j = 0; j < V; ++j) v[u][j] = part_o[from * D + lane * V + j];
@@ -581,43 +590,105 @@ kv8_attn_join_kernel(const float* __restrict__ part_o, const float2* __restrict_
       for (int j = 0; j < V; ++j) acc[j] = fmaf(w, ml[u].x == -INFINITY ? 0.f : v[u][j], acc[j]);
     }
   }
-  if constexpr (WARPS == 1) {
-    const float inv = 1.f / den;
-    uint32_t* to = reinterpret_cast<uint32_t*>(out + static_cast<size_t>(row) * D + lane * V);
+  const float inv = 1.f / den;
+  uint32_t* to = reinterpret_cast<uint32_t*>(out + static_cast<size_t>(row) * D + lane * V);
 #pragma unroll
-    for (int j = 0; j < V; j += 2) to[j / 2] = pack_bf16x2(acc[j] * inv, acc[j + 1] * inv);
-  } else {
-#pragma unroll
-    for (int j = 0; j < V; ++j) o_sm[warp][lane * V + j] = acc[j];
-    if (lane == 0) {
-      ml_sm[warp][0] = top;
-      ml_sm[warp][1] = den;
-    }
-    __syncthreads();
-    const int d = threadIdx.x;
-    if (d >= D) return;
-    float t = ml_sm[0][0];
-#pragma unroll
-    for (int w = 1; w < WARPS; ++w) t = fmaxf(t, ml_sm[w][0]);
-    const float ref = t == -INFINITY ? 0.f : t;
-    float num = 0.f, sum = 0.f;
-#pragma unroll
-    for (int w = 0; w < WARPS; ++w) {
-      const float x = fast_ex2(ml_sm[w][0] - ref);
-      num += x * o_sm[w][d];
-      sum += x * ml_sm[w][1];
-    }
-    out[static_cast<size_t>(row) * D + d] = __float2bfloat16(num / sum);
-  }
+  for (int j = 0; j < V; j += 2) to[j / 2] = pack_bf16x2(acc[j] * inv, acc[j + 1] * inv);
 }
 
+// The same for few rows of many parts: a CTA of WARPS warps per (row, query head) and 32 columns, eight lanes per part, so that all parts are
+// asked for at once: 32 parts a round with four warps, or 320 with sixteen.  (16 warps over all columns with three rounds: 8 us for 296 parts.)
+template <int D, int WARPS>
+__global__ void __launch_bounds__(32 * WARPS)
+kv8_attn_join_wide_kernel(const float* __restrict__ part_o, const float2* __restrict__ part_ml, const int2* __restrict__ rows,
+                          __nv_bfloat16* __restrict__ out, int num_q_heads, int parts) {
+  grid_dep_wait();
+  grid_dep_launch();
+  constexpr int kRound = WARPS == 4 ? 2 : 5;  // parts of a thread and round
+  __shared__ float4 o_sm[WARPS][8];
+  __shared__ float2 ml_sm[WARPS];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, col = blockIdx.y * 32 + (lane & 7) * 4;
+  const int row = blockIdx.x;
+  const Kv8Parts where(rows, row, num_q_heads, parts);
+  if (rows != nullptr && where.n <= 1) return;
+  float top = -INFINITY, den = 0.f;
+  float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 1
+  for (int k0 = warp * 4 + (lane >> 3); k0 < where.n; k0 += kRound * WARPS * 4) {
+    float4 v[kRound];
+    float2 ml[kRound];
+#pragma unroll
+    for (int u = 0; u < kRound; ++u) {
+      const int k = k0 + u * WARPS * 4;
+      ml[u] = make_float2(-INFINITY, 0.f);
+      v[u] = make_float4(0.f, 0.f, 0.f, 0.f);
+      if (k < where.n) {
+        const size_t from = where.at(k);
+        ml[u] = part_ml[from];
+        v[u] = *reinterpret_cast<const float4*>(part_o + from * D + col);
+      }
+    }
+    float t = top;
+#pragma unroll
+    for (int u = 0; u < kRound; ++u) t = fmaxf(t, ml[u].x);
+    const float ref = t == -INFINITY ? 0.f : t, a = fast_ex2(top - ref);
+    top = t;
+    den *= a;
+    acc.x *= a, acc.y *= a, acc.z *= a, acc.w *= a;
+#pragma unroll
+    for (int u = 0; u < kRound; ++u) {
+      const float w = fast_ex2(ml[u].x - ref);
+      den = fmaf(w, ml[u].y, den);
+      if (ml[u].x != -INFINITY) {
+        acc.x = fmaf(w, v[u].x, acc.x);
+        acc.y = fmaf(w, v[u].y, acc.y);
+        acc.z = fmaf(w, v[u].z, acc.z);
+        acc.w = fmaf(w, v[u].w, acc.w);
+      }
+    }
+  }
+  // the four parts that a warp takes side by side, then the warps, each time against the common reference
+  auto into = [](float mine, float common) { return fast_ex2(mine - (common == -INFINITY ? 0.f : common)); };
+  const float warp_top = warp_max(top), a = into(top, warp_top);
+  den *= a;
+  acc.x *= a, acc.y *= a, acc.z *= a, acc.w *= a;
+#pragma unroll
+  for (int o = 8; o < 32; o <<= 1) {
+    den += __shfl_xor_sync(0xffffffffu, den, o);
+    acc.x += __shfl_xor_sync(0xffffffffu, acc.x, o);
+    acc.y += __shfl_xor_sync(0xffffffffu, acc.y, o);
+    acc.z += __shfl_xor_sync(0xffffffffu, acc.z, o);
+    acc.w += __shfl_xor_sync(0xffffffffu, acc.w, o);
+  }
+  if (lane < 8) o_sm[warp][lane] = acc;
+  if (lane == 0) ml_sm[warp] = make_float2(warp_top, den);
+  __syncthreads();
+  if (threadIdx.x >= 32) return;
+  float t = ml_sm[0].x;
+#pragma unroll
+  for (int w = 1; w < WARPS; ++w) t = fmaxf(t, ml_sm[w].x);
+  float num = 0.f, sum = 0.f;
+#pragma unroll
+  for (int w = 0; w < WARPS; ++w) {
+    const float x = into(ml_sm[w].x, t);
+    num += x * reinterpret_cast<const float*>(o_sm[w])[lane];
+    sum += x * ml_sm[w].y;
+  }
+  out[static_cast<size_t>(row) * D + blockIdx.y * 32 + lane] = __float2bfloat16(num / sum);
+}
+
+// `expected`: parts that a row is likely to have.  The wide form where they are many and the rows few: us for a whole call, narrow and wide, 528 rows
+// of 18 parts 12.3, 10.3; 1088 rows of 11 parts 27.7, 29.7.
 template <int D>
-static int launch_join(const float* o, const float2* ml, const int2* rows, void* out, int hq, int num_rows, int parts, int most, cudaStream_t st) {
+static int launch_join(const float* o, const float2* ml, const int2* rows, void* out, int hq, int num_rows, int parts, int expected,
+                       cudaStream_t st) {
   __nv_bfloat16* to = static_cast<__nv_bfloat16*>(out);
-  if (most <= 16)
-    B200_CUDA(launch_overlapped(kv8_attn_join_kernel<D, 1>, dim3((num_rows + 3) / 4), dim3(128), 0, st, o, ml, rows, to, hq, num_rows, parts));
+  if (expected <= 8 || num_rows >= 1024)
+    B200_CUDA(launch_overlapped(kv8_attn_join_kernel<D>, dim3((num_rows + 3) / 4), dim3(128), 0, st, o, ml, rows, to, hq, num_rows, parts));
+  else if (expected <= 64)
+    B200_CUDA(launch_overlapped(kv8_attn_join_wide_kernel<D, 4>, dim3(num_rows, D / 32), dim3(128), 0, st, o, ml, rows, to, hq, parts));
   else
-    B200_CUDA(launch_overlapped(kv8_attn_join_kernel<D, 16>, dim3(num_rows), dim3(512), 0, st, o, ml, rows, to, hq, num_rows, parts));
+    B200_CUDA(launch_overlapped(kv8_attn_join_wide_kernel<D, 16>, dim3(num_rows, D / 32), dim3(512), 0, st, o, ml, rows, to, hq, parts));
   return 0;
 }
 int launch_kv8_join(int head_dim, const AttnWorkspace& w, void* out, int rows, int hq, int parts, cudaStream_t st) {
@@ -642,8 +713,6 @@ static int kv8_plan(int batch, int hq, int hkv, int head_dim, int max_pages, int
   p->min_run = split_tokens > 0 ? split_tokens / kKvPage : 2;
   return 0;
 }
-
-constexpr int kKv8FewRows = 8;  // from this on a row has a handful of parts
 
 struct Kv8Args {
   const void *q, *k_pool, *v_pool, *k_scale, *v_scale;
@@ -674,10 +743,10 @@ static int launch_kv8_decode(const Kv8Args& a) {
                               static_cast<const uint8_t*>(a.v_scale), a.table, a.ctx, a.w.o, a.w.ml, a.w.rows,
                               static_cast<__nv_bfloat16*>(a.out), a.w.err, a.batch, a.hq, a.hkv, a.num_blocks, a.max_pages, a.plan.min_run,
                               a.scale * 1.4426950408889634f));
-  // parts of a row at most
-  const int most = static_cast<int>(std::min<long long>(a.plan.runs, static_cast<long long>(a.max_pages - 1) / a.plan.min_run + 2));
-  if (a.batch == 1 && a.max_pages <= a.plan.min_run) return 0;
-  return launch_join<D>(a.w.o, a.w.ml, a.w.rows, a.out, a.hq, a.batch * a.hq, 0, a.batch >= kKv8FewRows ? 1 : most, a.st);
+  if (a.batch == 1 && a.max_pages <= a.plan.min_run) return 0;  // one run
+  // Rows share the runs: a row has about runs / batch parts, and no more than its pages give.
+  const int expected = static_cast<int>(std::min<long long>(a.plan.runs / a.batch, static_cast<long long>(a.max_pages - 1) / a.plan.min_run) + 1);
+  return launch_join<D>(a.w.o, a.w.ml, a.w.rows, a.out, a.hq, a.batch * a.hq, 0, expected, a.st);
 }
 
 template <int D, int NT>
