@@ -181,13 +181,14 @@ struct RowPiece {
     uint32_t codes[kNumbers / 4];
 #pragma unroll
     for (int k = 0; k < kNumbers / 4; ++k) {
-      float v[4];
+      float x[4];
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        const float x = value(4 * k + i);
-        v[i] = ODD && !(fabsf(x) < INFINITY) ? NAN : x * by;
+        x[i] = value(4 * k + i);
+        if (ODD && !(fabsf(x[i]) < INFINITY)) x[i] = NAN;
       }
-      codes[k] = to_e4m3x2(v[0], v[1]) | to_e4m3x2(v[2], v[3]) << 16;
+      const float2 lo = mul_pair(x[0], x[1], by), hi = mul_pair(x[2], x[3], by);
+      codes[k] = to_e4m3x4(lo.x, lo.y, hi.x, hi.y);
     }
     if constexpr (kNumbers == 8) *reinterpret_cast<uint2*>(to) = make_uint2(codes[0], codes[1]);
     else *reinterpret_cast<uint32_t*>(to) = codes[0];
@@ -199,7 +200,7 @@ __device__ __forceinline__ uint32_t round_again(uint32_t codes, float by) {
   uint32_t lo, hi;
   e4m3x4_to_f16(codes, lo, hi);
   const float2 a = __half22float2(*reinterpret_cast<const __half2*>(&lo)), b = __half22float2(*reinterpret_cast<const __half2*>(&hi));
-  return to_e4m3x2(a.x * by, a.y * by) | to_e4m3x2(b.x * by, b.y * by) << 16;
+  return to_e4m3x4(a.x * by, a.y * by, b.x * by, b.y * by);
 }
 
 template <typename T, int D>
@@ -225,11 +226,11 @@ kv8_append_kernel(const T* __restrict__ k_new, const T* __restrict__ v_new, long
   const int left = __shfl_up_sync(0xffffffffu, block, 1);
   unsigned starts = __ballot_sync(0xffffffffu, lane >= 1 && lane <= window && block >= 0 && block != left);
   const int items = 2 * num_kv_heads, total = __popc(starts) * items;
-  int run = 0;  // of the lowest bit left in `starts`
+  int item = warp;  // of the run of the lowest bit left in `starts`
 #pragma unroll 1
-  for (int it = warp; it < total; it += kAppendWarps) {
-    for (; run < it / items; ++run) starts &= starts - 1;
-    const int first = __ffs(starts) - 1, item = it % items;
+  for (int it = warp; it < total; it += kAppendWarps, item += kAppendWarps) {
+    for (; item >= items; item -= items) starts &= starts - 1;
+    const int first = __ffs(starts) - 1;
     const int page = __shfl_sync(0xffffffffu, block, first);
     const unsigned same = __ballot_sync(0xffffffffu, block == page) >> first;
     int n = __ffs(~same) - 1;  // rows of the run among those of the lanes; first >= 1, so a bit of `same` is clear

@@ -240,7 +240,7 @@ def kv_slot_map(ctx_lens, new_lens, block_table, supply, supply_used, num_rows: 
     need are taken from `supply` [any], free page ids, from entry supply_used [1] on, and entered into block_table [B, max_pages] in
     place.  `num_rows`: rows of the pass, at least the sum of new_lens; rows behind the last token get slot -1.  Slots are
     page * 16 + position % 16, for `kv8_append` or any other cache of 16-token pages; page ids outside [0, num_blocks) are findings."""
-    return KvSlotMap(*(_native or _load_native()).slot_map(ctx_lens, new_lens, block_table, supply, supply_used, num_rows, num_blocks, status))
+    return tuple.__new__(KvSlotMap, (_native or _load_native()).slot_map(ctx_lens, new_lens, block_table, supply, supply_used, num_rows, num_blocks, status))
 
 
 def kv8_append(k_new, v_new, k_pool, v_pool, k_scale, v_scale, slots, status: torch.Tensor | None = None) -> None:
