@@ -203,6 +203,15 @@ def test_wrappers_refuse(ops):
         ops.kv8_attn_decode(q, *pools, table, slots, -0.1)
     with pytest.raises(err, match="multiple of kv heads"):
         ops.kv8_attn_decode(q[:, :3].contiguous(), *pools, table, slots, 0.1)
+    for call in (lambda: ops.kv8_append(None, x, *pools, slots), lambda: ops.kv8_append(x, x, *pools, [0, 1, 2]),
+                 lambda: ops.kv_slot_map(slots, slots, table, slots, slots[:1], -1, 4), lambda: ops.kv_slot_map(slots, slots, table, slots, slots, 1, 4),
+                 lambda: ops.kv_slot_map(slots, slots[:2], table, slots, slots[:1], 1, 4), lambda: ops.kv_slot_map(slots, slots, table, slots, slots[:1], 2 ** 40, 4)):
+        with pytest.raises(ValueError):
+            call()
+    with pytest.raises(TypeError):
+        ops.kv8_attn_decode(q, *pools, table, slots, "0.1")
+    with pytest.raises(err, match="dimension"):
+        ops.kv_slot_map(slots, slots, table, slots, slots[:1], 4, 0)
     ops.kv8_append(x[:0], x[:0], *pools, slots[:0])
     assert ops.kv8_attn_decode(q[:0], *pools, table[:0], slots[:0], 0.1).shape == (0, 4, 64)
 
@@ -430,6 +439,72 @@ def test_prefill_findings_and_refusals(ops):
         with pytest.raises(ValueError):
             ops.kv8_attn_prefill(**(dict(q=q, k_pool=args[0], v_pool=args[1], k_scale=args[2], v_scale=args[3], table_row=row, first_pos=0, scale=0.1) | bad))
     assert ops.kv8_attn_prefill(q[:0], *args, row, 50, 0.1).shape == (0, 8, 64)
+
+
+def test_prefill_nan_reaches_its_key_tile_and_later_rows(ops):
+    """A NaN key is masked ahead of its token; a NaN value reaches the rows from at most 127 tokens before it on, in its kv head and column."""
+    rng = np.random.default_rng(34)
+    n = 400
+    q, kc, ke, vc, ve, table = attn_case(rng, [n], 8, 2, 64)
+    q = torch.from_numpy(rng.standard_normal((n, 8, 64)).astype(np.float32)).bfloat16().to(DEV)
+    args = lambda k, v: (plain.pool_of(k), plain.pool_of(v), plain.scale_of(ke), plain.scale_of(ve), torch.from_numpy(table[0]).to(DEV), 0, 0.1)
+    bad = kc.copy()
+    bad[table[0, 300 // 16], 1, 300 % 16, 9] = 127
+    got = ops.kv8_attn_prefill(q, *args(bad, vc)).isnan()
+    assert not got[:, :4].any() and not got[:300].any() and got[300:, 4:].all()
+    bad = vc.copy()
+    bad[table[0, 300 // 16], 0, 300 % 16, 9] = 255
+    got = ops.kv8_attn_prefill(q, *args(kc, bad)).isnan()
+    assert not got[:, 4:].any() and not got[:300 - 127].any() and got[300:, :4, 9].all()
+    got[:, :4, 9] = False
+    assert not got.any()
+    bad = q.clone()
+    bad[7, 3, 2] = float("inf")
+    bad[200, 5, 60] = float("nan")
+    got = ops.kv8_attn_prefill(bad, *args(kc, vc)).isnan()
+    assert got[7, 3].all() and got[200, 5].all() and int(got.sum()) == 128
+
+
+def test_prefill_captured_on_another_stream_beside_a_second_call(ops):
+    """A captured prompt pass - append, then attention over keys shared out in parts - replayed with other rows in its buffers, while a
+    call with a workspace of its own runs on a second stream."""
+    rng = np.random.default_rng(35)
+    H, Hq, D, n, first = 2, 8, 128, 40, 3000
+    _, kc, ke, vc, ve, table = attn_case(rng, [first + n], Hq, H, D)
+    codes = [np.where(c & 127 == 127, 0, c) for c in (kc, vc)]
+    cache = [plain.pool_of(c.copy()) for c in codes] + [plain.scale_of(ke), plain.scale_of(ve)]
+    other = [c.clone() for c in cache]
+    row = torch.from_numpy(table[0]).to(DEV)
+    slots = ints([int(table[0, p // 16]) * 16 + p % 16 for p in range(first, first + n)])
+    q = torch.zeros(n, Hq, D, device=DEV, dtype=torch.bfloat16)
+    k, v = torch.zeros(n, H, D, device=DEV, dtype=torch.bfloat16), torch.zeros(n, H, D, device=DEV, dtype=torch.bfloat16)
+    ws = [ops.kv8_attn_prefill_workspace(n, first, Hq, H, D, DEV) for _ in range(2)]
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    for s in streams:
+        s.wait_stream(torch.cuda.current_stream())
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=streams[0]):
+        ops.kv8_append(k, v, *cache, slots)
+        out = ops.kv8_attn_prefill(q, *cache, row, first, 0.1, workspace=ws[0])
+    still = torch.randn(n, Hq, D, device=DEV).bfloat16()
+    with torch.cuda.stream(streams[1]):
+        alone = ops.kv8_attn_prefill(still, *other, row, first, 0.1, workspace=ws[1])
+    host = [c.copy() for c in codes], [ke.copy(), ve.copy()]
+    for turn in range(3):
+        rows = rows_of(rng, n, H, D, torch.bfloat16)
+        with torch.cuda.stream(streams[0]):
+            q.copy_(torch.from_numpy(rng.standard_normal((n, Hq, D)).astype(np.float32)))
+            for x, r in zip((k, v), rows):
+                x.copy_(torch.from_numpy(r))
+            torch.cuda.synchronize()
+            graph.replay()
+        with torch.cuda.stream(streams[1]):
+            again = [ops.kv8_attn_prefill(still, *other, row, first, 0.1, workspace=ws[1]) for _ in range(4)]
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, alone) for a in again)
+        for x, c, e in zip((k, v), *host):
+            plain.append(x.double().cpu().numpy(), slots.tolist(), c, e)
+        check_attn(out, q.cpu(), host[0][0], host[1][0], host[0][1], host[1][1], [table[0]] * n, range(first + 1, first + n + 1), 0.1, 2.0 ** -10 / 224)
 
 
 def test_prefill_agrees_with_decode(ops):
