@@ -14,7 +14,8 @@ namespace b200 {
 // exclusive prefix sums; so do the rows of the new tokens.  Every CTA takes the sums of all sequences for itself (a few KB from L2, one
 // scan of pairs packed into 64 bits) and keeps them in shared memory; then a row finds its sequence, and a fresh page its place in the
 // table, by bisection.  So one launch does all of it, no CTA waits for another, and none reads what another writes: a row in a
-// fresh page takes the page from the list and not from the table.
+// fresh page takes the page from the list and not from the table.  Bound by the chain of loads (lengths, then list or table): 3.5 us for a
+// step of 256 sequences and for 48 prompts of 20000 tokens, a launch included; the scan is 256 sequences a round.
 constexpr int kMapThreads = 256;
 constexpr int kMapMaxSeqs = 4096;
 
@@ -146,6 +147,9 @@ kv_slot_map_kernel(const int* __restrict__ ctx_lens, const int* __restrict__ new
 // A CTA looks after `window` rows: it does the runs that begin there, its warps sharing (run, head, K or V) items.  Few rows per window
 // give a decode step, whose rows are runs of one, a CTA each; many rows per window keep a prompt, whose runs are 16 long, from
 // launching CTAs that find nothing to begin.
+//
+// Bound by memory for prompts, whose rows are read once (8970 rows of 4 heads of 128 in bf16, 28 MB read and written, 9.2 us; 4.2 at the copy
+// rate, the rest a launch and the chain slot -> rows -> largest magnitude -> scale -> stores), by that chain for steps (256 rows 3.5 us).
 constexpr int kAppendWarps = 8;
 constexpr int kAppendMaxWindow = 16;  // a run that begins in a window lies within the 32 rows that a warp's lanes look at
 
@@ -322,7 +326,9 @@ static int launch_append(const void* k_new, const void* v_new, long long ks, lon
   int sms = 0;
   int rc = device_sm_count(&sms);
   if (rc) return rc;
-  int window = 1;  // the fewest rows per CTA with which the grid fits the GPU at once
+  // The fewest rows per CTA with which the grid fits the GPU at once.  us with 4, 8 and 16 CTAs per SM in its place: 8970 rows of 4 heads of 128 in bf16 9.6, 11.9,
+  // 12.8; 61 short prompts of 2 heads of 64 in fp32 3.5, 4.1, 4.1.
+  int window = 1;
   while (window < kAppendMaxWindow && (rows + window - 1) / window > 4 * sms) window *= 2;
   B200_CUDA(launch_overlapped(kv8_append_kernel<T, D>, dim3((rows + window - 1) / window), dim3(kAppendWarps * 32), 0, st,
                               static_cast<const T*>(k_new), static_cast<const T*>(v_new), ks, vs, static_cast<uint8_t*>(k_pool),

@@ -209,8 +209,9 @@ PyObject* append(PyObject*, PyObject* const* args, Py_ssize_t n) {
     for (const at::Tensor* t : {&k, &v})
       if (!t->is_contiguous() && (t->stride(2) != 1 || (c.heads > 1 && t->stride(1) != c.dim) || (R > 1 && t->stride(0) < int64_t(c.heads) * c.dim)))
         refuse("k_new and v_new may be strided in their rows only");
+    const int64_t row = int64_t(c.heads) * c.dim;  // the stride of a single row says nothing
     const int rc = without_gil([&] {
-      return p_append(k.data_ptr(), v.data_ptr(), k.stride(0), v.stride(0), c.k.data_ptr(), c.v.data_ptr(), c.ks.data_ptr(), c.vs.data_ptr(),
+      return p_append(k.data_ptr(), v.data_ptr(), R > 1 ? k.stride(0) : row, R > 1 ? v.stride(0) : row, c.k.data_ptr(), c.v.data_ptr(), c.ks.data_ptr(), c.vs.data_ptr(),
                       slots.data_ptr<int32_t>(), status, R, c.heads, c.dim, c.blocks, dtype == at::kBFloat16 ? B200_DTYPE_BF16 : B200_DTYPE_F32,
                       stream_of(device));
     });

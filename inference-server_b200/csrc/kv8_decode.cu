@@ -6,11 +6,15 @@
 // e4m3 numbers k_t, the output is  sum_t 2^(s_t + ev) v_t / sum_t 2^s_t.  A value's scale is taken into its weight's exponent:
 // p_t = 2^(s_t + ev - m), where m follows the maximum of s_t + ev, so the largest weight sees the largest product and not the largest
 // score.  The denominator is sum_t p_t 2^-ev.  Everything that has a scale in it is an fp32 exponent; e4m3 numbers become f16 exactly, and
-// weights are f16, whose 11 bits leave them a 16th of the error of bf16.  Weights are taken so that
-// the largest is between 2^6 and 2^14; those below 2^-14 lose bits.  Queries are multiplied by a power of two that brings the largest of a kv group to 2^14 and become f16: what loses bits
-// is 2^-28 of the largest.  Sums are fp32.  With |ev| <= 32 the sums p_t 2^-ev stay below 2^14 * 2^32 * tokens.
+// weights are f16, whose 11 bits leave them an eighth of the error of bf16.  Weights are taken so that the largest is between 2^6 and
+// 2^14; those below 2^-14 lose bits.  Queries are multiplied by a power of two that brings the largest of a kv group to 2^14 and become
+// f16: what loses bits is 2^-28 of the largest.  Sums are fp32.  With |ev| <= 32 the sums p_t 2^-ev stay below 2^14 * 2^32 * tokens.
 //
-//   work   The pages of all rows, one row after the other, are cut into equal runs, one per CTA (2 per SM for 4 kv heads of 128), wherever
+// Bound by memory: 2 D bytes per token and kv head, one scale byte per 16 D of them.  256 rows of 512 to 4096 tokens, 32 / 4 heads of
+// 128, 592 MB: 100 us at 5.9 TB/s and 7 for the join, 106 in a row of calls.  The rest is a chain of 8 to 10 us that no call is without - lengths,
+// table, the first pages, the last pages' arithmetic, partials -: one row of 777 tokens 7.2 us, 131001 tokens 31.6 us (134 MB).
+//
+//   work   The pages of all rows, one row after the other, are cut into equal runs, one per CTA (kv8_ctas_per_sm), wherever
 //          that falls in a row: every CTA streams the same number of bytes without a break, whatever the rows' lengths, and there are no
 //          waves.  Each CTA finds its run by itself from the lengths (a scan of at most a few KB).  It meets at most one row that began in a
 //          run before and one that goes on in the next; those give fp32 partials (o, m, l), all others are written at once.
@@ -59,16 +63,26 @@ __device__ __forceinline__ uint32_t transpose_8x8(uint32_t x) {
   return y;
 }
 
-// CTAs that an SM holds: as many as leave each enough of the ring, and of the registers, to keep its share of the memory busy.
+// CTAs that an SM holds: as many as leave each enough of the ring, and of the registers, to keep its share of the memory busy.  More of
+// them cut more rows.  us for 128 rows of 512 to 4096 tokens: head_dim 128, 4 kv heads (256 rows) one 126, two 106; 2 kv heads of 8 queries two 39.8, three
+// 33.6, four 35.1, of 16 two 47.5, three 42.5; 1 kv head of 8 queries four 20.6, six 19.5, of 16 four 31.5, five 31.0.  head_dim 64, 4 kv heads of 8 two
+// 36.6, three 34.1, of 16 two 40.1, three 39.0; 2 kv heads of 8 four 22.5, five 21.1, of 16 three 27.7, four 24.2; 1 kv head of 8 four
+// 17.0, six 15.5, eight 16.1, of 16 five 21.9, six 19.9.
 constexpr int kv8_ctas_per_sm(int head_dim, int hkv, int nt) {
-  return hkv == 1 ? (nt == 1 ? 6 : 5) : hkv == 2 ? (nt == 1 ? 4 : 3) : hkv == 4 ? 2 : 1;
+  if (head_dim == 64) return hkv == 1 ? 6 : hkv == 2 ? (nt == 1 ? 5 : 4) : 3;
+  return hkv == 1 ? (nt == 1 ? 6 : 5) : hkv == 2 ? 3 : hkv == 4 ? 2 : 1;
+}
+// Kv heads of a CTA.  Eight of head_dim 64 leave an SM room for one CTA, which fills it less well than three of four heads: 128 rows of 512 to 4096
+// tokens, 64 / 8 heads 64.3 us, 58.3; of head_dim 128, 32 / 8 heads, 96.8 us and two of four 100.8.
+constexpr int kv8_heads_per_cta(int head_dim, int hkv) {
+  return hkv % 8 == 0 && head_dim == 128 ? 8 : hkv % 4 == 0 ? 4 : hkv % 2 == 0 ? 2 : 1;
 }
 
 // Workspace: the status word, per row where its parts are, then the parts: (m, l) and the unnormalised output per (run, which of its two
 // open rows, query head).
 struct Kv8Workspace {
   int* err;
-  int2* rows;  // run of the first part (its sign: the run's second open row), number of parts
+  int2* rows;  // first part as run * 2 + (is it the run's second open row?), number of parts
   float2* ml;
   float* o;
   size_t bytes;
@@ -186,7 +200,8 @@ kv8_attn_decode_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_c
   const uint32_t bars = ring + Cfg::kBars;  // full[STAGES], empty[STAGES], queries there, queries read
   const uint32_t bar_q = bars + 16 * STAGES;
 
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int lane = threadIdx.x & 31;
+  int warp = threadIdx.x >> 5;
   const int head_groups = num_kv_heads / HKV;
   const int kv0 = static_cast<int>(blockIdx.y) % head_groups * HKV;   // first kv head of this CTA
   const int q0 = static_cast<int>(blockIdx.y) / head_groups * (8 * NT);  // first query head of the group
@@ -207,7 +222,18 @@ kv8_attn_decode_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_c
     tma_prefetch_desc(&k_map);
     tma_prefetch_desc(&v_map);
   }
-  __syncthreads();
+  // Blocks of two warps would have all consumers on schedulers 0 and 2: every second pair of warps of the SM swaps its roles, whichever warps the
+  // hardware took (23.5 -> 19.5 us for 128 rows of 512 to 4096 tokens, 8 / 1 heads of 128).
+  if constexpr (HKV == 1) {
+    __shared__ int swap_roles;
+    int hardware_warp;
+    asm volatile("mov.u32 %0, %%warpid;" : "=r"(hardware_warp));
+    if (threadIdx.x == 0) swap_roles = (hardware_warp >> 2) & 1;
+    __syncthreads();
+    warp ^= swap_roles;
+  } else {
+    __syncthreads();
+  }
   grid_dep_wait();  // lengths, queries and the new tokens' pages come from the kernels before
   grid_dep_launch();
 
@@ -486,7 +512,7 @@ kv8_attn_decode_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_c
     // a part that begins with the run is the first of its two, one that does not is the second and the row's first part
     const bool second = walk.at != walk.begin;
     const size_t here = static_cast<size_t>(blockIdx.x) * 2 + second;
-    if (first_run == static_cast<int>(blockIdx.x) && blockIdx.y == 0 && threadIdx.x == 0)
+    if (first_run == static_cast<int>(blockIdx.x) && blockIdx.y == 0 && warp == 0 && lane == 0)
       rows[walk.row] = make_int2(first_run * 2 + second, parts);
 #pragma unroll
     for (int t = 0; t < NT; ++t)
@@ -702,7 +728,7 @@ struct Kv8Plan {
 };
 static int kv8_plan(int batch, int hq, int hkv, int head_dim, int max_pages, int split_tokens, Kv8Plan* p) {
   const int group = hq / hkv;
-  p->hkv = hkv % 8 == 0 ? 8 : hkv % 4 == 0 ? 4 : hkv % 2 == 0 ? 2 : 1;
+  p->hkv = kv8_heads_per_cta(head_dim, hkv);
   p->nt = group > 8 ? 2 : 1;
   p->slices = (group + 15) / 16;
   int sms = 0;
@@ -710,6 +736,8 @@ static int kv8_plan(int batch, int hq, int hkv, int head_dim, int max_pages, int
   if (rc) return rc;
   const int y = hkv / p->hkv * p->slices, held = kv8_ctas_per_sm(head_dim, p->hkv, p->nt) * sms;
   p->runs = y >= held ? 1 : held / y;
+  // Short rows: a run's start costs about as much as four pages, a join as much as a run.  us with runs of at least 1, 2, 4, 8 pages, 32 / 4 heads of 128: one row of
+  // 300 tokens 6.6, 6.9, 7.2, 8.7, of 1500 8.2, 7.4, 7.6, 9.0, of 6000 9.4 each; 4 rows of 300 7.6, 8.8, 9.4, 10.6, of 1000 10.5, 9.4, 9.9, 10.8.
   p->min_run = split_tokens > 0 ? split_tokens / kKvPage : 2;
   return 0;
 }
@@ -751,11 +779,13 @@ static int launch_kv8_decode(const Kv8Args& a) {
 
 template <int D, int NT>
 static int launch_kv8_heads(const Kv8Args& a) {
+  if constexpr (D == 128) {  // the only head_dim with 8 (kv8_heads_per_cta)
+    if (a.plan.hkv == 8) return launch_kv8_decode<D, 8, NT, 1, 5, kv8_ctas_per_sm(D, 8, NT)>(a);
+  }
   switch (a.plan.hkv) {
     case 1: return launch_kv8_decode<D, 1, NT, 2, 4, kv8_ctas_per_sm(D, 1, NT)>(a);
     case 2: return launch_kv8_decode<D, 2, NT, 2, D == 128 ? 3 : 4, kv8_ctas_per_sm(D, 2, NT)>(a);
-    case 4: return launch_kv8_decode<D, 4, NT, D == 128 && NT == 2 ? 1 : 2, D == 128 ? (NT == 2 ? 5 : 3) : 4, kv8_ctas_per_sm(D, 4, NT)>(a);
-    default: return launch_kv8_decode<D, 8, NT, 1, D == 128 ? 5 : 8, kv8_ctas_per_sm(D, 8, NT)>(a);
+    default: return launch_kv8_decode<D, 4, NT, D == 128 && NT == 2 ? 1 : 2, D == 128 ? (NT == 2 ? 5 : 3) : 4, kv8_ctas_per_sm(D, 4, NT)>(a);
   }
 }
 
@@ -795,6 +825,7 @@ extern "C" int b200_kv8_attn_decode(const void* q, const void* k_pool, const voi
   int rc = check_kv8("kv8_attn_decode", batch, num_q_heads, num_kv_heads, head_dim, num_blocks, max_pages_per_seq, q, k_pool, v_pool, out, scale);
   if (rc) return rc;
   B200_REQUIRE(split_tokens >= 0 && split_tokens % kKvPage == 0, "kv8_attn_decode: split_tokens %d not a multiple of %d", split_tokens, kKvPage);
+  B200_REQUIRE(static_cast<long long>(batch) * max_pages_per_seq < (1ll << 31), "kv8_attn_decode: the table has more than 2^31 entries");
   rc = check_device(nullptr);
   if (rc) return rc;
   Kv8Args a{q, k_pool, v_pool, k_scale, v_scale, block_table, ctx_lens, out, {}, batch, num_q_heads, num_kv_heads, num_blocks,
@@ -803,7 +834,6 @@ extern "C" int b200_kv8_attn_decode(const void* q, const void* k_pool, const voi
   if (rc) return rc;
   B200_REQUIRE(num_kv_heads / a.plan.hkv * a.plan.slices <= 65535 && static_cast<long long>(batch) * num_q_heads < (1ll << 31),
                "kv8_attn_decode: grid too large");
-  B200_REQUIRE(static_cast<long long>(batch) * max_pages_per_seq < (1ll << 31), "kv8_attn_decode: the table has more than 2^31 entries");
   B200_REQUIRE(reinterpret_cast<uintptr_t>(k_scale) % a.plan.hkv == 0 && reinterpret_cast<uintptr_t>(v_scale) % a.plan.hkv == 0,
                "kv8_attn_decode: scales must be %d-byte aligned", a.plan.hkv);
   a.w = carve_kv8(workspace, batch, a.plan.runs, num_q_heads, head_dim);

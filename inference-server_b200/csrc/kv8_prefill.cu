@@ -7,10 +7,10 @@
 //
 //   S = Q K^T   from the 8-bit keys as they are, kind::f8f6f4 with both operands K-major in shared memory.  A query is the sum of two
 //               e4m3 numbers, hi = the nearest and lo = what is left: bf16 has 8 bits, hi takes 4, and lo needs 4 more, so the sum is exact
-//               but for the ends of the range (rows are brought to a top of 256 to 448; a query 2^-7 of the row's largest
+//               but for the ends of the range (rows are brought to a top in (224, 448]; a query 2^-7 of the row's largest
 //               or smaller loses bits below 2^-19 of it).  Two products of twice the rate cost what one in 16 bits does, and keys need neither conversion
 //               nor room in 16 bits.
-//   P V         kind::f16: weights are f16 in TMEM (11 bits), values are converted to f16 (exactly) by two warps and
+//   P V         kind::f16: weights are f16 in TMEM (11 bits), values are converted to f16 (exactly) by four warps and
 //               stored as MN-major swizzled tiles.  A conversion serves both tiles of rows.
 //
 //   grid     (CTAs of tiles, late ones first) x splits of the keys x kv heads.  The keys are split where the tiles alone leave SMs idle; fp32
@@ -23,9 +23,13 @@
 //   warps 8-11, 12-15   first the queries of both tiles (bf16 to hi and lo, a row's top by shuffles), then the softmax of tile 0 and of tile 1,
 //            a thread per score row; the scales of a key tile's 8 pages come to each warp by its own lanes, two key tiles
 //            ahead (ids) and one (scales), and from a corner of shared memory to all lanes.  (Two threads per row, 16 softmax warps, and one
-//            predicate per key tile between them: 296 us where a thread per row took 276.)
+//            predicate per key tile between them: 296 us where a thread per row took 276, 1024 tokens behind 14336.)
 //   A CTA with one tile of rows takes every second key tile of it on the other tile's warps, with an accumulator and reference of their own,
 //   and adds the two up at the end.
+//
+// Bound by the softmax: a key tile of a CTA with two tiles of rows takes about 3800 cycles, of which the special-function units need 2048 for the
+// exponentials alone and the tensor core is busy for 1024.  32 / 4 heads of 128: 2048 tokens 52 us, 1024 behind 14336 240 us (1.04 PFLOP/s; 202 over
+// 16-bit pools, whose values need no conversion), 17 behind 14001 (64 / 4 heads) 27 us.
 //
 // Every mbarrier wait is bounded; a wait that runs out records kErrDevWaitTimeout and the thread stops waiting but keeps the loop
 // structure, so the kernel ends.
@@ -606,8 +610,10 @@ static int kv8_prefill_plan(int num_tokens, int first_pos, int hq, int hkv, Kv8P
   const int qt = kTcRows / (hq / hkv), key_tiles = (first_pos + num_tokens - 1) / kTcKeys + 1;
   p->ctas = (num_tokens + qt - 1) / qt - p->pairs;
   const long long all = static_cast<long long>(p->ctas) * hkv;
-  // as many parts as SMs are there for, of two key tiles at least: a part's set-up and its partials cost about as much
-  const int want = static_cast<int>(std::max(1ll, std::min<long long>(sms / all, (key_tiles + 1) / 2)));
+  // As many parts as SMs are there for, down to one key tile: us with parts of at least 1, 2, 4, 8 key tiles, a token behind 600 (32 / 4 heads of 128) 9.3,
+  // 10.3, 11.4, 12.2, behind 3000 10.2, 10.3, 12.4, 16.5; 64 tokens behind 2000 (8 / 2 of 64) 11.4, 12.3, 13.4, 15.4; 128 behind 1100 (8 / 1 of 128)
+  // 15.5, 14.4, 17.5, 17.2.
+  const int want = static_cast<int>(std::max(1ll, std::min<long long>(sms / all, key_tiles)));
   p->split_tiles = (key_tiles + want - 1) / want;
   p->splits = (key_tiles + p->split_tiles - 1) / p->split_tiles;
   return 0;

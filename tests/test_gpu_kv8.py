@@ -180,6 +180,14 @@ def test_append_of_strided_rows_and_slots_that_are_none(ops):
     check_append(ops, None, slots, codes, exps, torch.bfloat16, kv=(fused[:, 16:16 + H], fused[:, 16 + H:]), code=16)
 
 
+def test_append_of_a_single_row_of_any_stride(ops):
+    """One row may be a view whose row stride is no multiple of anything: it says nothing."""
+    rng = np.random.default_rng(36)
+    codes, exps = plain.random_cache(rng, 3, 2, 64)
+    kv = [torch.from_numpy(rng.standard_normal((1, 2, 64)).astype(np.float32)).to(DEV).as_strided((1, 2, 64), (stride, 64, 1)) for stride in (3, 1001)]
+    check_append(ops, None, [21], codes, exps, torch.float32, kv=kv)
+
+
 def test_wrappers_refuse(ops):
     pools = ops.kv8_pools(4, 2, 64, DEV)
     x, slots = torch.zeros(3, 2, 64, device=DEV), ints([0, 1, 2])
@@ -210,6 +218,9 @@ def test_wrappers_refuse(ops):
             call()
     with pytest.raises(TypeError):
         ops.kv8_attn_decode(q, *pools, table, slots, "0.1")
+    odd = torch.zeros(17, device=DEV, dtype=torch.uint8)[1:9].view(4, 2).view(ops.KV8_SCALE_DTYPE)
+    with pytest.raises(err, match="aligned"):
+        ops.kv8_attn_decode(q, pools[0], pools[1], odd, pools[3], table, slots, 0.1)
     with pytest.raises(err, match="dimension"):
         ops.kv_slot_map(slots, slots, table, slots, slots[:1], 4, 0)
     ops.kv8_append(x[:0], x[:0], *pools, slots[:0])

@@ -89,6 +89,7 @@ def test_decode_refuses():
         refused(call(**{name: P + 8}), "16-byte")
     for scale in (0.0, -1.0, float("inf"), float("nan")):
         refused(call(scale=scale), "scale")
+    refused(call(B=2 ** 20, width=2 ** 12), "2^31 entries")
     refused(call(split=24), "split_tokens 24")
     refused(call(split=-16), "split_tokens -16")
 
