@@ -22,14 +22,17 @@
 //            may hold NaN.  One such warp per scheduler: with two of them on two, the softmax warps beside them held up the others.
 //   warps 8-11, 12-15   first the queries of both tiles (bf16 to hi and lo, a row's top by shuffles), then the softmax of tile 0 and of tile 1,
 //            a thread per score row; the scales of a key tile's 8 pages come to each warp by its own lanes, two key tiles
-//            ahead (ids) and one (scales), and from a corner of shared memory to all lanes.  (Two threads per row, 16 softmax warps, and one
-//            predicate per key tile between them: 296 us where a thread per row took 276, 1024 tokens behind 14336.)
+//            ahead (ids) and one (scales), and from a corner of shared memory to all lanes, put there once the tile before is done, so that
+//            nothing lies between a tile's scores and their room being free again.  (Two threads per row, 16 softmax warps, and one
+//            predicate per key tile between them: 296 us where a thread per row took 276.)
 //   A CTA with one tile of rows takes every second key tile of it on the other tile's warps, with an accumulator and reference of their own,
 //   and adds the two up at the end.
 //
-// Bound by the softmax: a key tile of a CTA with two tiles of rows takes about 3800 cycles, of which the special-function units need 2048 for the
-// exponentials alone and the tensor core is busy for 1024.  32 / 4 heads of 128: 2048 tokens 52 us, 1024 behind 14336 240 us (1.04 PFLOP/s; 202 over
-// 16-bit pools, whose values need no conversion), 17 behind 14001 (64 / 4 heads) 27 us.
+// Bound by the softmax: a key tile of a CTA with two tiles of rows takes about 3650 cycles, in which each scheduler issues 2000 instructions of its
+// three busy warps, the special-function units need 2048 for the exponentials and the tensor core is busy for 1024.  Dependent steps (scores, maximum,
+// exponentials, weights) leave the rest; halves of 64 keys by turns, the next one fetched meanwhile, made the steps more and not shorter
+// (359 us), and so did a quarter of the exponentials by a polynomial (271).  32 / 4 heads of 128: 2048 tokens 51 us, 1024 behind 14336 231 us
+// (1.08 PFLOP/s; 202 over 16-bit pools, whose values need no conversion), 17 behind 14001 (64 / 4 heads) 27 us.
 //
 // Every mbarrier wait is bounded; a wait that runs out records kErrDevWaitTimeout and the thread stops waiting but keeps the loop
 // structure, so the kernel ends.
@@ -98,8 +101,9 @@ __device__ __forceinline__ float max_of_3(float a, float b, float c) {
 // One warp's quarter of a tile of values, rows row0 .. row0 + 31, to f16; those from `rows` on hold no tokens and become zero (a page may hold
 // NaN there).  A lane takes 16 bytes of a row at a time, which become two pieces of a swizzled row.  For head_dim 128 a quarter warp
 // takes the first half of one row and the second half of the next: its loads are in different banks, and so are its stores,
-// whose pieces are XORed with numbers that differ in bit 0.  The loop is short code on purpose: unrolled, half a tile took 2900 cycles, nearly all
-// of them waits for instructions, which the softmax warps' long straight-line code keeps out of the instruction cache.
+// whose pieces are XORed with numbers that differ in bit 0.  Addresses are a register and a constant: with address arithmetic in a loop 1024 tokens behind
+// 14336 took 234 us instead of 231, for these warps share their schedulers' issue slots with the softmax warps.  (By the same token, integer
+// arithmetic instead of conversions, 10 instructions for 2 per four numbers, took 250 us.)
 template <int D>
 __device__ __forceinline__ void values_to_f16(uint32_t from, uint32_t to, int row0, int rows, int lane) {
   constexpr int kPieces = D / 16, kRowsAt = 32 / kPieces;  // pieces of a row; rows that the warp takes at a time
@@ -112,24 +116,26 @@ __device__ __forceinline__ void values_to_f16(uint32_t from, uint32_t to, int ro
   const int odd = (lane >> 2) & 1;
   const int c = D == 128 ? (lane & 3) + 4 * (((lane >> 3) & 1) ^ odd) : lane & 3;
   const int lr = D == 128 ? 2 * (lane >> 4) + odd : lane >> 2;
-  const uint32_t half_off = (c >> 2) * 1024;
-  const int piece = (2 * c) & 7;
-  uint32_t src = from + (row0 + lr) * D + c * 16;
+  const uint32_t src = from + (row0 + lr) * D + c * 16;
+  const uint32_t row = to + (row0 >> 3) * kAtomGroup + (c >> 2) * 1024;
+  constexpr int kOdd = kRowsAt == 4 ? 2 : 1;  // rows of a lane within a group of 8
+  uint32_t put[kOdd][2];
+#pragma unroll
+  for (int u = 0; u < kOdd; ++u)
+#pragma unroll
+    for (int k = 0; k < 2; ++k) put[u][k] = row + swz128(lr + u * kRowsAt, ((2 * c) & 7) + k);
+  constexpr int kSteps = kTcKeys / 4 / kRowsAt;
   uint32_t w[4];
   lds_words<16>(src, w);
-#pragma unroll 2
-  for (int r = row0 + lr; r < row0 + kTcKeys / 4; r += kRowsAt) {
-    uint32_t x[4], a[8];
 #pragma unroll
-    for (int k = 0; k < 4; ++k) x[k] = w[k];
-    src += kRowsAt * D;
-    if (r + kRowsAt < row0 + kTcKeys / 4) lds_words<16>(src, w);
+  for (int r = 0; r < kSteps; ++r) {
+    uint32_t a[8];
 #pragma unroll
-    for (int k = 0; k < 4; ++k) e4m3x4_to_f16(x[k], a[2 * k], a[2 * k + 1]);
-    const uint32_t row = to + (r >> 3) * kAtomGroup + half_off;
+    for (int k = 0; k < 4; ++k) e4m3x4_to_f16(w[k], a[2 * k], a[2 * k + 1]);
+    if (r + 1 < kSteps) lds_words<16>(src + (r + 1) * kRowsAt * D, w);
 #pragma unroll
     for (int k = 0; k < 2; ++k)
-      asm volatile("st.shared.v4.b32 [%0], {%1,%2,%3,%4};" ::"r"(row + swz128(r & 7, piece + k)), "r"(a[4 * k]), "r"(a[4 * k + 1]), "r"(a[4 * k + 2]),
+      asm volatile("st.shared.v4.b32 [%0], {%1,%2,%3,%4};" ::"r"(put[r % kOdd][k] + r / kOdd * kAtomGroup), "r"(a[4 * k]), "r"(a[4 * k + 1]), "r"(a[4 * k + 2]),
                    "r"(a[4 * k + 3])
                    : "memory");
   }
@@ -427,6 +433,14 @@ kv8_attn_prefill_kernel(const __grid_constant__ CUtensorMap k_map, const uint8_t
     float m_run = -INFINITY, l_run = 0.f;
     bool alive = true, s_ready = false;
     int kbase = first_tile * kTcKeys;
+    auto put_scales = [&](int i) {
+      const int ev = scale_exponent(vb);
+      if (lane < 8) scales[(i & 1) * 8 + pg] = make_float4(power_of_two(scale_exponent(kb)), static_cast<float>(ev), power_of_two(-ev), 0.f);
+      __syncwarp();
+      ask_scales();  // of the next key tile; past the last one those of the last page
+      id = page_id(i + 2);
+    };
+    put_scales(0);
 #pragma unroll 1
     for (int i = 0; i < n_own; ++i, kbase += stride * kTcKeys) {
       if (!__all_sync(0xffffffffu, s_ready) && alive) alive = mbar_wait(sfull, i & 1, err);
@@ -440,18 +454,11 @@ kv8_attn_prefill_kernel(const __grid_constant__ CUtensorMap k_map, const uint8_t
       // while S is on its way: the pages' scales, and the next key tile's are asked for
       const float4* sc = scales + (i & 1) * 8;
       float f[8], lv[8];
-      {
-        const int ev = scale_exponent(vb);
-        if (lane < 8) scales[(i & 1) * 8 + pg] = make_float4(power_of_two(scale_exponent(kb)), static_cast<float>(ev), power_of_two(-ev), 0.f);
-        __syncwarp();
-        ask_scales();  // of the next key tile; past the last one those of the last page
-        id = page_id(i + 2);
 #pragma unroll
-        for (int p = 0; p < 8; ++p) {
-          const float2 w = *reinterpret_cast<const float2*>(sc + p);
-          f[p] = f_q * w.x;
-          lv[p] = w.y;
-        }
+      for (int p = 0; p < 8; ++p) {
+        const float2 w = *reinterpret_cast<const float2*>(sc + p);
+        f[p] = f_q * w.x;
+        lv[p] = w.y;
       }
       tmem_ld_wait();
       tc_fence_before();
@@ -523,6 +530,7 @@ kv8_attn_prefill_kernel(const __grid_constant__ CUtensorMap k_map, const uint8_t
         __syncwarp();
         if (lane == 0) mbar_arrive(pfull + 8 * half);
       }
+      put_scales(i + 1);
     }
     // ---- epilogue, once the products of the last key tiles have finished.  The warps of a CTA with one tile take half of the columns each, for
     // the sum of both accumulators.
