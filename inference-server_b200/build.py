@@ -78,7 +78,7 @@ def build_binding(force: bool = False) -> str:
     cmd = ["g++", "-O2", "-std=c++17", "-fPIC", "-shared", "-o", BINDING_PATH + ".tmp", source, "-I", INCLUDE, "-I", os.path.join(base, "include"),
            "-I", os.path.join(base, "include", "torch", "csrc", "api", "include"), "-I", sysconfig.get_path("include"),
            "-I", os.path.join(cuda, "include"), f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
-           "-L", lib, "-ltorch_python", "-ltorch", "-ltorch_cpu", "-lc10", "-lc10_cuda"]
+           "-L", lib, "-ltorch_python", "-ltorch", "-ltorch_cpu", "-ltorch_cuda", "-lc10", "-lc10_cuda"]
     res = subprocess.run(cmd, stdout=subprocess.PIPE, stderr=subprocess.STDOUT, text=True)
     if res.returncode != 0:
         raise RuntimeError(f"g++ failed on {BINDING}:\n{res.stdout}")

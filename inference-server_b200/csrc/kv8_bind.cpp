@@ -1,12 +1,12 @@
 // Native binding of the 8-bit page cache operators: the argument checks of ops.py's wrappers, the outputs, and the call of the C ABI, for
 // calls whose kernels take a few microseconds.  Through ctypes and checks in Python such a call costs the host 8 to 15 us, most of it
-// reading tensor attributes and converting 20 arguments one by one; here 4 to 8, most of it launches.
+// reading tensor attributes and converting 20 arguments one by one; here 3 to 7, most of it launches.
 //
 // The C ABI stays the only way to the kernels: ops.py hands over the addresses of its entry points (bind), so that this module
 // has no library of its own to find and follows whichever one _lib.py loaded.
 
 #include <ATen/ATen.h>
-#include <ATen/core/LegacyTypeDispatch.h>
+#include <ATen/cuda/EmptyTensor.h>
 #include <c10/cuda/CUDAFunctions.h>
 #include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/Exceptions.h>
@@ -67,6 +67,17 @@ int whole(PyObject* o) {
 int narrow(int64_t v, const char* what) {
   if (v > INT_MAX) refuse(std::string(what) + " of " + std::to_string(v) + " does not fit 32 bits");
   return static_cast<int>(v);
+}
+// An uninitialised tensor of the type and on the device of `like`, from the caching allocator without a detour through the dispatcher.
+at::Tensor fresh_tensor(at::IntArrayRef sizes, const at::Tensor& like) {
+  return at::detail::empty_cuda(sizes, like.scalar_type(), like.device(), std::nullopt);
+}
+// Numbers offset .. offset + n - 1 of a row of whole numbers, as a tensor on the same memory (six of them by way of the dispatcher: 2 us).
+at::Tensor part_of(const at::Tensor& all, int64_t offset, int64_t n) {
+  at::Tensor t = at::detail::make_tensor<c10::TensorImpl>(c10::TensorImpl::VIEW, c10::Storage(all.storage()), all.key_set(), all.dtype());
+  t.unsafeGetTensorImpl()->set_storage_offset(offset);
+  t.unsafeGetTensorImpl()->set_sizes_contiguous({n});
+  return t;
 }
 // An optional status word on `device`.
 void* status_word(PyObject* o, int device) {
@@ -166,10 +177,9 @@ PyObject* slot_map(PyObject*, PyObject* const* args, Py_ssize_t n) {
     const int B = narrow(ctx.size(0), "sequences"), R = whole(args[5]), blocks = whole(args[6]);
     const int pages = narrow(supply.numel(), "supply"), width = narrow(table.size(1), "block table");
     if (R < 0) refuse(std::to_string(R) + " rows");
-    // one allocation; every output is a part of it.  No gradient has a part in whole numbers: the dispatcher need not look for one.
-    at::AutoDispatchBelowADInplaceOrView below;
+    // one allocation; every output is a part of it
     const int64_t sizes[6] = {B, B + int64_t(1), R, R, R, 1};
-    at::Tensor all = at::empty({2 * int64_t(B) + 2 + 3 * int64_t(R)}, ctx.options());
+    at::Tensor all = fresh_tensor({2 * int64_t(B) + 2 + 3 * int64_t(R)}, ctx);
     int32_t* at[6];
     int32_t* next = all.data_ptr<int32_t>();
     for (int i = 0; i < 6; ++i) {
@@ -182,9 +192,13 @@ PyObject* slot_map(PyObject*, PyObject* const* args, Py_ssize_t n) {
                         stream_of(device));
     });
     if (rc) return failed(rc, "b200_kv_slot_map");
-    const auto parts = all.split_with_sizes(at::IntArrayRef(sizes, 6));
     PyObject* result = PyTuple_New(6);
-    for (int i = 0; i < 6; ++i) PyTuple_SET_ITEM(result, i, THPVariable_Wrap(parts[i]));
+    if (result == nullptr) throw python_error();
+    int64_t offset = 0;
+    for (int i = 0; i < 6; ++i) {
+      PyTuple_SET_ITEM(result, i, THPVariable_Wrap(part_of(all, offset, sizes[i])));
+      offset += sizes[i];
+    }
     return result;
   });
 }
@@ -232,7 +246,7 @@ PyObject* decode(PyObject*, PyObject* const* args, Py_ssize_t n) {
     const double scale = PyFloat_AsDouble(args[7]);
     if (scale == -1.0 && PyErr_Occurred()) throw python_error();
     const int split = whole(args[8]), width = narrow(x.index.size(1), "block table");
-    if (!x.out.defined()) x.out = at::empty(x.q.sizes(), x.q.options());
+    if (!x.out.defined()) x.out = fresh_tensor(x.q.sizes(), x.q);
     if (x.rows > 0) {
       const at::Tensor ws = workspace_of(args[9], p_decode_bytes, {x.rows, x.heads, c.heads, c.dim, width, split}, x.q);
       const int rc = without_gil([&] {
@@ -256,7 +270,7 @@ PyObject* prefill(PyObject*, PyObject* const* args, Py_ssize_t n) {
     const int first = whole(args[6]), width = narrow(x.index.numel(), "table row");
     const double scale = PyFloat_AsDouble(args[7]);
     if (scale == -1.0 && PyErr_Occurred()) throw python_error();
-    if (!x.out.defined()) x.out = at::empty(x.q.sizes(), x.q.options());
+    if (!x.out.defined()) x.out = fresh_tensor(x.q.sizes(), x.q);
     if (x.rows > 0) {
       const at::Tensor ws = workspace_of(args[8], prefill_bytes, {x.rows, first, x.heads, c.heads, c.dim, 0}, x.q);
       const int rc = without_gil([&] {
