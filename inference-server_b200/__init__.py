@@ -6,7 +6,7 @@ The directory name contains a hyphen, so import it with
 - ``_lib``      ctypes binding of ``libb200decode.so`` (the C-ABI in
                 ``include/b200_decode.h``); fails loudly if the library is absent.
 - ``ops``       operator wrappers on torch CUDA tensors (paged attention, KV
-                append, MoE route/permute/quant/GEMM/combine).
+                append, 8-bit page cache, MoE route/permute/quant/GEMM/combine).
 - ``quant``     load-time e4m3 128x128 block quantisation of expert weights.
 - ``engine``    ``PagedEngine`` (step, graphs, prompt passes) and the Qwen3-MoE
                 ``DecodeEngine`` on it.
