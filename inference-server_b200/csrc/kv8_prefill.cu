@@ -31,7 +31,7 @@
 // Bound by the softmax: a key tile of a CTA with two tiles of rows takes about 3650 cycles, in which each scheduler issues 2000 instructions of its
 // three busy warps, the special-function units need 2048 for the exponentials and the tensor core is busy for 1024.  Dependent steps (scores, maximum,
 // exponentials, weights) leave the rest; halves of 64 keys by turns, the next one fetched meanwhile, made the steps more and not shorter
-// (359 us), and so did a quarter of the exponentials by a polynomial (271).  32 / 4 heads of 128: 2048 tokens 51 us, 1024 behind 14336 231 us
+// (359 us), and so did a quarter of the exponentials by a polynomial (271).  32 / 4 heads of 128: 2048 tokens 50 us, 1024 behind 14336 231 us
 // (1.08 PFLOP/s; 202 over 16-bit pools, whose values need no conversion), 17 behind 14001 (64 / 4 heads) 27 us.
 //
 // Every mbarrier wait is bounded; a wait that runs out records kErrDevWaitTimeout and the thread stops waiting but keeps the loop
@@ -262,17 +262,18 @@ kv8_attn_prefill_kernel(const __grid_constant__ CUtensorMap k_map, const uint8_t
       // ------------------------------------------------- S = Q K^T ------
       if (elect_one()) {
         constexpr uint32_t idesc_s = umma_idesc_f8(kTcRows, kTcKeys);
-        bool alive = mbar_wait(bar_q, 0, err);
+        bool alive = true;
         uint32_t n = 0, st = 0, phase = 0;
 #pragma unroll 1
         for (int j = 0; j < n_tiles && alive; ++j) {
           alive = mbar_wait(bar_kfull + 8 * st, phase, err);
+          if (j == 0 && alive) alive = mbar_wait(bar_q, 0, err);
           const uint64_t b0 = desc_k8<D>(base + Cfg::kK + st * Cfg::kTile8);
 #pragma unroll 1
           for (int t = 0; t < 2; ++t) {
             // none of this tile's rows sees these keys, or they are the other accumulator's
             if (own == 2 ? j >= (t ? n_of[1] : n_of[0]) : (j & 1) != t) continue;
-            if (alive) alive = mbar_wait(bar_sempty, (n & 1) ^ 1, err);
+            if (n > 0 && alive) alive = mbar_wait(bar_sempty, (n & 1) ^ 1, err);  // nothing has been written yet at first
             if (!alive) break;
             ++n;
             tc_fence_after();

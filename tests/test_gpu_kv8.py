@@ -380,6 +380,38 @@ def test_decode_pages_past_32_bits_of_bytes(ops):
     assert torch.equal(got, ops.kv8_attn_decode(q, *small, ints([[0, 1, 2]]), ints([41]), 0.1))
     check_attn(got, q.cpu(), *(f(c) for c in (small[0], small[2], small[1], small[3]) for f in [lambda c: c.view(torch.uint8).cpu().numpy()
                if c.dtype == plain.E4M3 else c.view(torch.uint8).cpu().numpy().astype(int) - 127]), np.array([[0, 1, 2]]), [41], 0.1)
+    q = torch.randn(5, 32, D, device=DEV).bfloat16()
+    assert torch.equal(ops.kv8_attn_prefill(q, *cache, table[0], 36, 0.1), ops.kv8_attn_prefill(q, *small, ints([0, 1, 2]), 36, 0.1))
+
+
+@pytest.mark.parametrize("Hq,H,D", [(32, 4, 128), (5, 1, 64)])
+def test_pages_that_rows_share_or_name_twice(ops, Hq, H, D):
+    """Rows with common pages ahead of their own, a row that is another one again, a row that names a page three times."""
+    rng = np.random.default_rng(37)
+    q, kc, ke, vc, ve, table = attn_case(rng, [160, 40, 40, 64], Hq, H, D)
+    table[1, :2], table[2], table[3, :4] = table[0, :2], table[1], table[0, [5, 5, 2, 5]]
+    lens = [160, 40, 40, 64]
+    out = run_decode(ops, q, kc, ke, vc, ve, table, lens, 0.1)
+    check_attn(out, q, kc, ke, vc, ve, table, lens, 0.1)
+    q = torch.from_numpy(rng.standard_normal((20, Hq, D)).astype(np.float32)).bfloat16()
+    got = ops.kv8_attn_prefill(q.to(DEV), plain.pool_of(kc), plain.pool_of(vc), plain.scale_of(ke), plain.scale_of(ve), ints(table[3].tolist()), 44, 0.1)
+    check_attn(got, q, kc, ke, vc, ve, [table[3]] * 20, range(45, 65), 0.1, 2.0 ** -10 / 224)
+
+
+def test_attention_in_place(ops):
+    """The output may be the queries' own memory: a query is read before anything is written over it."""
+    rng = np.random.default_rng(38)
+    lens = [700, 0, 33, 1, 2500]
+    q, kc, ke, vc, ve, table = attn_case(rng, lens, 12, 4, 128)
+    cache = [plain.pool_of(kc), plain.pool_of(vc), plain.scale_of(ke), plain.scale_of(ve)]
+    table, lens = torch.from_numpy(table).to(DEV), ints(lens)
+    want, q = ops.kv8_attn_decode(q.to(DEV), *cache, table, lens, 0.1), q.to(DEV)
+    assert ops.kv8_attn_decode(q, *cache, table, lens, 0.1, out=q) is q and torch.equal(q, want)
+    for n, first in ((300, 400), (9, 2400)):
+        row = table[0 if first == 400 else 4]
+        q = torch.from_numpy(rng.standard_normal((n, 12, 128)).astype(np.float32)).to(DEV, torch.bfloat16)
+        want = ops.kv8_attn_prefill(q, *cache, row, first, 0.1)
+        assert torch.equal(ops.kv8_attn_prefill(q, *cache, row, first, 0.1, out=q), want)
 
 
 # -------------------------------------------------------------------- prompt
