@@ -272,7 +272,8 @@ kv8_attn_decode_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_c
         return id;
       };
       int next_ids = page_id(lane), ids = 0;
-      alive = mbar_wait_warp(bar_q + 8, (part & 1) ^ 1, err);
+      // (rooms that are free from the start are not waited for: 7.4 -> 7.05 us for one row of 777 tokens)
+      if (part > 0) alive = mbar_wait_warp(bar_q + 8, (part & 1) ^ 1, err);
       if (!alive) break;
       const uint32_t q_bytes = heads * D * 2;
       if (lane == 0) mbar_arrive_expect_tx(bar_q, HKV * q_bytes);
@@ -292,7 +293,7 @@ kv8_attn_decode_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_c
         }
         const int id = __shfl_sync(0xffffffffu, ids, (p + lp) & 31);
         const int slot = stage % STAGES, pages = min(PPS, n - p);
-        alive = mbar_wait_warp(bars + 8 * (STAGES + slot), (stage / STAGES & 1) ^ 1, err);
+        if (stage >= STAGES) alive = mbar_wait_warp(bars + 8 * (STAGES + slot), (stage / STAGES & 1) ^ 1, err);
         if (!alive) break;
         // The copies may end before the stage's bytes are announced: its phase cannot, without the arrival that comes with them.
         // So they do not wait for the scales.
