@@ -247,11 +247,12 @@ int b200_kv_append(const void* k_new, const void* v_new, void* k_pool, void* v_p
  * b200_kv8_attn_decode: softmax(q K^T * scale) V, one query row per sequence over its pages.  q, out [batch, num_q_heads, head_dim] bf16, any
  * number of query heads per kv head.  scale > 0.  The pages of all rows are cut into equal runs, one per CTA.  workspace:
  * b200_kv8_attn_workspace_bytes bytes, 16-byte aligned, starting with the status word; calls that share it must not overlap.  split_tokens: tokens of a run at least, a multiple of 16; 0: the library's choice, the same for
- * both calls.  A row without tokens is zero.  Pages behind a row's last token are not read, and what the last page
+ * both calls.  A weight times its page's value scale is rounded to 11 bits, but to no finer a step than 2^-30 of the row's largest such product:
+ * next to a page whose scale is 2^20 times larger, values lose precision.  A row without tokens is zero.  Pages behind a row's last token are not read, and what the last page
  * holds behind it does not matter, NaN included.
  *
  * b200_kv8_attn_prefill: causal attention of num_tokens consecutive tokens of one sequence, at positions first_position .., whose keys
- * and values are in their slots.  q, out [num_tokens, num_q_heads, head_dim] bf16, at most 128 query heads per kv head.  workspace:
+ * and values are in their slots.  q, out [num_tokens, num_q_heads, head_dim] bf16, at most 128 query heads per kv head, the arithmetic of decode.  workspace:
  * b200_kv8_attn_prefill_workspace_bytes bytes (the same rules).  A NaN value of a token reaches the rows of up to 127 tokens before it.
  */
 int b200_kv_slot_map(const int32_t* ctx_lens, const int32_t* new_lens, int32_t* block_table, const int32_t* supply,

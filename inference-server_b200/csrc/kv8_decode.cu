@@ -12,7 +12,7 @@
 //
 // Bound by memory: 2 D bytes per token and kv head, one scale byte per 16 D of them.  256 rows of 512 to 4096 tokens, 32 / 4 heads of
 // 128, 592 MB: 100 us at 5.9 TB/s and 7 for the join, 106 in a row of calls.  The rest is a chain of 8 to 10 us that no call is without - lengths,
-// table, the first pages, the last pages' arithmetic, partials -: one row of 777 tokens 7.2 us, 131001 tokens 31.6 us (134 MB).
+// table, the first pages, the last pages' arithmetic, partials -: one row of 777 tokens 7.1 us, 131001 tokens 31.7 us (134 MB).
 //
 //   work   The pages of all rows, one row after the other, are cut into equal runs, one per CTA (kv8_ctas_per_sm), wherever
 //          that falls in a row: every CTA streams the same number of bytes without a break, whatever the rows' lengths, and there are no

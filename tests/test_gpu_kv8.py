@@ -298,7 +298,7 @@ def test_decode_scale_bytes_beyond_the_range(ops):
     check_attn(run_decode(ops, q, kc, ke, vc, ve, table, lens, 1e-12), q, kc, ke, vc, ve, table, lens, 1e-12)
 
 
-@pytest.mark.parametrize("B,top", [(1, 20011), (3, 6000), (70, 900), (300, 130)])
+@pytest.mark.parametrize("B,top", [(1, 20011), (3, 6000), (70, 900), (300, 130), (5000, 40)])
 def test_decode_batches(ops, B, top):
     rng = np.random.default_rng(B)
     lens = [int(x) for x in rng.integers(0, top + 1, B)]
@@ -448,7 +448,7 @@ def test_prefill_every_row(ops, Hq, H, D, n, first):
 
 
 @pytest.mark.parametrize("Hq,H,D,n,first", [(32, 4, 128, 1500, 100), (32, 4, 128, 2048, 0), (8, 8, 128, 700, 900), (16, 2, 64, 2000, 3000), (64, 4, 128, 40, 9001),
-                                            (8, 2, 64, 3, 12000)])
+                                            (8, 2, 64, 3, 12000), (16, 4, 128, 20000, 0), (128, 1, 64, 700, 5)])
 def test_prefill_long(ops, Hq, H, D, n, first):
     run_prefill(ops, n, first, Hq, H, D, seed=n, rows=[0, 1, 127, 128, n // 3, n // 2, n - 17, n - 1])
 
