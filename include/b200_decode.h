@@ -238,22 +238,24 @@ int b200_kv_append(const void* k_new, const void* v_new, void* k_pool, void* v_p
  * than 2^31 tokens in the table.  lens and supply_used_out must not be inputs.
  *
  * b200_kv8_append: rows of keys and values (bf16 or fp32; [num_rows, num_kv_heads, head_dim] with a row stride in elements) into
- * their slots; a negative slot is no slot.  Rows that go to one page stand side by side, in rising order and without gaps, and the page is no other
- * sequence's: two groups of rows of one page in a call race for its scale.  Naming a slot twice in a row keeps the last.
+ * their slots; a negative slot is no slot.  Rows that go to one page stand side by side, in rising order and without gaps, and the page is no
+ * other sequence's: two groups of rows of one page in a call race for its scale.  Naming a slot twice in a row keeps the last.
  * The scale of a page becomes the smallest 2^e with largest finite magnitude <= 448 * 2^e; that of a page whose first slot is not
  * among the rows never falls, and where it grows, the rows ahead of the new ones are rounded again.  Slots behind the new ones
  * are left as they were.  Numbers are rounded to nearest even; infinities and NaN become NaN.
  *
  * b200_kv8_attn_decode: softmax(q K^T * scale) V, one query row per sequence over its pages.  q, out [batch, num_q_heads, head_dim] bf16, any
- * number of query heads per kv head.  scale > 0.  The pages of all rows are cut into equal runs, one per CTA.  workspace:
- * b200_kv8_attn_workspace_bytes bytes, 16-byte aligned, starting with the status word; calls that share it must not overlap.  split_tokens: tokens of a run at least, a multiple of 16; 0: the library's choice, the same for
- * both calls.  A weight times its page's value scale is rounded to 11 bits, but to no finer a step than 2^-30 of the row's largest such product:
- * next to a page whose scale is 2^20 times larger, values lose precision.  A row without tokens is zero.  Pages behind a row's last token are not read, and what the last page
- * holds behind it does not matter, NaN included.
+ * number of query heads per kv head.  scale > 0.  The pages of all rows are cut into equal runs, one per CTA.
+ *   workspace     b200_kv8_attn_workspace_bytes bytes, 16-byte aligned, starting with the status word; calls that share it must not overlap
+ *   split_tokens  tokens of a run at least, a multiple of 16; 0: the library's choice; the same for both calls
+ * A weight times its page's value scale is rounded to 11 bits, but to no finer a step than 2^-30 of the row's largest such product: next to a
+ * page whose scale is 2^20 times larger, values lose precision.  A row without tokens is zero.  Pages behind a row's last token are not read,
+ * and what the last page holds behind it does not matter, NaN included.
  *
- * b200_kv8_attn_prefill: causal attention of num_tokens consecutive tokens of one sequence, at positions first_position .., whose keys
- * and values are in their slots.  q, out [num_tokens, num_q_heads, head_dim] bf16, at most 128 query heads per kv head, the arithmetic of decode.  workspace:
- * b200_kv8_attn_prefill_workspace_bytes bytes (the same rules).  A NaN value of a token reaches the rows of up to 127 tokens before it.
+ * b200_kv8_attn_prefill: causal attention of num_tokens consecutive tokens of one sequence, at positions first_position .., whose keys and
+ * values are in their slots.  q, out [num_tokens, num_q_heads, head_dim] bf16, at most 128 query heads per kv head, the arithmetic of decode.
+ * workspace: b200_kv8_attn_prefill_workspace_bytes bytes (the same rules).  A NaN value of a token reaches the rows of up to 127 tokens ahead
+ * of it.
  */
 int b200_kv_slot_map(const int32_t* ctx_lens, const int32_t* new_lens, int32_t* block_table, const int32_t* supply,
                      const int32_t* supply_used, int supply_len, int32_t* lens, int32_t* row_start, int32_t* row_seq,

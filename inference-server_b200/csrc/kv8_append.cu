@@ -326,8 +326,8 @@ static int launch_append(const void* k_new, const void* v_new, long long ks, lon
   int sms = 0;
   int rc = device_sm_count(&sms);
   if (rc) return rc;
-  // The fewest rows per CTA with which the grid fits the GPU at once.  us with 4, 8 and 16 CTAs per SM in its place: 8970 rows of 4 heads of 128 in bf16 9.6, 11.9,
-  // 12.8; 61 short prompts of 2 heads of 64 in fp32 3.5, 4.1, 4.1.
+  // The fewest rows per CTA with which the grid fits the GPU at once.  us with 4, 8 and 16 CTAs per SM in its place: 8970 rows of 4 heads
+  // of 128 in bf16 9.6, 11.9, 12.8; 61 short prompts of 2 heads of 64 in fp32 3.5, 4.1, 4.1.
   int window = 1;
   while (window < kAppendMaxWindow && (rows + window - 1) / window > 4 * sms) window *= 2;
   B200_CUDA(launch_overlapped(kv8_append_kernel<T, D>, dim3((rows + window - 1) / window), dim3(kAppendWarps * 32), 0, st,

@@ -64,10 +64,10 @@ __device__ __forceinline__ uint32_t transpose_8x8(uint32_t x) {
 }
 
 // CTAs that an SM holds: as many as leave each enough of the ring, and of the registers, to keep its share of the memory busy.  More of
-// them cut more rows.  us for 128 rows of 512 to 4096 tokens: head_dim 128, 4 kv heads (256 rows) one 126, two 106; 2 kv heads of 8 queries two 39.8, three
-// 33.6, four 35.1, of 16 two 47.5, three 42.5; 1 kv head of 8 queries four 20.6, six 19.5, of 16 four 31.5, five 31.0.  head_dim 64, 4 kv heads of 8 two
-// 36.6, three 34.1, of 16 two 40.1, three 39.0; 2 kv heads of 8 four 22.5, five 21.1, of 16 three 27.7, four 24.2; 1 kv head of 8 four
-// 17.0, six 15.5, eight 16.1, of 16 five 21.9, six 19.9.
+// them cut more rows.  us for 128 rows of 512 to 4096 tokens: head_dim 128, 4 kv heads (256 rows) one 126, two 106; 2 kv heads of 8 queries
+// two 39.8, three 33.6, four 35.1, of 16 two 47.5, three 42.5; 1 kv head of 8 queries four 20.6, six 19.5, of 16 four 31.5, five 31.0.
+// head_dim 64, 4 kv heads of 8 two 36.6, three 34.1, of 16 two 40.1, three 39.0; 2 kv heads of 8 four 22.5, five 21.1, of 16 three 27.7,
+// four 24.2; 1 kv head of 8 four 17.0, six 15.5, eight 16.1, of 16 five 21.9, six 19.9.
 constexpr int kv8_ctas_per_sm(int head_dim, int hkv, int nt) {
   if (head_dim == 64) return hkv == 1 ? 6 : hkv == 2 ? (nt == 1 ? 5 : 4) : 3;
   return hkv == 1 ? (nt == 1 ? 6 : 5) : hkv == 2 ? 3 : hkv == 4 ? 2 : 1;
@@ -704,8 +704,8 @@ kv8_attn_join_wide_kernel(const float* __restrict__ part_o, const float2* __rest
   out[static_cast<size_t>(row) * D + blockIdx.y * 32 + lane] = __float2bfloat16(num / sum);
 }
 
-// `expected`: parts that a row is likely to have.  The wide form where they are many and the rows few: us for a whole call, narrow and wide, 528 rows
-// of 18 parts 12.3, 10.3; 1088 rows of 11 parts 27.7, 29.7.
+// `expected`: parts that a row is likely to have.  The wide form where they are many and the rows few: us for a whole call, narrow and
+// wide, 528 rows of 18 parts 12.3, 10.3; 1088 rows of 11 parts 27.7, 29.7.
 template <int D>
 static int launch_join(const float* o, const float2* ml, const int2* rows, void* out, int hq, int num_rows, int parts, int expected,
                        cudaStream_t st) {
@@ -737,8 +737,9 @@ static int kv8_plan(int batch, int hq, int hkv, int head_dim, int max_pages, int
   if (rc) return rc;
   const int y = hkv / p->hkv * p->slices, held = kv8_ctas_per_sm(head_dim, p->hkv, p->nt) * sms;
   p->runs = y >= held ? 1 : held / y;
-  // Short rows: a run's start costs about as much as four pages, a join as much as a run.  us with runs of at least 1, 2, 4, 8 pages, 32 / 4 heads of 128: one row of
-  // 300 tokens 6.6, 6.9, 7.2, 8.7, of 1500 8.2, 7.4, 7.6, 9.0, of 6000 9.4 each; 4 rows of 300 7.6, 8.8, 9.4, 10.6, of 1000 10.5, 9.4, 9.9, 10.8.
+  // Short rows: a run's start costs about as much as four pages, a join as much as a run.  us with runs of at least 1, 2, 4, 8 pages, 32 /
+  // 4 heads of 128: one row of 300 tokens 6.6, 6.9, 7.2, 8.7, of 1500 8.2, 7.4, 7.6, 9.0, of 6000 9.4 each; 4 rows of 300 7.6, 8.8, 9.4,
+  // 10.6, of 1000 10.5, 9.4, 9.9, 10.8.
   p->min_run = split_tokens > 0 ? split_tokens / kKvPage : 2;
   return 0;
 }

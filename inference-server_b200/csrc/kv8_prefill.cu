@@ -8,8 +8,8 @@
 //   S = Q K^T   from the 8-bit keys as they are, kind::f8f6f4 with both operands K-major in shared memory.  A query is the sum of two
 //               e4m3 numbers, hi = the nearest and lo = what is left: bf16 has 8 bits, hi takes 4, and lo needs 4 more, so the sum is exact
 //               but for the ends of the range (rows are brought to a top in (224, 448]; a query 2^-7 of the row's largest
-//               or smaller loses bits below 2^-19 of it).  Two products of twice the rate cost what one in 16 bits does, and keys need neither conversion
-//               nor room in 16 bits.
+//               or smaller loses bits below 2^-19 of it).  Two products of twice the rate cost what one in 16 bits does, and keys need
+//               neither conversion nor room in 16 bits.
 //   P V         kind::f16: weights are f16 in TMEM (11 bits), values are converted to f16 (exactly) by four warps and
 //               stored as MN-major swizzled tiles.  A conversion serves both tiles of rows.
 //
@@ -29,10 +29,10 @@
 //   and adds the two up at the end.
 //
 // Bound by the softmax: a key tile of a CTA with two tiles of rows takes about 3650 cycles, in which each scheduler issues 2000 instructions of its
-// three busy warps, the special-function units need 2048 for the exponentials and the tensor core is busy for 1024.  Dependent steps (scores, maximum,
-// exponentials, weights) leave the rest; halves of 64 keys by turns, the next one fetched meanwhile, made the steps more and not shorter
-// (359 us), and so did a quarter of the exponentials by a polynomial (271).  32 / 4 heads of 128: 2048 tokens 50 us, 1024 behind 14336 231 us
-// (1.08 PFLOP/s; 202 over 16-bit pools, whose values need no conversion), 17 behind 14001 (64 / 4 heads) 27 us.
+// three busy warps, the special-function units need 2048 for the exponentials and the tensor core is busy for 1024.  Dependent steps
+// (scores, maximum, exponentials, weights) leave the rest; halves of 64 keys by turns, the next one fetched meanwhile, made the steps more
+// and not shorter (359 us), and so did a quarter of the exponentials by a polynomial (271).  32 / 4 heads of 128: 2048 tokens 50 us, 1024
+// behind 14336 231 us (1.08 PFLOP/s; 202 over 16-bit pools, whose values need no conversion), 17 behind 14001 (64 / 4 heads) 27 us.
 //
 // Every mbarrier wait is bounded; a wait that runs out records kErrDevWaitTimeout and the thread stops waiting but keeps the loop
 // structure, so the kernel ends.
@@ -101,9 +101,9 @@ __device__ __forceinline__ float max_of_3(float a, float b, float c) {
 // One warp's quarter of a tile of values, rows row0 .. row0 + 31, to f16; those from `rows` on hold no tokens and become zero (a page may hold
 // NaN there).  A lane takes 16 bytes of a row at a time, which become two pieces of a swizzled row.  For head_dim 128 a quarter warp
 // takes the first half of one row and the second half of the next: its loads are in different banks, and so are its stores,
-// whose pieces are XORed with numbers that differ in bit 0.  Addresses are a register and a constant: with address arithmetic in a loop 1024 tokens behind
-// 14336 took 234 us instead of 231, for these warps share their schedulers' issue slots with the softmax warps.  (By the same token, integer
-// arithmetic instead of conversions, 10 instructions for 2 per four numbers, took 250 us.)
+// whose pieces are XORed with numbers that differ in bit 0.  Addresses are a register and a constant: with address arithmetic in a loop
+// 1024 tokens behind 14336 took 234 us instead of 231, for these warps share their schedulers' issue slots with the softmax warps.  (By the
+// same token, integer arithmetic instead of conversions, 10 instructions for 2 per four numbers, took 250 us.)
 template <int D>
 __device__ __forceinline__ void values_to_f16(uint32_t from, uint32_t to, int row0, int rows, int lane) {
   constexpr int kPieces = D / 16, kRowsAt = 32 / kPieces;  // pieces of a row; rows that the warp takes at a time
@@ -619,9 +619,9 @@ static int kv8_prefill_plan(int num_tokens, int first_pos, int hq, int hkv, Kv8P
   const int qt = kTcRows / (hq / hkv), key_tiles = (first_pos + num_tokens - 1) / kTcKeys + 1;
   p->ctas = (num_tokens + qt - 1) / qt - p->pairs;
   const long long all = static_cast<long long>(p->ctas) * hkv;
-  // As many parts as SMs are there for, down to one key tile: us with parts of at least 1, 2, 4, 8 key tiles, a token behind 600 (32 / 4 heads of 128) 9.3,
-  // 10.3, 11.4, 12.2, behind 3000 10.2, 10.3, 12.4, 16.5; 64 tokens behind 2000 (8 / 2 of 64) 11.4, 12.3, 13.4, 15.4; 128 behind 1100 (8 / 1 of 128)
-  // 15.5, 14.4, 17.5, 17.2.
+  // As many parts as SMs are there for, down to one key tile: us with parts of at least 1, 2, 4, 8 key tiles, a token behind 600 (32 / 4
+  // heads of 128) 9.3, 10.3, 11.4, 12.2, behind 3000 10.2, 10.3, 12.4, 16.5; 64 tokens behind 2000 (8 / 2 of 64) 11.4, 12.3, 13.4, 15.4;
+  // 128 behind 1100 (8 / 1 of 128) 15.5, 14.4, 17.5, 17.2.
   const int want = static_cast<int>(std::max(1ll, std::min<long long>(sms / all, key_tiles)));
   p->split_tiles = (key_tiles + want - 1) / want;
   p->splits = (key_tiles + p->split_tiles - 1) / p->split_tiles;
