@@ -7,8 +7,9 @@
 // p_t = 2^(s_t + ev - m), where m follows the maximum of s_t + ev, so the largest weight sees the largest product and not the largest
 // score.  The denominator is sum_t p_t 2^-ev.  Everything that has a scale in it is an fp32 exponent; e4m3 numbers become f16 exactly, and
 // weights are f16, whose 11 bits leave them an eighth of the error of bf16.  Weights are taken so that the largest is between 2^6 and
-// 2^14; those below 2^-14 lose bits.  Queries are multiplied by a power of two that brings the largest of a kv group to 2^14 and become
-// f16: what loses bits is 2^-28 of the largest.  Sums are fp32.  With |ev| <= 32 the sums p_t 2^-ev stay below 2^14 * 2^32 * tokens.
+// 2^14; those below 2^-14 lose bits.  A head's query is multiplied by a power of two that brings its largest number to 2^14 and becomes
+// f16: what loses bits is 2^-28 of the largest.  (One power for a kv group would let a head that is 2^30 times larger than its neighbours, or
+// not finite, take their bits.)  Sums are fp32.  With |ev| <= 32 the sums p_t 2^-ev stay below 2^14 * 2^32 * tokens.
 //
 // Bound by memory: 2 D bytes per token and kv head, one scale byte per 16 D of them.  256 rows of 512 to 4096 tokens, 32 / 4 heads of
 // 128, 592 MB: 100 us at 5.9 TB/s and 7 for the join, 106 in a row of calls.  The rest is a chain of 8 to 10 us that no call is without - lengths,
@@ -47,7 +48,7 @@ namespace b200 {
 
 constexpr float kKv8RefSlack = 8.f;    // a score may pass its reference by 2^8 before the reference moves
 constexpr float kKv8Lift = 6.f;        // weights are taken times 2^6: at most 2^14 in f16
-constexpr int kKv8QueryTop = 14;       // exponent that the largest query of a kv group is brought to
+constexpr int kKv8QueryTop = 14;       // exponent that the largest number of a head's query is brought to
 
 // D(16x8, f32) += A(16x16, f16, row) * B(16x8, f16, col)
 __device__ __forceinline__ void mma_f16_16816(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
@@ -343,34 +344,46 @@ kv8_attn_decode_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_c
     const size_t row0 = static_cast<size_t>(walk.row) * num_q_heads + kvh * group + q0;
     // Q^T fragments, f16.  k-step 4 c + w of thread tq: elements 64 c + 16 tq + 4 w + 0..3 of head_dim (16 tq + 4 w + .. for D = 64).
     uint32_t qb[NT][KS][2];
-    float f_q;  // what a score is to be multiplied by, but for the page's scale
+    // What scores of heads 8 t + 2 tq and + 1 are to be multiplied by, but for the page's scale.  One tile: two factors.  Two tiles, where four
+    // registers across the loop made the compiler spill others (16 heads on one 168 against 162 us): the two powers of two of a tile in the halves
+    // of a register, taken apart where they are used.  (One tile in that form: a row of 777 tokens 6.8 against 6.3 us.)
+    uint32_t back[2];
+    auto factor = [&](int t, int k) { return __uint_as_float(NT == 1 ? back[k] : k ? back[t] & 0xffff0000u : back[t] << 16); };
     {
       if (alive) alive = mbar_wait_warp(bar_q, part & 1, err);
-      uint32_t top = 0;
+      uint32_t top[NT];  // largest magnitudes of head 8 t + g so far, two side by side
 #pragma unroll
-      for (int t = 0; t < NT; ++t)
+      for (int t = 0; t < NT; ++t) {
+        top[t] = 0;
 #pragma unroll
         for (int ks = 0; ks < KS; ++ks) {
           qb[t][ks][0] = qb[t][ks][1] = 0u;
           if (8 * t + g < heads)
             lds_words<8>(q_sm + ((warp * heads + 8 * t + g) * D + (ks >> 2) * 64 + tq * 16 + (ks & 3) * 4) * 2, qb[t][ks]);
-          const uint32_t a = qb[t][ks][0] & 0x7fff7fffu, c = qb[t][ks][1] & 0x7fff7fffu;
-          top = max(top, max(max(a >> 16, a & 0xffffu), max(c >> 16, c & 0xffffu)));
+          top[t] = __vmaxu2(top[t], __vmaxu2(qb[t][ks][0] & 0x7fff7fffu, qb[t][ks][1] & 0x7fff7fffu));
         }
+      }
       __syncwarp();
       if (lane == 0) mbar_arrive(bar_q + 8);
-      top = __reduce_max_sync(0xffffffffu, top);
-      // bf16 and fp32 have the same exponents, -127 (zeros) to 128 (infinities); tiny queries may stay below the top
-      const int shift = min(kKv8QueryTop - (static_cast<int>(top >> 7) - 127), 100);
-      const float by = power_of_two(shift);
-      f_q = scale_log2 * power_of_two(-shift);
 #pragma unroll
-      for (int t = 0; t < NT; ++t)
+      for (int t = 0; t < NT; ++t) {
+        uint32_t m2 = max(top[t] >> 16, top[t] & 0xffffu);  // the head's four lanes share it
+        m2 = max(m2, __shfl_xor_sync(0xffffffffu, m2, 1));
+        m2 = max(m2, __shfl_xor_sync(0xffffffffu, m2, 2));
+        // bf16 and fp32 have the same exponents, -127 (zeros) to 128 (infinities); tiny queries may stay below the top.  Scores of a head that
+        // is not finite are all infinite or NaN, so its softmax is NaN.
+        const int shift = min(kKv8QueryTop - (static_cast<int>(m2 >> 7) - 127), 100);
+        const float by = m2 < 0x7f80u ? power_of_two(shift) : NAN;
+        const uint32_t mine = __float_as_uint((NT == 1 ? scale_log2 : 1.f) * power_of_two(-shift));
+        const uint32_t a = __shfl_sync(0xffffffffu, mine, 8 * tq), b = __shfl_sync(0xffffffffu, mine, 8 * tq + 4);  // of lanes whose g is 2 tq (+ 1)
+        if (NT == 1) back[0] = a, back[1] = b;
+        else back[t] = a >> 16 | b;
 #pragma unroll
         for (int ks = 0; ks < KS; ++ks)
 #pragma unroll
           for (int k = 0; k < 2; ++k)
             qb[t][ks][k] = pack_f16x2(__uint_as_float(qb[t][ks][k] << 16) * by, __uint_as_float(qb[t][ks][k] & 0xffff0000u) * by);
+      }
     }
 
     float o[NT][D / 16][4];  // O^T: rows g * VB + 2 j (+ 1), columns: heads 2 tq, 2 tq + 1
@@ -418,14 +431,17 @@ kv8_attn_decode_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_c
         int kbyte, vbyte;
         asm volatile("ld.shared.u8 %0, [%1];" : "=r"(kbyte) : "r"(scale_sm + (slot * PPS + u) * 16 + warp));
         asm volatile("ld.shared.u8 %0, [%1];" : "=r"(vbyte) : "r"(scale_sm + (slot * PPS + u) * 16 + 8 + warp));
-        const float f = f_q * power_of_two(scale_exponent(kbyte));
+        const float f = (NT == 1 ? 1.f : scale_log2) * power_of_two(scale_exponent(kbyte));
         ev[u] = scale_exponent(vbyte);
         const float lv = static_cast<float>(ev[u]);
         const int here = left - u * kKvPage;  // tokens of this page, if fewer than 16
 #pragma unroll
-        for (int t = 0; t < NT; ++t)
+        for (int t = 0; t < NT; ++t) {
+          if constexpr (NT == 2) asm volatile("" : "+r"(back[t]));  // not ahead of the loop
+          const float f_t[2] = {factor(t, 0) * f, factor(t, 1) * f};
 #pragma unroll
-          for (int k = 0; k < 4; ++k) s[u][t][k] = tok + (k >> 1) * 8 < here ? fmaf(acc[t][k], f, lv) : -INFINITY;
+          for (int k = 0; k < 4; ++k) s[u][t][k] = tok + (k >> 1) * 8 < here ? fmaf(acc[t][k], f_t[k & 1], lv) : -INFINITY;
+        }
         if (here < kKvPage) {
           // the last page: what lies behind the last token may be NaN, which a weight of zero does not undo
           const uint32_t vb = kb + Cfg::kPageBytes;

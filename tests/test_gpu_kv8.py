@@ -643,3 +643,34 @@ def test_two_calls_at_once_and_again(ops):
     torch.cuda.synchronize()
     for i in range(2):
         assert all(torch.equal(o, alone[i]) for o in outs[i])
+
+
+@pytest.mark.parametrize("Hq,H,D", [(32, 4, 128), (64, 4, 128), (16, 2, 64), (7, 1, 128), (40, 1, 128), (16, 8, 64), (64, 8, 128)])
+@pytest.mark.parametrize("lens", [[1, 40, 531, 16], [9000], [700] * 40])
+def test_decode_query_heads_that_are_not_finite(ops, Hq, H, D, lens):
+    """A NaN or an infinity in the query of one head of each group: that head is NaN, all others have their own weights.  (Their bits may change: the
+    heads of a group move their references together, and a weight below 2^-14 is rounded to the reference's steps, which the tolerance counts.)"""
+    rng = np.random.default_rng(40)
+    q, kc, ke, vc, ve, table = attn_case(rng, lens, Hq, H, D)
+    clean = run_decode(ops, q, kc, ke, vc, ve, table, lens, 0.1)
+    hit = torch.zeros(len(lens), Hq, dtype=torch.bool)
+    bad = q.clone()
+    for b in range(len(lens)):
+        for g in range(H):
+            h = g * (Hq // H) + int(rng.integers(Hq // H))
+            bad[b, h, int(rng.integers(D))] = [float("nan"), float("inf"), -float("inf")][(b + g) % 3]
+            hit[b, h] = True
+    got = run_decode(ops, bad, kc, ke, vc, ve, table, lens, 0.1).cpu()
+    assert got[hit].isnan().all()
+    got[hit] = clean.cpu()[hit]
+    check_attn(got, q, kc, ke, vc, ve, table, lens, 0.1)
+
+
+@pytest.mark.parametrize("Hq,H,D", [(32, 4, 128), (64, 4, 128), (16, 2, 64), (40, 1, 128)])
+def test_decode_query_heads_far_apart(ops, Hq, H, D):
+    """Heads of one kv head whose queries differ by up to 2^120 each have their own weights."""
+    rng = np.random.default_rng(41)
+    lens = [100, 1, 700]
+    q, kc, ke, vc, ve, table = attn_case(rng, lens, Hq, H, D)
+    q = (q.double() * 2.0 ** torch.tensor([0, 60, -60, 0, 15, -15, 30])[torch.arange(Hq) % 7][:, None]).bfloat16()
+    check_attn(run_decode(ops, q, kc, ke, vc, ve, table, lens, 0.1), q, kc, ke, vc, ve, table, lens, 0.1)
