@@ -234,8 +234,9 @@ int b200_kv_append(const void* k_new, const void* v_new, void* k_pool, void* v_p
  *                        position % 16.  Rows behind the last token: -1, 0, -1.
  *   supply_used_out [1]  entries of the supply that are used now
  * Findings (status word, optional): a sequence with a negative length or more tokens than its table row gets nothing; more tokens
- * than num_rows; fewer free pages than needed or a page id outside [0, num_blocks): slots of -1.  At most 4096 sequences and fewer
- * than 2^31 tokens in the table.  lens and supply_used_out must not be inputs.
+ * than num_rows; fewer free pages than needed or a page id outside [0, num_blocks): slots of -1, and -1 in the table for a fresh page,
+ * which the calls after this one find again.  At most 4096 sequences and fewer than 2^31 tokens in the table.  lens and supply_used_out
+ * must not be inputs.
  *
  * b200_kv8_append: rows of keys and values (bf16 or fp32; [num_rows, num_kv_heads, head_dim] with a row stride in elements) into
  * their slots; a negative slot is no slot.  Rows that go to one page stand side by side, in rising order and without gaps, and the page is no

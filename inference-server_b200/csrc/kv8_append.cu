@@ -104,11 +104,13 @@ kv_slot_map_kernel(const int* __restrict__ ctx_lens, const int* __restrict__ new
 
   const int stride = gridDim.x * kMapThreads;
   const int handed = min(pages, supply_len - used);
-  for (int p = blockIdx.x * kMapThreads + tid; p < handed; p += stride) {
-    const int id = supply[used + p];
+  // A page that is not there, or is none, is -1 in the table: lens counts it, so the next call takes the entry for the sequence's own page,
+  // and what a table row of earlier use names there belongs to another sequence by now.
+  for (int p = blockIdx.x * kMapThreads + tid; p < pages; p += stride) {
+    int id = p < handed ? supply[used + p] : -1;
     if (id < 0 || id >= num_blocks) {
-      set_error(err, kErrDevBadBlockId);
-      continue;
+      if (p < handed) set_error(err, kErrDevBadBlockId);
+      id = -1;
     }
     // of sequences that begin at the same page the last is the one that gets it
     const int b = bisect(pages_at, num_seqs, p);

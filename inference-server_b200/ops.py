@@ -239,7 +239,8 @@ def kv_slot_map(ctx_lens, new_lens, block_table, supply, supply_used, num_rows: 
     """Where the new tokens of a pass go, worked out on the GPU: sequence b has ctx_lens[b] tokens and gets new_lens[b] more.  Pages they
     need are taken from `supply` [any], free page ids, from entry supply_used [1] on, and entered into block_table [B, max_pages] in
     place.  `num_rows`: rows of the pass, at least the sum of new_lens; rows behind the last token get slot -1.  Slots are
-    page * 16 + position % 16, for `kv8_append` or any other cache of 16-token pages; page ids outside [0, num_blocks) are findings."""
+    page * 16 + position % 16, for `kv8_append` or any other cache of 16-token pages; page ids outside [0, num_blocks) are findings.  A page
+    that the supply does not have is a finding too, and -1 in the table: no later call takes an older entry for it."""
     return tuple.__new__(KvSlotMap, (_native or _load_native()).slot_map(ctx_lens, new_lens, block_table, supply, supply_used, num_rows, num_blocks, status))
 
 

@@ -674,3 +674,38 @@ def test_decode_query_heads_far_apart(ops, Hq, H, D):
     q, kc, ke, vc, ve, table = attn_case(rng, lens, Hq, H, D)
     q = (q.double() * 2.0 ** torch.tensor([0, 60, -60, 0, 15, -15, 30])[torch.arange(Hq) % 7][:, None]).bfloat16()
     check_attn(run_decode(ops, q, kc, ke, vc, ve, table, lens, 0.1), q, kc, ke, vc, ve, table, lens, 0.1)
+
+
+def test_slot_map_pages_that_cannot_be_had(ops):
+    """Rows of a table that was used before hold ids of pages that are others' by now: where no page, or none that is one, can be handed out, the entry says so."""
+    was = np.arange(100, 100 + 4 * 5, dtype=np.int32).reshape(4, 5)
+    for supply, used, gets, code in (([7, 8], 0, [7, 8, -1, -1], 21), ([7, 8], 2, [-1] * 4, 21), ([7, 8], 3, [-1] * 4, 21), ([7, 8], -1, [-1] * 4, 21),
+                                     ([], 0, [-1] * 4, 21), ([7, 999, -3, 8], 0, [7, -1, -1, 8], 16)):
+        table, status = torch.from_numpy(was.copy()).to(DEV), status_word()
+        m = ops.kv_slot_map(ints([16, 3, 0, 20]), ints([33, 2, 1, 1]), table, ints(supply), ints([used]), 40, 200, status=status)
+        want = was.copy()
+        want[0, 1:4], want[2, 0] = gets[:3], gets[3]
+        assert table.tolist() == want.tolist() and status.item() == code
+        assert m.lens.tolist() == [49, 5, 1, 21] and m.row_start.tolist() == [0, 33, 35, 36, 37]
+        slots = [want[0, 1 + i // 16] * 16 + i % 16 if want[0, 1 + i // 16] >= 0 else -1 for i in range(33)] + [105 * 16 + 3, 105 * 16 + 4]
+        assert m.slots.tolist() == slots + [want[2, 0] * 16 if want[2, 0] >= 0 else -1, 116 * 16 + 4] + [-1] * 3
+
+
+def test_a_step_after_pages_ran_out_touches_no_page_of_others(ops):
+    """Sequence 0 needs a page that is not there, and its table row still names one from before, sequence 1's.  The steps after that go on with the lengths."""
+    rng = np.random.default_rng(42)
+    H, D, blocks = 2, 64, 8
+    codes, exps = plain.random_cache(rng, blocks, H, D)
+    cache = [plain.pool_of(codes.copy()), plain.pool_of(codes.copy()), plain.scale_of(exps), plain.scale_of(exps)]
+    table, ctx, used = ints([[1, 3, 3], [2, 3, -1]]), ints([15, 20]), ints([1])
+    for step in range(3):
+        status = status_word()
+        m = ops.kv_slot_map(ctx, ints([1, 0]), table, ints([5]), used, 1, blocks, status=status)
+        k, v = (torch.from_numpy(r).to(DEV) for r in rows_of(rng, 1, H, D, torch.float32))
+        ops.kv8_append(k, v, *cache, m.slots, status=status)
+        assert status.item() == [0, 21, 16][step] and m.slots.tolist() == [[31], [-1], [-1]][step]
+        ctx, used = m.lens, m.supply_used
+    for pool in cache[:2]:
+        got = pool.view(torch.uint8).cpu().numpy()
+        assert np.array_equal(np.delete(got, 1, 0), np.delete(codes, 1, 0))
+    assert table.tolist() == [[1, -1, 3], [2, 3, -1]]
