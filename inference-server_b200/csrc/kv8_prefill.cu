@@ -543,8 +543,11 @@ kv8_attn_prefill_kernel(const __grid_constant__ CUtensorMap k_map, const uint8_t
     const size_t oidx = static_cast<size_t>(tok) * num_q_heads + h * gr + (r - rt * gr);
     const bool second = own == 1 && n_of[1] > 0;  // there is an accumulator 1 to be added
     float l = l_run, w0 = 1.f, w1 = 0.f;
+    bool any0 = true, any1 = false;  // the accumulator holds something
     if (own == 1) {
       const float m0 = refs[r], m1 = refs[kTcRows + r];
+      any0 = m0 > -INFINITY;
+      any1 = m1 > -INFINITY;
       m_run = fmaxf(m0, m1);
       const float ref = m_run == -INFINITY ? 0.f : m_run;
       w0 = fast_exp2(m0 - ref);
@@ -565,16 +568,17 @@ kv8_attn_prefill_kernel(const __grid_constant__ CUtensorMap k_map, const uint8_t
         uint32_t o[32];
         tmem_ld32(acc + c0, o);
         tmem_ld_wait();
-        // the weight of an accumulator that holds nothing is 0, but what it holds may not be a number
+        // What is in an accumulator that holds nothing may not be a number, and its weight of 0 would not undo that.  A weight that vanished
+        // beside the other's is taken: times a NaN it is one.
 #pragma unroll
-        for (int c = 0; c < 32; ++c) o[c] = __float_as_uint(w0 == 0.f ? none : __uint_as_float(o[c]) * (w0 * inv));
+        for (int c = 0; c < 32; ++c) o[c] = __float_as_uint(any0 ? __uint_as_float(o[c]) * (w0 * inv) : none);
         if (second) {
           uint32_t o1[32];
           tmem_ld32(acc + kTcKeys + c0, o1);
           tmem_ld_wait();
 #pragma unroll
           for (int c = 0; c < 32; ++c)
-            if (w1 != 0.f) o[c] = __float_as_uint(fmaf(__uint_as_float(o1[c]), w1 * inv, __uint_as_float(o[c])));
+            if (any1) o[c] = __float_as_uint(fmaf(__uint_as_float(o1[c]), w1 * inv, __uint_as_float(o[c])));
         }
         if (real && alive) {
           if (splits > 1) {

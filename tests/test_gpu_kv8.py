@@ -709,3 +709,19 @@ def test_a_step_after_pages_ran_out_touches_no_page_of_others(ops):
         got = pool.view(torch.uint8).cpu().numpy()
         assert np.array_equal(np.delete(got, 1, 0), np.delete(codes, 1, 0))
     assert table.tolist() == [[1, -1, 3], [2, 3, -1]]
+
+
+@pytest.mark.parametrize("H,D", [(1, 64), (1, 128), (100, 64), (100, 128)])
+def test_prefill_value_of_nan_whose_weight_vanishes(ops, H, D):
+    """A NaN value under a weight of 2^-400: a softmax in floating point multiplies it by zero, which is NaN."""
+    rng = np.random.default_rng(45)
+    n, first = 2, 254
+    _, kc, ke, vc, ve, table = attn_case(rng, [first + n], H, H, D)
+    ke[:], ve[:] = 0, 0
+    kc[:] = 0
+    q = torch.ones(n, H, D, device=DEV, dtype=torch.bfloat16)
+    for t in range(128, 256):  # the second tile of keys: scores of 8 D
+        kc[table[0, t // 16], :, t % 16] = int(plain.encode(np.array([8.0]))[0])
+    vc[table[0, 0], 0, 3, 5] = 127
+    got = ops.kv8_attn_prefill(q, plain.pool_of(kc), plain.pool_of(vc), plain.scale_of(ke), plain.scale_of(ve), ints(table[0].tolist()), first, 1.0).isnan()
+    assert got[:, 0, 5].all() and int(got.sum()) == n
