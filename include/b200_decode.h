@@ -255,8 +255,8 @@ int b200_kv_append(const void* k_new, const void* v_new, void* k_pool, void* v_p
  *
  * b200_kv8_attn_prefill: causal attention of num_tokens consecutive tokens of one sequence, at positions first_position .., whose keys and
  * values are in their slots.  q, out [num_tokens, num_q_heads, head_dim] bf16, at most 128 query heads per kv head, the arithmetic of decode.
- * workspace: b200_kv8_attn_prefill_workspace_bytes bytes (the same rules).  A NaN value of a token reaches the rows of up to 127 tokens ahead
- * of it.
+ * workspace: b200_kv8_attn_prefill_workspace_bytes bytes (the same rules).  A NaN value of a token makes its column NaN in the rows from that
+ * token on, and touches no row ahead of it.
  */
 int b200_kv_slot_map(const int32_t* ctx_lens, const int32_t* new_lens, int32_t* block_table, const int32_t* supply,
                      const int32_t* supply_used, int supply_len, int32_t* lens, int32_t* row_start, int32_t* row_seq,

@@ -19,7 +19,8 @@
 //            else: when it converted values too, it asked for keys so late that S waited for memory.
 //   warp 1   S issuer (one thread), warp 2 P V issuer (one thread).
 //   warps 4-7    a quarter of a tile's values each: 16 bytes of a row to 16 f16 numbers; zero for what lies behind the last token, where a page
-//            may hold NaN.  One such warp per scheduler: with two of them on two, the softmax warps beside them held up the others.
+//            may hold NaN, and for NaN in a tile that some row sees in part; what they took out there they put into the rows that see it, at the
+//            end.  One such warp per scheduler: with two of them on two, the softmax warps beside them held up the others.
 //   warps 8-11, 12-15   first the queries of both tiles (bf16 to hi and lo, a row's top by shuffles), then the softmax of tile 0 and of tile 1,
 //            a thread per score row; the scales of a key tile's 8 pages come to each warp by its own lanes, two key tiles
 //            ahead (ids) and one (scales), and from a corner of shared memory to all lanes, put there once the tile before is done, so that
@@ -143,6 +144,32 @@ __device__ __forceinline__ void values_to_f16(uint32_t from, uint32_t to, int ro
   __syncwarp();
 }
 
+// The NaN codes of four e4m3 numbers: the top bit of each such byte.
+__device__ __forceinline__ uint32_t nan_codes(uint32_t w) { return ((w & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u; }
+
+// Makes NaN zero in the first `rows` rows of a warp's quarter of a raw tile; whether there was any.
+template <int D>
+__device__ __forceinline__ bool nan_to_zero(uint32_t from, int rows, int lane) {
+  bool any = false;
+#pragma unroll
+  for (int i0 = 0; i0 < kTcKeys / 4 * (D / 16); i0 += 32) {
+    const int i = i0 + lane;
+    if (i >= rows * (D / 16)) continue;
+    uint32_t w[4], nan[4];
+    lds_words<16>(from + i * 16, w);
+#pragma unroll
+    for (int k = 0; k < 4; ++k) nan[k] = nan_codes(w[k]);
+    if (nan[0] | nan[1] | nan[2] | nan[3]) {
+      any = true;
+#pragma unroll
+      for (int k = 0; k < 4; ++k) w[k] &= ~((nan[k] >> 7) * 0xffu);
+      asm volatile("st.shared.v4.b32 [%0], {%1,%2,%3,%4};" ::"r"(from + i * 16), "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3]) : "memory");
+    }
+  }
+  __syncwarp();  // other lanes read what this one wrote
+  return __any_sync(0xffffffffu, any);
+}
+
 template <int D>
 __global__ void __launch_bounds__(kKv8PrefillThreads, 1)
 kv8_attn_prefill_kernel(const __grid_constant__ CUtensorMap k_map, const uint8_t* __restrict__ v_pool, const uint8_t* __restrict__ k_scale,
@@ -169,6 +196,7 @@ kv8_attn_prefill_kernel(const __grid_constant__ CUtensorMap k_map, const uint8_t
   const uint32_t bar_odone = bars + 160;                          // [2 tiles] O += P V finished
   const uint32_t bar_pfull = bars + 176;                          // [2 tiles][2 halves of 64 keys] P written, O rescaled
   uint32_t* tmem_base_sm = reinterpret_cast<uint32_t*>(base_ptr + Cfg::kBars + 240);
+  volatile int* nan_sm = reinterpret_cast<int*>(base_ptr + Cfg::kBars + 244);  // a NaN value was taken out of a tile that some row sees in part
   float* row_scale = reinterpret_cast<float*>(base_ptr + Cfg::kRowScale);
   float* sums = reinterpret_cast<float*>(base_ptr + Cfg::kSums);
   float* refs = reinterpret_cast<float*>(base_ptr + Cfg::kRefs);
@@ -176,6 +204,7 @@ kv8_attn_prefill_kernel(const __grid_constant__ CUtensorMap k_map, const uint8_t
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   if (threadIdx.x == 32) tma_prefetch_desc(&k_map);
   if (threadIdx.x == 0) {
+    *nan_sm = 0;
     for (int s = 0; s < 2; ++s) {
       mbar_init(bar_rawfull + 8 * s, 1);
       mbar_init(bar_rawempty + 8 * s, 4);
@@ -322,17 +351,47 @@ kv8_attn_prefill_kernel(const __grid_constant__ CUtensorMap k_map, const uint8_t
   } else if (warp < 8) {
     // ------------------------------------------------- V in f16 ------
     asm volatile("setmaxnreg.dec.sync.aligned.u32 40;");
+    // Key tiles from this one on hold keys that some row of the CTA does not see.  A product takes a weight of zero times such a key's value, and a
+    // NaN among the values would spoil rows ahead of it: they are taken out of these tiles, and put back by the rows that see them.
+    const int edge_tile = (first_pos + t0 + 1) / kTcKeys;
     bool alive = true;
 #pragma unroll 1
     for (int j = 0; j < n_tiles && alive; ++j) {
       const int st = j & 1;
       alive = mbar_wait_warp(bar_rawfull + 8 * st, (j >> 1) & 1, err) && mbar_wait_warp(bar_vempty + 8 * st, ((j >> 1) & 1) ^ 1, err);
       if (!alive) break;
+      if (kt0 + j >= edge_tile) {
+        const int row0 = (warp - 4) * (kTcKeys / 4), rows = min(max(last_pos - (kt0 + j) * kTcKeys + 1 - row0, 0), kTcKeys / 4);
+        if (nan_to_zero<D>(base + Cfg::kRaw + st * Cfg::kTile8 + row0 * D, rows, lane)) *nan_sm = 1;
+      }
       values_to_f16<D>(base + Cfg::kRaw + st * Cfg::kTile8, base + Cfg::kV + st * Cfg::kTile16, (warp - 4) * (kTcKeys / 4),
                        last_pos - (kt0 + j) * kTcKeys + 1, lane);
       if (lane == 0) {
         mbar_arrive(bar_vfull + 8 * st);
         mbar_arrive(bar_rawempty + 8 * st);
+      }
+    }
+    // Once the rows are written, those that see such a NaN get it: a thread finds a column's first and goes through the rows from there on.  (Two
+    // plain loops: loops within loops, a row a thread, took the compiler's care from the softmax warps' loop although they hardly ever run, 229 ->
+    // 245 us for 1024 tokens behind 14336, here, in an idle warp or behind the rows' own stores alike.)
+    __syncwarp();
+    asm volatile("bar.sync 2, 384;" ::: "memory");
+    const int c = threadIdx.x - 128;
+    if (*nan_sm && c < D) {
+      int x = max(edge_tile, kt0) * kTcKeys;
+      const int end = min(last_pos + 1, (kt0 + n_tiles) * kTcKeys);
+#pragma unroll 1
+      for (; x < end; ++x) {
+        const int page = __ldg(table_row + x / kKvPage);
+        const size_t cell = static_cast<size_t>(page < 0 || page >= num_blocks ? 0 : page) * num_kv_heads + h;
+        if ((__ldg(v_pool + cell * kPageBytes8 + x % kKvPage * D + c) & 0x7f) == 0x7f) break;
+      }
+      const int rows = x < end ? (t_end - t0) * gr : 0;
+#pragma unroll 1
+      for (int i = max(x - first_pos - t0, 0) * gr; i < rows; ++i) {
+        const size_t oidx = static_cast<size_t>(t0 + i / gr) * num_q_heads + h * gr + i % gr;
+        if (splits > 1) part_o[(oidx * splits + split) * D + c] = NAN;
+        else out[oidx * D + c] = __ushort_as_bfloat16(0x7fffu);
       }
     }
   } else {
@@ -598,6 +657,8 @@ kv8_attn_prefill_kernel(const __grid_constant__ CUtensorMap k_map, const uint8_t
         }
       }
     }
+    __syncwarp();
+    asm volatile("bar.arrive 2, 384;" ::: "memory");  // rows written
   }
 
   tc_fence_before();

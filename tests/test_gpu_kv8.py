@@ -725,3 +725,39 @@ def test_prefill_value_of_nan_whose_weight_vanishes(ops, H, D):
     vc[table[0, 0], 0, 3, 5] = 127
     got = ops.kv8_attn_prefill(q, plain.pool_of(kc), plain.pool_of(vc), plain.scale_of(ke), plain.scale_of(ve), ints(table[0].tolist()), first, 1.0).isnan()
     assert got[:, 0, 5].all() and int(got.sum()) == n
+
+
+def prompt_of(ops, n, first, Hq, H, D, seed):
+    rng = np.random.default_rng(seed)
+    _, kc, ke, vc, ve, table = attn_case(rng, [first + n], Hq, H, D)
+    q = torch.from_numpy(rng.standard_normal((n, Hq, D)).astype(np.float32)).bfloat16().to(DEV)
+
+    def run(v, k=kc):
+        ws = ops.kv8_attn_prefill_workspace(n, first, Hq, H, D, DEV)
+        ws[4:] = 255
+        out = ops.kv8_attn_prefill(q, plain.pool_of(k), plain.pool_of(v), plain.scale_of(ke), plain.scale_of(ve), torch.from_numpy(table[0]).to(DEV), first, 0.1,
+                                   workspace=ws, out=torch.full_like(q, float("nan")))
+        ops.read_status(ws, "prompt")
+        return out
+
+    return run, kc, vc, table[0]
+
+
+@pytest.mark.parametrize("Hq,H,D,n,first", [(32, 32, 64, 2048, 1), (32, 32, 128, 700, 1), (32, 4, 128, 1500, 77), (8, 2, 64, 400, 0), (3, 3, 128, 130, 5), (64, 4, 128, 17, 5001),
+                                            (8, 2, 128, 300, 900), (5, 1, 64, 200, 333), (100, 1, 64, 9, 120), (4, 4, 64, 128, 127)])
+def test_prefill_masked_values_of_nan_reach_nothing(ops, Hq, H, D, n, first):
+    """A NaN value of a token is NaN in its column for the rows from that token on and nothing to the rows ahead of it, which keep their bits."""
+    run, _, vc, row = prompt_of(ops, n, first, Hq, H, D, seed=43)
+    clean, bad = run(vc), vc.copy()
+    rng = np.random.default_rng(44)
+    want = torch.zeros(n, Hq, D, dtype=torch.bool)
+    last = first + n - 1
+    for t in {0, first, first + 1, first + n // 2, (first + n // 2) // 128 * 128 + 127, first + min(n - 1, 255), last - 1, last, *(int(x) for x in rng.integers(first, first + n, 4))}:
+        if not 0 <= t <= last:
+            continue
+        h, c = int(rng.integers(H)), int(rng.integers(D))
+        bad[row[t // 16], h, t % 16, c] = (127, 255)[t & 1]
+        want[max(t - first, 0):, h * (Hq // H):(h + 1) * (Hq // H), c] = True
+    got = run(bad)
+    assert torch.equal(got.isnan().cpu(), want)
+    assert torch.equal(got.cpu()[~want], clean.cpu()[~want])
