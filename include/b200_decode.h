@@ -223,6 +223,7 @@ int b200_kv_append(const void* k_new, const void* v_new, void* k_pool, void* v_p
  *   k_pool/v_pool   [num_blocks, num_kv_heads, 16, head_dim] e4m3, head_dim 64 or 128, 16-byte aligned
  *   k_scale/v_scale [num_blocks, num_kv_heads] bytes: the numbers of a page and kv head stand for themselves times 2^(byte - 127)
  *                   (e8m0).  Exponents go from -32 to 31; a byte beyond is taken for the nearest.
+ *   Tables, lengths, slots and status words are 4-byte aligned.
  *
  * b200_kv_slot_map: slots of new tokens from request lengths, pages for them from a list of free ones.
  *   ctx_lens, new_lens [num_seqs]   tokens that a sequence has, and gets

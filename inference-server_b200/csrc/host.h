@@ -110,6 +110,12 @@ inline AttnWorkspace carve(void* ws, int batch, int hq, int D, int max_splits) {
   return w;
 }
 
+// Whether all pointers are on a boundary of 4 bytes: a kernel's access to a word off it is a fault.
+template <typename... T>
+bool on_words(const T*... p) {
+  return ((reinterpret_cast<uintptr_t>(p) | ...) & 3) == 0;
+}
+
 // Argument checks that the attention entry points of the 8-bit page cache share; joining their partials (kv8_decode.cu).
 int check_kv8(const char* name, int rows, int hq, int hkv, int head_dim, int num_blocks, int max_pages, const void* q, const void* k_pool,
               const void* v_pool, const void* out, float scale);

@@ -350,6 +350,8 @@ extern "C" int b200_kv_slot_map(const int32_t* ctx_lens, const int32_t* new_lens
   B200_REQUIRE(ctx_lens && new_lens && block_table && supply_used && lens && row_start && supply_used_out &&
                    (supply || supply_len == 0) && ((row_seq && positions && slots) || num_rows == 0),
                "kv_slot_map: null pointer");
+  B200_REQUIRE(on_words(ctx_lens, new_lens, block_table, supply, supply_used, lens, row_start, row_seq, positions, slots, supply_used_out, status_word),
+               "kv_slot_map: whole numbers and the status word must be 4-byte aligned");
   B200_REQUIRE(num_seqs > 0 && num_seqs <= kMapMaxSeqs, "kv_slot_map: %d sequences outside [1, %d]", num_seqs, kMapMaxSeqs);
   B200_REQUIRE(num_rows >= 0 && supply_len >= 0 && num_blocks > 0 && max_pages_per_seq > 0, "kv_slot_map: bad dimension");
   B200_REQUIRE(static_cast<long long>(num_seqs) * max_pages_per_seq * kKvPage < (1ll << 31) &&
@@ -375,6 +377,7 @@ extern "C" int b200_kv8_append(const void* k_new, const void* v_new, int64_t k_r
                                void* k_scale, void* v_scale, const int32_t* slots, void* status_word, int num_rows, int num_kv_heads,
                                int head_dim, int num_blocks, int dtype, void* stream) {
   B200_REQUIRE(k_new && v_new && k_pool && v_pool && k_scale && v_scale && slots, "kv8_append: null pointer");
+  B200_REQUIRE(on_words(slots, status_word), "kv8_append: slots and the status word must be 4-byte aligned");
   B200_REQUIRE(num_rows > 0 && num_kv_heads > 0 && num_blocks > 0, "kv8_append: non-positive dimension");
   B200_REQUIRE(head_dim == 64 || head_dim == 128, "kv8_append: head_dim %d is neither 64 nor 128", head_dim);
   B200_REQUIRE(dtype == 0 || dtype == 1, "kv8_append: dtype %d is neither 0 (bf16) nor 1 (f32)", dtype);

@@ -842,6 +842,7 @@ extern "C" int b200_kv8_attn_decode(const void* q, const void* k_pool, const voi
   B200_REQUIRE(q && k_pool && v_pool && k_scale && v_scale && block_table && ctx_lens && out && workspace, "kv8_attn_decode: null pointer");
   int rc = check_kv8("kv8_attn_decode", batch, num_q_heads, num_kv_heads, head_dim, num_blocks, max_pages_per_seq, q, k_pool, v_pool, out, scale);
   if (rc) return rc;
+  B200_REQUIRE(on_words(block_table, ctx_lens), "kv8_attn_decode: block table and lengths must be 4-byte aligned");
   B200_REQUIRE(split_tokens >= 0 && split_tokens % kKvPage == 0, "kv8_attn_decode: split_tokens %d not a multiple of %d", split_tokens, kKvPage);
   B200_REQUIRE(static_cast<long long>(batch) * max_pages_per_seq < (1ll << 31), "kv8_attn_decode: the table has more than 2^31 entries");
   rc = check_device(nullptr);

@@ -733,6 +733,7 @@ extern "C" int b200_kv8_attn_prefill(const void* q, const void* k_pool, const vo
   int rc = check_kv8("kv8_attn_prefill", num_tokens, num_q_heads, num_kv_heads, head_dim, num_blocks, max_pages_per_seq, q, k_pool, v_pool, out,
                      scale);
   if (rc) return rc;
+  B200_REQUIRE(on_words(block_table_row), "kv8_attn_prefill: the table row must be 4-byte aligned");
   B200_REQUIRE(num_q_heads / num_kv_heads <= kTcRows, "kv8_attn_prefill: more than %d q heads per kv head", kTcRows);
   B200_REQUIRE(first_position >= 0 && static_cast<long long>(first_position) + num_tokens <= static_cast<long long>(max_pages_per_seq) * kKvPage,
                "kv8_attn_prefill: positions %d .. of %d tokens do not fit %d pages", first_position, num_tokens, max_pages_per_seq);

@@ -761,3 +761,13 @@ def test_prefill_masked_values_of_nan_reach_nothing(ops, Hq, H, D, n, first):
     got = run(bad)
     assert torch.equal(got.isnan().cpu(), want)
     assert torch.equal(got.cpu()[~want], clean.cpu()[~want])
+
+
+def test_status_words_off_their_boundary_are_refused(ops):
+    odd = torch.zeros(12, dtype=torch.uint8, device=DEV)[2:10]
+    pools = ops.kv8_pools(4, 2, 64, DEV)
+    x, slots = torch.zeros(3, 2, 64, device=DEV), ints([0, 1, 2])
+    with pytest.raises(pkg("_lib").B200Error, match="4-byte"):
+        ops.kv8_append(x, x, *pools, slots, status=odd)
+    with pytest.raises(pkg("_lib").B200Error, match="4-byte"):
+        ops.kv_slot_map(slots, slots, slots.view(3, 1), slots, slots[:1], 4, 4, status=odd)

@@ -129,3 +129,30 @@ def test_wrappers_refuse_what_is_not_on_a_gpu():
         ops.kv8_attn_decode(torch.zeros(3, 4, 64, dtype=torch.bfloat16), *pools, i.view(3, 1), i, 0.1)
     with pytest.raises(ValueError, match="CUDA"):
         ops.kv8_attn_prefill(torch.zeros(3, 4, 64, dtype=torch.bfloat16), *pools, i, 0, 0.1)
+
+
+def test_whole_numbers_and_status_words_off_their_boundary_are_refused():
+    """A word that the GPU would read, or record a finding in, has to lie on a multiple of its 4 bytes: an access off it is a fault there."""
+    lib = pkg("_lib").load()
+
+    def slot_map(**at):
+        a = dict(ctx=P, new=P, table=P, supply=P, used=P, lens=P + 64, start=P, seq=P, pos=P, slots=P, out=P + 128, status=P) | at
+        return lib.b200_kv_slot_map(a["ctx"], a["new"], a["table"], a["supply"], a["used"], 5, a["lens"], a["start"], a["seq"], a["pos"], a["slots"], a["out"],
+                                    a["status"], 3, 7, 9, 4, None)
+
+    for name in ("ctx", "new", "table", "supply", "used", "lens", "start", "seq", "pos", "slots", "out", "status"):
+        for off in (1, 2, 3):
+            refused(slot_map(**{name: P + 256 + off}), "4-byte")
+
+    def append(slots=P, status=P):
+        return lib.b200_kv8_append(P, P, 512, 512, P, P, P, P, slots, status, 4, 4, 128, 9, 0, None)
+
+    refused(append(slots=P + 2), "4-byte")
+    refused(append(status=P + 1), "4-byte")
+
+    def decode(table=P, ctx=P):
+        return lib.b200_kv8_attn_decode(P, P, P, P, P, table, ctx, P, P, 1 << 20, 2, 8, 2, 64, 9, 4, 0.1, 0, None)
+
+    refused(decode(table=P + 2), "4-byte")
+    refused(decode(ctx=P + 3), "4-byte")
+    refused(lib.b200_kv8_attn_prefill(P, P, P, P, P, P + 1, P, P, 1 << 20, 5, 0, 8, 2, 64, 9, 4, 0.1, None), "4-byte")
