@@ -137,13 +137,32 @@ Queries queries_of(PyObject* q_arg, PyObject* out_arg, PyObject* index_arg, cons
   }
   return r;
 }
-at::Tensor workspace_of(PyObject* o, size_t (*bytes)(int, int, int, int, int, int), const int (&a)[6], const at::Tensor& q) {
-  if (o == Py_None) return at::zeros({static_cast<int64_t>(bytes(a[0], a[1], a[2], a[3], a[4], a[5]))}, q.options().dtype(at::kByte));
-  const at::Tensor& t = tensor(o, "workspace");
-  need(t, "workspace", at::kByte);
-  device_of({&q, &t});
-  return t;
-}
+// The workspace of an attention call.  Without one of the caller's it is made here, all of it uninitialised but the status word, which takes what the
+// caller's status word says and is handed back to it (done): findings of such a call are not lost with its workspace.
+struct Workspace {
+  at::Tensor all, word, status;
+  Workspace(PyObject* o, PyObject* status_arg, size_t (*bytes)(int, int, int, int, int, int), const int (&a)[6], const at::Tensor& q) {
+    void* at = status_word(status_arg, q.get_device());
+    if (o != Py_None) {
+      if (at != nullptr) refuse("a call with a workspace records findings in its first word: status goes with workspace=None");
+      all = tensor(o, "workspace");
+      need(all, "workspace", at::kByte);
+      device_of({&q, &all});
+      return;
+    }
+    all = at::empty({static_cast<int64_t>(bytes(a[0], a[1], a[2], a[3], a[4], a[5]))}, q.options().dtype(at::kByte));
+    word = all.narrow(0, 0, 4);
+    if (at == nullptr) {
+      word.zero_();
+    } else {
+      status = at::from_blob(at, {4}, word.options());
+      word.copy_(status);
+    }
+  }
+  void done() {
+    if (status.defined()) status.copy_(word);
+  }
+};
 size_t prefill_bytes(int tokens, int first, int hq, int hkv, int dim, int) { return p_prefill_bytes(tokens, first, hq, hkv, dim); }
 
 // Turns what a body throws into Python errors.
@@ -234,9 +253,9 @@ PyObject* append(PyObject*, PyObject* const* args, Py_ssize_t n) {
   });
 }
 
-// (q, k_pool, v_pool, k_scale, v_scale, block_table, ctx_lens, scale, split_tokens, workspace, out) -> out
+// (q, k_pool, v_pool, k_scale, v_scale, block_table, ctx_lens, scale, split_tokens, workspace, out, status) -> out
 PyObject* decode(PyObject*, PyObject* const* args, Py_ssize_t n) {
-  return guarded(n, 11, [&]() -> PyObject* {
+  return guarded(n, 12, [&]() -> PyObject* {
     const Cache c = cache_of(args + 1);
     Queries x = queries_of(args[0], args[10], args[5], "block_table", c.dim);
     const at::Tensor& ctx = tensor(args[6], "ctx_lens");
@@ -248,21 +267,22 @@ PyObject* decode(PyObject*, PyObject* const* args, Py_ssize_t n) {
     const int split = whole(args[8]), width = narrow(x.index.size(1), "block table");
     if (!x.out.defined()) x.out = fresh_tensor(x.q.sizes(), x.q);
     if (x.rows > 0) {
-      const at::Tensor ws = workspace_of(args[9], p_decode_bytes, {x.rows, x.heads, c.heads, c.dim, width, split}, x.q);
+      Workspace ws(args[9], args[11], p_decode_bytes, {x.rows, x.heads, c.heads, c.dim, width, split}, x.q);
       const int rc = without_gil([&] {
         return p_decode(x.q.data_ptr(), c.k.data_ptr(), c.v.data_ptr(), c.ks.data_ptr(), c.vs.data_ptr(), x.index.data_ptr<int32_t>(),
-                        ctx.data_ptr<int32_t>(), x.out.data_ptr(), ws.data_ptr(), ws.nbytes(), x.rows, x.heads, c.heads, c.dim, c.blocks, width,
+                        ctx.data_ptr<int32_t>(), x.out.data_ptr(), ws.all.data_ptr(), ws.all.nbytes(), x.rows, x.heads, c.heads, c.dim, c.blocks, width,
                         static_cast<float>(scale), split, stream_of(device));
       });
       if (rc) return failed(rc, "b200_kv8_attn_decode");
+      ws.done();
     }
     return THPVariable_Wrap(x.out);
   });
 }
 
-// (q, k_pool, v_pool, k_scale, v_scale, table_row, first_pos, scale, workspace, out) -> out
+// (q, k_pool, v_pool, k_scale, v_scale, table_row, first_pos, scale, workspace, out, status) -> out
 PyObject* prefill(PyObject*, PyObject* const* args, Py_ssize_t n) {
-  return guarded(n, 10, [&]() -> PyObject* {
+  return guarded(n, 11, [&]() -> PyObject* {
     const Cache c = cache_of(args + 1);
     Queries x = queries_of(args[0], args[9], args[5], "table_row", c.dim);
     if (x.index.dim() != 1) refuse("table_row must be one row of a block table");
@@ -272,13 +292,14 @@ PyObject* prefill(PyObject*, PyObject* const* args, Py_ssize_t n) {
     if (scale == -1.0 && PyErr_Occurred()) throw python_error();
     if (!x.out.defined()) x.out = fresh_tensor(x.q.sizes(), x.q);
     if (x.rows > 0) {
-      const at::Tensor ws = workspace_of(args[8], prefill_bytes, {x.rows, first, x.heads, c.heads, c.dim, 0}, x.q);
+      Workspace ws(args[8], args[10], prefill_bytes, {x.rows, first, x.heads, c.heads, c.dim, 0}, x.q);
       const int rc = without_gil([&] {
         return p_prefill(x.q.data_ptr(), c.k.data_ptr(), c.v.data_ptr(), c.ks.data_ptr(), c.vs.data_ptr(), x.index.data_ptr<int32_t>(),
-                         x.out.data_ptr(), ws.data_ptr(), ws.nbytes(), x.rows, first, x.heads, c.heads, c.dim, c.blocks, width,
+                         x.out.data_ptr(), ws.all.data_ptr(), ws.all.nbytes(), x.rows, first, x.heads, c.heads, c.dim, c.blocks, width,
                          static_cast<float>(scale), stream_of(device));
       });
       if (rc) return failed(rc, "b200_kv8_attn_prefill");
+      ws.done();
     }
     return THPVariable_Wrap(x.out);
   });

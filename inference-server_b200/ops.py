@@ -260,10 +260,11 @@ def kv8_attn_workspace(batch: int, num_q_heads: int, num_kv_heads: int, head_dim
 
 
 def kv8_attn_decode(q, k_pool, v_pool, k_scale, v_scale, block_table, ctx_lens, scale: float, split_tokens: int = 0,
-                    workspace: torch.Tensor | None = None, out: torch.Tensor | None = None) -> torch.Tensor:
+                    workspace: torch.Tensor | None = None, out: torch.Tensor | None = None, status: torch.Tensor | None = None) -> torch.Tensor:
     """`paged_attn_decode` over an 8-bit page cache: softmax(q K^T * scale) V for one bf16 query row [B, Hq, D] per sequence; head_dim 64
-    or 128, any head grouping.  `split_tokens`: tokens that a CTA takes at least; 0: the library's choice."""
-    return (_native or _load_native()).decode(q, k_pool, v_pool, k_scale, v_scale, block_table, ctx_lens, scale, split_tokens, workspace, out)
+    or 128, any head grouping.  `split_tokens`: tokens that a CTA takes at least; 0: the library's choice.  Findings (a page outside the pool, a
+    length beyond the table) are in the workspace's first word, `read_status`; a call without a workspace records them in `status`, if given."""
+    return (_native or _load_native()).decode(q, k_pool, v_pool, k_scale, v_scale, block_table, ctx_lens, scale, split_tokens, workspace, out, status)
 
 
 def kv8_attn_prefill_workspace(num_tokens: int, first_pos: int, num_q_heads: int, num_kv_heads: int, head_dim: int, device) -> torch.Tensor:
@@ -273,11 +274,12 @@ def kv8_attn_prefill_workspace(num_tokens: int, first_pos: int, num_q_heads: int
 
 
 def kv8_attn_prefill(q, k_pool, v_pool, k_scale, v_scale, table_row, first_pos: int, scale: float, workspace: torch.Tensor | None = None,
-                     out: torch.Tensor | None = None) -> torch.Tensor:
+                     out: torch.Tensor | None = None, status: torch.Tensor | None = None) -> torch.Tensor:
     """`paged_attn_prefill` over an 8-bit page cache: causal attention of consecutive prompt tokens of one sequence, q [R, Hq, D] bf16 at
     positions first_pos .. first_pos + R - 1, keys and values already in their slots; table_row [max_pages] int32.  head_dim 64 or 128,
-    up to 128 query heads per kv head.  Few rows over many keys are shared out along the keys and joined in the workspace."""
-    return (_native or _load_native()).prefill(q, k_pool, v_pool, k_scale, v_scale, table_row, first_pos, scale, workspace, out)
+    up to 128 query heads per kv head.  Few rows over many keys are shared out along the keys and joined in the workspace.  Findings as
+    those of `kv8_attn_decode`.  A captured call serves its own first_pos and number of rows: how it is laid out follows from them."""
+    return (_native or _load_native()).prefill(q, k_pool, v_pool, k_scale, v_scale, table_row, first_pos, scale, workspace, out, status)
 
 
 # ---------------------------------------------------------- dense projections

@@ -771,3 +771,52 @@ def test_status_words_off_their_boundary_are_refused(ops):
         ops.kv8_append(x, x, *pools, slots, status=odd)
     with pytest.raises(pkg("_lib").B200Error, match="4-byte"):
         ops.kv_slot_map(slots, slots, slots.view(3, 1), slots, slots[:1], 4, 4, status=odd)
+
+
+def test_findings_without_a_workspace(ops):
+    rng = np.random.default_rng(46)
+    lens = [40, 40]
+    q, kc, ke, vc, ve, table = attn_case(rng, lens, 8, 2, 64)
+    cache = [plain.pool_of(kc), plain.pool_of(vc), plain.scale_of(ke), plain.scale_of(ve)]
+    q, good = q.to(DEV), torch.from_numpy(np.where(table < 0, 0, table)).to(DEV)
+    bad = good.clone()
+    bad[1, 1] = 10 ** 6
+    for call in (lambda t, s: ops.kv8_attn_decode(q, *cache, t, ints(lens), 0.1, status=s), lambda t, s: ops.kv8_attn_prefill(q, *cache, t[1], 38, 0.1, status=s)):
+        status = status_word()
+        want = call(good, status)
+        assert status.item() == 0 and torch.equal(want, call(good, None))
+        call(bad, status)
+        assert status.item() == 16
+
+
+def test_status_beside_a_workspace_is_refused(ops):
+    pools = ops.kv8_pools(4, 2, 64, DEV)
+    q, table, lens = torch.zeros(3, 4, 64, device=DEV, dtype=torch.bfloat16), ints([[0], [1], [2]]), ints([1, 2, 3])
+    ws = ops.kv8_attn_workspace(3, 4, 2, 64, 1, DEV)
+    for bad in (dict(status=status_word(), workspace=ws), dict(status=torch.zeros(1, dtype=torch.int32)), dict(status=torch.zeros(3, dtype=torch.uint8, device=DEV))):
+        with pytest.raises(ValueError, match="status"):
+            ops.kv8_attn_decode(q, *pools, table, lens, 0.1, **bad)
+        with pytest.raises(ValueError, match="status"):
+            ops.kv8_attn_prefill(q, *pools, table[0], 0, 0.1, **bad)
+
+
+def test_findings_without_a_workspace_in_a_captured_call(ops):
+    """The first finding stays: a later clean call leaves it in the status word."""
+    rng = np.random.default_rng(49)
+    q, kc, ke, vc, ve, table = attn_case(rng, [40, 40], 8, 2, 64)
+    cache = [plain.pool_of(kc), plain.pool_of(vc), plain.scale_of(ke), plain.scale_of(ve)]
+    q, table, status = q.to(DEV), torch.from_numpy(np.where(table < 0, 0, table)).to(DEV), status_word()
+    want = ops.kv8_attn_decode(q, *cache, table, ints([40, 40]), 0.1)
+    lens = ints([40, 40])
+    graph, stream = torch.cuda.CUDAGraph(), torch.cuda.Stream()
+    stream.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.graph(graph, stream=stream):
+        out = ops.kv8_attn_decode(q, *cache, table, lens, 0.1, status=status)
+    codes = []
+    with torch.cuda.stream(stream):
+        for L in (40, -1, 40):
+            lens.fill_(L)
+            graph.replay()
+            stream.synchronize()
+            codes.append(status.item())
+    assert codes == [0, 17, 17] and torch.equal(out, want)
