@@ -29,7 +29,6 @@ SUBSETS = {
 }
 HEADERS = ["common.cuh", "glue.cuh", "host.h", "kv8.cuh", "prefill_tc.cuh"]
 BINDING = "kv8_bind.cpp"  # a Python extension module over the C ABI (see there)
-BINDING_PATH = os.path.join(PKG_DIR, "_kv8.so")
 NVCC_FLAGS = [
     "-gencode", "arch=compute_100a,code=sm_100a", "-lineinfo", "-O3", "-std=c++17",
     "-Xcompiler", "-fPIC", "-I", INCLUDE, "-I", CSRC,
@@ -64,36 +63,47 @@ def subset_path(subset: str) -> str:
     return LIB_PATH.replace(".so", f"_{subset}.so")
 
 
+def binding_path() -> str:
+    """File of the native binding for the running Python and the installed torch, whose C++ classes it is compiled against: after an upgrade
+    of either it is another file, which is not there yet."""
+    import torch
+    return os.path.join(PKG_DIR, f"_kv8-{sys.implementation.cache_tag}-torch{torch.__version__}-abi{int(torch._C._GLIBCXX_USE_CXX11_ABI)}.so")
+
+
 def build_binding(force: bool = False) -> str:
     """Compile the native binding against the installed torch and Python.  Returns its path."""
-    source = os.path.join(CSRC, BINDING)
-    if not force and _mtime(BINDING_PATH) >= max(_mtime(source), _mtime(os.path.join(INCLUDE, "b200_decode.h"))):
-        return BINDING_PATH
+    source, path = os.path.join(CSRC, BINDING), binding_path()
+    if not force and _mtime(path) >= max(_mtime(source), _mtime(os.path.join(INCLUDE, "b200_decode.h"))):
+        return path
     import sysconfig
 
     import torch
     base = os.path.dirname(torch.__file__)
     cuda = os.path.dirname(os.path.dirname(os.path.realpath(_nvcc())))
     lib = os.path.join(base, "lib")
-    cmd = ["g++", "-O2", "-std=c++17", "-fPIC", "-shared", "-o", BINDING_PATH + ".tmp", source, "-I", INCLUDE, "-I", os.path.join(base, "include"),
+    cmd = ["g++", "-O2", "-std=c++17", "-fPIC", "-shared", "-o", path + ".tmp", source, "-I", INCLUDE, "-I", os.path.join(base, "include"),
            "-I", os.path.join(base, "include", "torch", "csrc", "api", "include"), "-I", sysconfig.get_path("include"),
            "-I", os.path.join(cuda, "include"), f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
            "-L", lib, "-ltorch_python", "-ltorch", "-ltorch_cpu", "-ltorch_cuda", "-lc10", "-lc10_cuda"]
     res = subprocess.run(cmd, stdout=subprocess.PIPE, stderr=subprocess.STDOUT, text=True)
     if res.returncode != 0:
         raise RuntimeError(f"g++ failed on {BINDING}:\n{res.stdout}")
-    os.replace(BINDING_PATH + ".tmp", BINDING_PATH)
-    return BINDING_PATH
+    os.replace(path + ".tmp", path)
+    return path
 
 
 def build_library(force: bool = False, verbose: bool = False, subset: str | None = None) -> str:
     """Compile what is out of date of the .cu files under csrc/ (of one of SUBSETS if given) and link the shared library; without a
-    subset the native binding too.  Returns the library's path."""
+    subset the native binding too, behind it, for the library does not need torch.  Returns the library's path."""
     sources, lib_path = (SOURCES, LIB_PATH) if subset is None else (SUBSETS[subset], subset_path(subset))
+    if force or not _fresh(lib_path, sources):
+        _compile_and_link(sources, lib_path, force, verbose)
     if subset is None:
         build_binding(force)
-    if not force and _fresh(lib_path, sources):
-        return lib_path
+    return lib_path
+
+
+def _compile_and_link(sources: list[str], lib_path: str, force: bool, verbose: bool) -> None:
     nvcc = _nvcc()
     obj_dir = os.path.join(ROOT_DIR, "build")
     os.makedirs(obj_dir, exist_ok=True)
@@ -122,7 +132,6 @@ def build_library(force: bool = False, verbose: bool = False, subset: str | None
     if res.returncode != 0:
         raise RuntimeError(f"link failed:\n{res.stdout}")
     os.replace(tmp, lib_path)
-    return lib_path
 
 
 def library_for(subset: str) -> str:

@@ -214,12 +214,19 @@ def _load_native():
     strides, all on the current device - and raises ValueError, makes the outputs and calls the C ABI on the current stream."""
     global _native
     import ctypes
-    import importlib
-    lib = _lib.load()
+    import importlib.util
+    import os
+
+    from . import build
+    lib, path = _lib.load(), build.binding_path()
+    if not os.path.exists(path):
+        raise RuntimeError(f"the native binding {os.path.basename(path)} is missing; build it with `python inference-server_b200/build.py`")
     try:
-        module = importlib.import_module("._kv8", __package__)
+        spec = importlib.util.spec_from_file_location(__package__ + "._kv8", path)
+        module = importlib.util.module_from_spec(spec)
+        spec.loader.exec_module(module)
     except ImportError as e:
-        raise RuntimeError("the native binding _kv8.so is missing or does not load; build it with `python inference-server_b200/build.py`") from e
+        raise RuntimeError(f"{path} does not load; build it anew with `python inference-server_b200/build.py --force`") from e
     names = ("b200_kv_slot_map", "b200_kv8_append", "b200_kv8_attn_workspace_bytes", "b200_kv8_attn_decode", "b200_kv8_attn_prefill_workspace_bytes",
              "b200_kv8_attn_prefill")
     module.bind(check, *(ctypes.cast(getattr(lib, n), ctypes.c_void_p).value for n in names))
