@@ -14,8 +14,8 @@ namespace b200 {
 // exclusive prefix sums; so do the rows of the new tokens.  Every CTA takes the sums of all sequences for itself (a few KB from L2, one
 // scan of pairs packed into 64 bits) and keeps them in shared memory; then a row finds its sequence, and a fresh page its place in the
 // table, by bisection.  So one launch does all of it, no CTA waits for another, and none reads what another writes: a row in a
-// fresh page takes the page from the list and not from the table.  Bound by the chain of loads (lengths, then list or table): 3.5 us for a
-// step of 256 sequences and for 48 prompts of 20000 tokens, a launch included; the scan is 256 sequences a round.
+// fresh page takes the page from the list and not from the table.  Bound by the chain of loads (lengths, then list or table): 3.3 us for a
+// step of 256 sequences, 3.1 for 48 prompts of 20000 tokens, in a graph of calls; the scan is 256 sequences a round.
 constexpr int kMapThreads = 256;
 constexpr int kMapMaxSeqs = 4096;
 
@@ -150,8 +150,8 @@ kv_slot_map_kernel(const int* __restrict__ ctx_lens, const int* __restrict__ new
 // give a decode step, whose rows are runs of one, a CTA each; many rows per window keep a prompt, whose runs are 16 long, from
 // launching CTAs that find nothing to begin.
 //
-// Bound by memory for prompts, whose rows are read once (8970 rows of 4 heads of 128 in bf16, 28 MB read and written, 9.2 us; 4.2 at the copy
-// rate, the rest a launch and the chain slot -> rows -> largest magnitude -> scale -> stores), by that chain for steps (256 rows 3.5 us).
+// Bound by memory for prompts, whose rows are read once (8970 rows of 4 heads of 128 in bf16, 28 MB read and written, 8.8 us; 4.2 at the copy
+// rate, the rest a launch and the chain slot -> rows -> largest magnitude -> scale -> stores), by that chain for steps (256 rows 3.0 us).
 constexpr int kAppendWarps = 8;
 constexpr int kAppendMaxWindow = 16;  // a run that begins in a window lies within the 32 rows that a warp's lanes look at
 
@@ -329,7 +329,7 @@ static int launch_append(const void* k_new, const void* v_new, long long ks, lon
   int rc = device_sm_count(&sms);
   if (rc) return rc;
   // The fewest rows per CTA with which the grid fits the GPU at once.  us with 4, 8 and 16 CTAs per SM in its place: 8970 rows of 4 heads
-  // of 128 in bf16 9.6, 11.9, 12.8; 61 short prompts of 2 heads of 64 in fp32 3.5, 4.1, 4.1.
+  // of 128 in bf16 8.8, 11.4, 12.2; 61 short prompts of 2 heads of 64 in fp32 2.4, 3.1, 3.0.
   int window = 1;
   while (window < kAppendMaxWindow && (rows + window - 1) / window > 4 * sms) window *= 2;
   B200_CUDA(launch_overlapped(kv8_append_kernel<T, D>, dim3((rows + window - 1) / window), dim3(kAppendWarps * 32), 0, st,

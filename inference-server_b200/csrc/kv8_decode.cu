@@ -12,8 +12,9 @@
 // not finite, take their bits.)  Sums are fp32.  With |ev| <= 32 the sums p_t 2^-ev stay below 2^14 * 2^32 * tokens.
 //
 // Bound by memory: 2 D bytes per token and kv head, one scale byte per 16 D of them.  256 rows of 512 to 4096 tokens, 32 / 4 heads of
-// 128, 592 MB: 100 us at 5.9 TB/s and 7 for the join, 106 in a row of calls.  The rest is a chain of 8 to 10 us that no call is without - lengths,
-// table, the first pages, the last pages' arithmetic, partials -: one row of 777 tokens 7.1 us, 131001 tokens 31.7 us (134 MB).
+// 128, 623 MB: 109 us with the join in a graph of calls, 5.7 TB/s.  The rest is a chain that no call is without - lengths, table, the first pages, the
+// last pages' arithmetic, partials, the join -: one row of 777 tokens 6.5 us, 131001 tokens 31.6 us (134 MB).  More than 16 query heads of a kv head
+// read its pages again for every 16: 128 rows, 40 heads on one 68 us, 128 on one 162.
 //
 //   work   The pages of all rows, one row after the other, are cut into equal runs, one per CTA (kv8_ctas_per_sm), wherever
 //          that falls in a row: every CTA streams the same number of bytes without a break, whatever the rows' lengths, and there are no
@@ -68,7 +69,8 @@ __device__ __forceinline__ uint32_t transpose_8x8(uint32_t x) {
 // them cut more rows.  us for 128 rows of 512 to 4096 tokens: head_dim 128, 4 kv heads (256 rows) one 126, two 106; 2 kv heads of 8 queries
 // two 39.8, three 33.6, four 35.1, of 16 two 47.5, three 42.5; 1 kv head of 8 queries four 20.6, six 19.5, of 16 four 31.5, five 31.0.
 // head_dim 64, 4 kv heads of 8 two 36.6, three 34.1, of 16 two 40.1, three 39.0; 2 kv heads of 8 four 22.5, five 21.1, of 16 three 27.7,
-// four 24.2; 1 kv head of 8 four 17.0, six 15.5, eight 16.1, of 16 five 21.9, six 19.9.
+// four 24.2; 1 kv head of 8 four 17.0, six 15.5, eight 16.1, of 16 five 21.9, six 19.9.  (With one power of two for the queries of a kv head; one for
+// each query head makes those of 16 one or two percent longer.)
 constexpr int kv8_ctas_per_sm(int head_dim, int hkv, int nt) {
   if (head_dim == 64) return hkv == 1 ? 6 : hkv == 2 ? (nt == 1 ? 5 : 4) : 3;
   return hkv == 1 ? (nt == 1 ? 6 : 5) : hkv == 2 ? 3 : hkv == 4 ? 2 : 1;

@@ -32,8 +32,10 @@
 // Bound by the softmax: a key tile of a CTA with two tiles of rows takes about 3650 cycles, in which each scheduler issues 2000 instructions of its
 // three busy warps, the special-function units need 2048 for the exponentials and the tensor core is busy for 1024.  Dependent steps
 // (scores, maximum, exponentials, weights) leave the rest; halves of 64 keys by turns, the next one fetched meanwhile, made the steps more
-// and not shorter (359 us), and so did a quarter of the exponentials by a polynomial (271).  32 / 4 heads of 128: 2048 tokens 50 us, 1024
-// behind 14336 231 us (1.08 PFLOP/s; 202 over 16-bit pools, whose values need no conversion), 17 behind 14001 (64 / 4 heads) 27 us.
+// and not shorter (359 us), and so did a quarter of the exponentials by a polynomial (271).  32 / 4 heads of 128, in graphs of calls: 2048 tokens 50
+// to 53 us, 1024 behind 14336 233 to 249 us by the clock (1.07 to 1.00 PFLOP/s; 202 over 16-bit pools, whose values need no conversion), 17 behind
+// 14001 (64 / 4 heads) 27 us.  Heads of 64 have half the products for the same exponentials: 2048 tokens 26 us with 16 / 2 heads, 1024 behind
+// 14336 127 us with 16 / 2 and 221 with 32 / 4, where exponentials alone are 54 and 108.
 //
 // Every mbarrier wait is bounded; a wait that runs out records kErrDevWaitTimeout and the thread stops waiting but keeps the loop
 // structure, so the kernel ends.
@@ -679,6 +681,10 @@ static int kv8_prefill_plan(int num_tokens, int first_pos, int hq, int hkv, Kv8P
   int sms = 0;
   const int rc = device_sm_count(&sms);
   if (rc) return rc;
+  // The 16-bit kernel's rule, whose tile costs are not quite those here.  us with its choice, all single tiles, all pairs; 32 / 4 heads of 128:
+  // 2048 tokens 50, 64, 51; 1500 behind 100 36, 45, 36; 1024 25.4, 23.9, 25.4; 600 16.6, 16.6, 19.3; 1024 behind 14336 233, 285, 233; 1500 behind
+  // 14001 353, 417, 436; 300 behind 3000 36.1, 36.0, 37.8.  64 / 4: 512 behind 4096 79, 90, 79.  8 / 8: 700 behind 900 19.6, 19.6, 26.5.  32 / 4 of
+  // 64: 2048 41, 52, 41; 16 / 2: 2048 26.6, 26.5, 35.1; 2048 behind 2048 63.7, 58.7, 63.7; 1024 behind 14336 126.5, 126.2, 122.0.
   p->pairs = b200_paged_attn_prefill_pairs(num_tokens, first_pos, hq, hkv, 0, sms, nullptr);
   if (p->pairs < 0) return p->pairs;
   const int qt = kTcRows / (hq / hkv), key_tiles = (first_pos + num_tokens - 1) / kTcKeys + 1;
@@ -686,7 +692,9 @@ static int kv8_prefill_plan(int num_tokens, int first_pos, int hq, int hkv, Kv8P
   const long long all = static_cast<long long>(p->ctas) * hkv;
   // As many parts as SMs are there for, down to one key tile: us with parts of at least 1, 2, 4, 8 key tiles, a token behind 600 (32 / 4
   // heads of 128) 9.3, 10.3, 11.4, 12.2, behind 3000 10.2, 10.3, 12.4, 16.5; 64 tokens behind 2000 (8 / 2 of 64) 11.4, 12.3, 13.4, 15.4;
-  // 128 behind 1100 (8 / 1 of 128) 15.5, 14.4, 17.5, 17.2.
+  // 128 behind 1100 (8 / 1 of 128) 15.5, 14.4, 17.5, 17.2.  Where CTAs of pairs are 60 to 70 % of the SMs, three or four parts may gain: 700 behind
+  // 8000 (32 / 4 of 128) 141 in one, 160, 126, 144 in two, three, four; 400 behind 12000 (64 / 4) 196, 216, 221, 190; but 1024 behind 14336 245, 272,
+  // 291, 296, 512 behind 4096 (64 / 4) 79, 108, 126, 133.
   const int want = static_cast<int>(std::max(1ll, std::min<long long>(sms / all, key_tiles)));
   p->split_tiles = (key_tiles + want - 1) / want;
   p->splits = (key_tiles + p->split_tiles - 1) / p->split_tiles;
