@@ -251,7 +251,8 @@ int b200_kv_append(const void* k_new, const void* v_new, void* k_pool, void* v_p
  *   workspace     b200_kv8_attn_workspace_bytes bytes, 16-byte aligned, starting with the status word; calls that share it must not overlap
  *   split_tokens  tokens of a run at least, a multiple of 16; 0: the library's choice; the same for both calls
  * A weight times its page's value scale is rounded to 11 bits, but to no finer a step than 2^-30 of the row's largest such product: next to a
- * page whose scale is 2^20 times larger, values lose precision.  A row without tokens is zero.  Pages behind a row's last token are not read,
+ * page whose scale is 2^20 times larger, values lose precision.  A query with an infinity or NaN makes its own head's output NaN and no other.
+ * A row without tokens is zero.  Pages behind a row's last token are not read,
  * and what the last page holds behind it does not matter, NaN included.
  *
  * b200_kv8_attn_prefill: causal attention of num_tokens consecutive tokens of one sequence, at positions first_position .., whose keys and
